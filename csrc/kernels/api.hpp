@@ -6,9 +6,12 @@
 #include <cuda_runtime.h>
 
 #include <functional>
+#include <vector>
 
+#include <deep_ep/kernels/embedding_args.hpp>
 #include <deep_ep/kernels/ep_args.hpp>
 #include <deep_ep/kernels/ep_layout_args.hpp>
+#include <deep_ep/kernels/grad_norm_args.hpp>
 #include <deep_ep/kernels/grouped_gemm_args.hpp>
 #include <deep_ep/kernels/misc_args.hpp>
 
@@ -77,6 +80,28 @@ void row_quant_ue8m0(const void* x, void* q, void* sf, int64_t rows, int cols, c
 void swiglu_quant_ue8m0(const void* h, const float* row_scale, void* act, void* q, void* sf, int64_t rows, int inter,
                         cudaStream_t stream);
 void block_quant_ue8m0(const void* w, void* q, void* sf, void* qt, void* sft, int64_t rows, int cols, int n, cudaStream_t stream);
+
+// Scaled rows of an embedding table, and the gradient of that: `embedding_sort` orders the token positions by id (stable) in
+// `workspace` (`embedding_sort_workspace_ints` ints) and says where the sorted ids and positions lie; `embedding_grad` sums the
+// gradient rows over that order (`args.chunk` from `embedding_grad_chunk`).
+void embedding_lookup(const kernels::EmbLookupArgs& args, kernels::EmbType type, cudaStream_t stream);
+int64_t embedding_sort_workspace_ints(int num_tokens);
+void embedding_sort(kernels::EmbSortArgs args, int* workspace, const int** ids, const int** order, cudaStream_t stream);
+int embedding_grad_chunk(int num_tokens);
+void embedding_grad(const kernels::EmbGradArgs& args, kernels::EmbType in, kernels::EmbType out, cudaStream_t stream);
+
+// Gradient norm and clipping over lists of dense tensors. `grad_square_sums` fills at most `grad_norm_max_sums` slots and
+// returns how many; the finish and clip kernels add them up.
+struct GradTensor {
+    const void* in;
+    void* out;
+    int64_t numel;            // > 0
+    kernels::GradType in_type, out_type;
+};
+int grad_norm_max_sums(int num_tensors);
+int grad_square_sums(const std::vector<GradTensor>& tensors, double* partial, cudaStream_t stream);
+void grad_norm_finish(const kernels::GradClipArgs& args, cudaStream_t stream);
+void grad_clip(const std::vector<GradTensor>& tensors, kernels::GradClipArgs args, cudaStream_t stream);
 
 // Test hook: a one-warp kernel that waits (bounded) for a flag nobody sets and records the status.
 void bounded_wait_probe(layout::CommonSignals* cs, layout::HostStatus* host_status, long long timeout_ns,

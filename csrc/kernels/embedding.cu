@@ -1,0 +1,166 @@
+// Launchers of the embedding kernels: vector widths by alignment, grids by size, the passes of the sort.
+#include <algorithm>
+#include <bit>
+
+#include <deep_ep/common/exception.hpp>
+#include <deep_ep/kernels/embedding.cuh>
+
+#include "api.hpp"
+
+namespace deep_ep::launch {
+
+using namespace kernels;
+
+namespace {
+
+bool aligned(const void* p, int64_t row_bytes, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 and row_bytes % bytes == 0; }
+
+template <typename In, typename Out, int kElems, int kUnroll>
+void launch_lookup(EmbLookupArgs a, cudaStream_t stream) {
+    const int64_t slices = math::ceil_div(a.hidden / kElems, 32 * kUnroll);
+    // item numbers are 32-bit in the kernel: very long inputs go in pieces
+    const int64_t most = std::max<int64_t>(1, ((int64_t(1) << 31) - 8) / slices);
+    for (int64_t done = 0, total = a.num_tokens; done < total; done += most) {
+        EmbLookupArgs piece = a;
+        piece.num_tokens = std::min(most, total - done);
+        piece.idx = static_cast<const uint8_t*>(a.idx) + done * (a.idx64 ? 8 : 4);
+        piece.out = static_cast<Out*>(a.out) + done * a.hidden;
+        const auto blocks = static_cast<unsigned>((piece.num_tokens * slices + 7) / 8);
+        embedding_lookup_kernel<In, Out, kElems, kUnroll><<<blocks, 256, 0, stream>>>(piece);
+        CUDA_CHECK(cudaGetLastError());
+    }
+}
+
+// Widest access that both the table's rows and the result's allow: 16 bytes, 4 bytes, one element.
+template <typename In, typename Out>
+void choose_lookup(const EmbLookupArgs& a, cudaStream_t stream) {
+    constexpr int kWide = 16 / sizeof(In), kHalf = 4 / sizeof(In);
+    const auto fits = [&](int elems) {
+        return a.hidden % elems == 0 and aligned(a.table, a.table_stride * sizeof(In), elems * int(sizeof(In))) and
+               aligned(a.out, int64_t(a.hidden) * sizeof(Out), std::min(16, elems * int(sizeof(Out))));
+    };
+    if (fits(kWide)) {
+        // few rows: one access per lane and item, so that a row is spread over more SMs
+        const bool small = a.num_tokens * math::ceil_div(a.hidden / kWide, 32) < 148 * 64;
+        if (small) launch_lookup<In, Out, kWide, 1>(a, stream);
+        else launch_lookup<In, Out, kWide, 4>(a, stream);
+    } else if (kHalf > 1 and fits(kHalf)) {
+        launch_lookup<In, Out, kHalf, 4>(a, stream);
+    } else {
+        launch_lookup<In, Out, 1, 4>(a, stream);
+    }
+}
+
+}  // namespace
+
+void embedding_lookup(const EmbLookupArgs& args, EmbType type, cudaStream_t stream) {
+    if (args.num_tokens == 0 or args.hidden == 0) return;
+    switch (type) {
+        case EmbType::kBF16: return choose_lookup<__nv_bfloat16, __nv_bfloat16>(args, stream);
+        case EmbType::kFP16: return choose_lookup<__half, __half>(args, stream);
+        case EmbType::kFP32: return choose_lookup<float, float>(args, stream);
+        case EmbType::kE4M3: return choose_lookup<__nv_fp8_e4m3, __nv_bfloat16>(args, stream);
+    }
+}
+
+// ---------------------------------------------------------------------------------------- sort
+namespace {
+
+constexpr int kSoloKeys = 8192;        // one CTA sorts up to this many keys, see `embedding_sort`
+constexpr int kKeysPerCta = 2048;
+
+int sort_ctas(int num_tokens) { return std::min(148, math::ceil_div(num_tokens, kKeysPerCta)); }
+
+// ids are 0 .. num_rows (num_rows = masked): as few passes of at most `most` bits as cover them, of equal width
+void choose_digits(EmbSortArgs& a, int most) {
+    const int bits = std::max(1, int(std::bit_width(static_cast<unsigned>(a.num_rows))));
+    a.num_passes = math::ceil_div(bits, most);
+    a.digit_bits = math::ceil_div(bits, a.num_passes);
+}
+
+}  // namespace
+
+int64_t embedding_sort_workspace_ints(int num_tokens) {
+    // two key and two value buffers, the counts of a pass
+    return 4ll * num_tokens + int64_t(sort_ctas(num_tokens)) * (1 << kEmbMaxDigitBits);
+}
+
+void embedding_sort(EmbSortArgs args, int* workspace, const int** ids, const int** order, cudaStream_t stream) {
+    const int n = args.num_tokens;
+    args.keys[0] = workspace, args.keys[1] = workspace + n;
+    args.vals[0] = workspace + 2ll * n, args.vals[1] = workspace + 3ll * n;
+    if (n <= kSoloKeys) {
+        choose_digits(args, 9);
+        args.keys_per_warp = std::max(32, math::align(math::ceil_div(n, kEmbSortSoloThreads / 32), 32));
+        const int bins = 1 << args.digit_bits;
+        const int smem = (kEmbSortSoloThreads / 32 + 1) * bins * 4 + 128;
+        CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_solo_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        embedding_sort_solo_kernel<<<1, kEmbSortSoloThreads, smem, stream>>>(args);
+        CUDA_CHECK(cudaGetLastError());
+    } else {
+        choose_digits(args, kEmbMaxDigitBits);
+        args.hist = workspace + 4ll * n;
+        const int ctas = sort_ctas(n), warps = kEmbSortThreads / 32, bins = 1 << args.digit_bits;
+        args.keys_per_warp = math::align(math::ceil_div(n, ctas * warps), 32);
+        const int smem = (warps + 2) * bins * 4 + 128;
+        for (args.pass = 0; args.pass < args.num_passes; ++args.pass) {
+            embedding_sort_count_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
+            embedding_sort_scatter_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
+        }
+        CUDA_CHECK(cudaGetLastError());
+    }
+    *ids = args.keys[(args.num_passes - 1) & 1], *order = args.vals[(args.num_passes - 1) & 1];
+}
+
+// ---------------------------------------------------------------------------------------- gradient
+int embedding_grad_chunk(int num_tokens) {
+    // 32 sorted positions per chunk; longer chunks for long inputs, so that a run over all of them is joined from at most
+    // about 2048 pieces
+    int chunk = 32;
+    while (math::ceil_div(num_tokens, chunk) > 2048) chunk *= 2;
+    return chunk;
+}
+
+namespace {
+
+template <typename In, typename Out, int kElems>
+void launch_grad(const EmbGradArgs& a, cudaStream_t stream) {
+    const int64_t slices = math::ceil_div(a.hidden, 32 * kElems);
+    const int64_t sums = int64_t(a.num_chunks) * slices, fills = a.touched != nullptr ? a.num_rows : 0;
+    EP_HOST_ASSERT(sums < (int64_t(1) << 31));
+    if (sums + fills > 0) {
+        embedding_grad_kernel<In, Out, kElems><<<static_cast<unsigned>((sums + fills + 7) / 8), 256, 0, stream>>>(a);
+        CUDA_CHECK(cudaGetLastError());
+    }
+    if (a.num_chunks > 1) {
+        const dim3 grid(a.num_chunks, static_cast<unsigned>(std::min<int64_t>(slices, 4)));
+        embedding_grad_join_kernel<Out, kElems><<<grid, 256, 0, stream>>>(a);
+        CUDA_CHECK(cudaGetLastError());
+    }
+}
+
+template <typename In, typename Out>
+void choose_grad(const EmbGradArgs& a, cudaStream_t stream) {
+    constexpr int kWide = 16 / sizeof(In), kHalf = 4 / sizeof(In);
+    const auto fits = [&](int elems) {
+        return a.hidden % elems == 0 and aligned(a.dy, a.dy_stride * sizeof(In), elems * int(sizeof(In))) and
+               aligned(a.out, a.out_stride * sizeof(Out), std::min(16, elems * int(sizeof(Out))));
+    };
+    if (fits(kWide)) launch_grad<In, Out, kWide>(a, stream);
+    else if (kHalf > 1 and fits(kHalf)) launch_grad<In, Out, kHalf>(a, stream);
+    else launch_grad<In, Out, 1>(a, stream);
+}
+
+}  // namespace
+
+void embedding_grad(const EmbGradArgs& a, EmbType in, EmbType out, cudaStream_t stream) {
+    if (a.hidden == 0) return;
+    if (in == EmbType::kBF16 and out == EmbType::kBF16) return choose_grad<__nv_bfloat16, __nv_bfloat16>(a, stream);
+    if (in == EmbType::kBF16 and out == EmbType::kFP32) return choose_grad<__nv_bfloat16, float>(a, stream);
+    if (in == EmbType::kFP16 and out == EmbType::kFP16) return choose_grad<__half, __half>(a, stream);
+    if (in == EmbType::kFP16 and out == EmbType::kFP32) return choose_grad<__half, float>(a, stream);
+    if (in == EmbType::kFP32 and out == EmbType::kFP32) return choose_grad<float, float>(a, stream);
+    EP_HOST_UNREACHABLE("gradient types");
+}
+
+}  // namespace deep_ep::launch

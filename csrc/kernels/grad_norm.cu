@@ -1,0 +1,83 @@
+// Launchers of the gradient-norm kernels: the tensor list is cut into tables that fit a kernel's parameters.
+#include <algorithm>
+#include <vector>
+
+#include <deep_ep/common/exception.hpp>
+#include <deep_ep/kernels/grad_norm.cuh>
+
+#include "api.hpp"
+
+namespace deep_ep::launch {
+
+using namespace kernels;
+
+namespace {
+
+constexpr int kFewTensors = 64;
+
+template <int kTensors>
+int fill_table(GradTable<kTensors>& table, const GradTensor* tensors, int count) {
+    int chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        table.in[i] = tensors[i].in, table.out[i] = tensors[i].out, table.numel[i] = tensors[i].numel;
+        table.in_type[i] = static_cast<uint8_t>(tensors[i].in_type), table.out_type[i] = static_cast<uint8_t>(tensors[i].out_type);
+        table.first_chunk[i] = chunks;
+        chunks += static_cast<int>(math::ceil_div<int64_t>(tensors[i].numel, kGradChunk));
+    }
+    table.first_chunk[count] = chunks, table.num_tensors = count;
+    return chunks;
+}
+
+// A launch that may begin while the one before it in the stream still runs: the kernel waits for it where it needs its results.
+template <typename... Params, typename... Args>
+void launch_early(void (*kernel)(Params...), int grid, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid), config.blockDim = dim3(kGradThreads), config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr, config.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
+template <int kTensors>
+int square_sum(const GradTensor* tensors, int count, double* partial, cudaStream_t stream) {
+    GradTable<kTensors> table;
+    const int grid = std::min(fill_table(table, tensors, count), kGradCtas);
+    grad_square_sum_kernel<kTensors><<<grid, kGradThreads, 0, stream>>>(table, GradNormArgs{partial});
+    CUDA_CHECK(cudaGetLastError());
+    return grid;
+}
+
+template <int kTensors>
+void clip(const GradTensor* tensors, int count, const GradClipArgs& args, cudaStream_t stream) {
+    GradTable<kTensors> table;
+    const int grid = std::min(fill_table(table, tensors, count), kGradCtas);
+    launch_early(grad_clip_kernel<kTensors>, grid, stream, table, args);
+}
+
+}  // namespace
+
+int grad_norm_max_sums(int num_tensors) { return math::ceil_div(num_tensors, kGradMaxTensors) * kGradCtas; }
+
+int grad_square_sums(const std::vector<GradTensor>& tensors, double* partial, cudaStream_t stream) {
+    int sums = 0;
+    for (size_t i = 0; i < tensors.size(); i += kGradMaxTensors) {
+        const int count = static_cast<int>(std::min<size_t>(kGradMaxTensors, tensors.size() - i));
+        sums += count <= kFewTensors ? square_sum<kFewTensors>(tensors.data() + i, count, partial + sums, stream)
+                                     : square_sum<kGradMaxTensors>(tensors.data() + i, count, partial + sums, stream);
+    }
+    return sums;
+}
+
+void grad_norm_finish(const GradClipArgs& args, cudaStream_t stream) { launch_early(grad_norm_finish_kernel, 1, stream, args); }
+
+void grad_clip(const std::vector<GradTensor>& tensors, GradClipArgs args, cudaStream_t stream) {
+    for (size_t i = 0; i < tensors.size(); i += kGradMaxTensors) {
+        const int count = static_cast<int>(std::min<size_t>(kGradMaxTensors, tensors.size() - i));
+        if (count <= kFewTensors) clip<kFewTensors>(tensors.data() + i, count, args, stream);
+        else clip<kGradMaxTensors>(tensors.data() + i, count, args, stream);
+        args.norm = nullptr;
+    }
+}
+
+}  // namespace deep_ep::launch

@@ -1,0 +1,112 @@
+// Torch-facing entry points of the embedding kernels: argument checks, outputs, workspaces.
+#pragma once
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <limits>
+#include <optional>
+
+#include <deep_ep/common/exception.hpp>
+
+#include "../kernels/api.hpp"
+
+namespace deep_ep::ops {
+
+inline kernels::EmbType embedding_type(const torch::Tensor& t) {
+    switch (t.scalar_type()) {
+        case torch::kBFloat16: return kernels::EmbType::kBF16;
+        case torch::kFloat16: return kernels::EmbType::kFP16;
+        case torch::kFloat32: return kernels::EmbType::kFP32;
+        case torch::kFloat8_e4m3fn: return kernels::EmbType::kE4M3;
+        default: EP_HOST_UNREACHABLE("embedding tables are bf16, fp16, fp32 or e4m3");
+    }
+}
+
+// A matrix whose columns are contiguous; rows may lie further apart.
+inline void check_rows(const torch::Tensor& t) {
+    EP_HOST_ASSERT_MSG(t.is_cuda() and t.dim() == 2 and (t.size(1) <= 1 or t.stride(1) == 1) and t.stride(0) >= 0,
+                       "a CUDA matrix with contiguous columns is needed");
+}
+
+inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
+    EP_HOST_ASSERT_MSG(idx.is_contiguous() and (idx.scalar_type() == torch::kInt64 or idx.scalar_type() == torch::kInt32),
+                       "indices are contiguous int64 or int32");
+    EP_HOST_ASSERT_MSG(idx.device() == with.device(), "all tensors of a call lie on one device");
+}
+
+// [num_tokens, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
+inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale,
+                                      const std::optional<torch::Tensor>& table_sf) {
+    check_rows(table), check_ids(idx, table);
+    const auto type = embedding_type(table);
+    EP_HOST_ASSERT_MSG((type == kernels::EmbType::kE4M3) == table_sf.has_value(), "an e4m3 table comes with its scales, another without");
+    EP_HOST_ASSERT(table.size(1) <= std::numeric_limits<int>::max());
+    const c10::cuda::CUDAGuard guard(table.device());
+    kernels::EmbLookupArgs a = {};
+    a.table = table.data_ptr(), a.table_stride = table.stride(0);
+    a.idx = idx.data_ptr(), a.idx64 = idx.scalar_type() == torch::kInt64;
+    a.num_tokens = idx.numel(), a.num_rows = table.size(0), a.hidden = static_cast<int>(table.size(1));
+    a.scale = static_cast<float>(scale);
+    if (table_sf.has_value()) {
+        check_rows(*table_sf);
+        EP_HOST_ASSERT_MSG(a.hidden % 128 == 0 and table_sf->scalar_type() == torch::kFloat32 and table_sf->size(0) == a.num_rows and
+                           table_sf->size(1) == a.hidden / 128 and table_sf->device() == table.device(),
+                           "scales are fp32 [rows, hidden / 128], hidden a multiple of 128");
+        a.table_sf = table_sf->data_ptr<float>(), a.sf_stride = table_sf->stride(0);
+    }
+    auto out = torch::empty({a.num_tokens, a.hidden}, table.options().dtype(
+        type == kernels::EmbType::kE4M3 ? torch::kBFloat16 : table.scalar_type()));
+    a.out = out.data_ptr();
+    launch::embedding_lookup(a, type, c10::cuda::getCurrentCUDAStream());
+    return out;
+}
+
+// out[v] (+)= scale * sum of dy[t] over idx[t] == v; `out` fp32 or of dy's type, `accumulate` only for fp32
+inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, double scale, const torch::Tensor& out, bool accumulate) {
+    check_rows(dy), check_rows(out), check_ids(idx, dy);
+    EP_HOST_ASSERT_MSG(out.device() == dy.device(), "all tensors of a call lie on one device");
+    EP_HOST_ASSERT_MSG(dy.size(0) == idx.numel() and dy.size(1) == out.size(1), "dy is [number of indices, hidden], out [rows, hidden]");
+    EP_HOST_ASSERT_MSG(dy.scalar_type() == out.scalar_type() or out.scalar_type() == torch::kFloat32, "out is fp32 or of dy's type");
+    EP_HOST_ASSERT_MSG(not accumulate or out.scalar_type() == torch::kFloat32, "only an fp32 gradient is accumulated into");
+    EP_HOST_ASSERT_MSG(out.size(0) <= 1 or out.stride(0) >= out.size(1), "rows of out overlap");
+    constexpr int64_t kMost = std::numeric_limits<int>::max() / 2;
+    EP_HOST_ASSERT_MSG(idx.numel() <= kMost and out.size(0) <= kMost and out.size(1) <= kMost, "sizes above 2^30");
+    const auto in_type = embedding_type(dy), out_type = embedding_type(out);
+    EP_HOST_ASSERT(in_type != kernels::EmbType::kE4M3);
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    const int num_tokens = static_cast<int>(idx.numel()), num_rows = static_cast<int>(out.size(0)), hidden = static_cast<int>(out.size(1));
+    if (num_rows == 0 or hidden == 0) return;
+
+    kernels::EmbGradArgs g = {};
+    g.dy = dy.data_ptr(), g.dy_stride = dy.stride(0);
+    g.num_tokens = num_tokens, g.num_rows = num_rows, g.hidden = hidden, g.scale = static_cast<float>(scale);
+    g.out = out.data_ptr(), g.out_stride = out.stride(0), g.accumulate = accumulate;
+    if (num_tokens == 0) {
+        if (not accumulate) out.zero_();
+        return;
+    }
+    g.chunk = launch::embedding_grad_chunk(num_tokens), g.num_chunks = (num_tokens + g.chunk - 1) / g.chunk;
+    // scratch of this call, from the caching allocator: freed in stream order, private to a graph that is being captured
+    const int64_t bitmap_ints = accumulate ? 0 : (num_rows + 31) / 32;
+    const auto ints = torch::empty({launch::embedding_sort_workspace_ints(num_tokens) + bitmap_ints}, idx.options().dtype(torch::kInt32));
+    const auto partial = torch::empty({g.num_chunks > 1 ? 2ll * g.num_chunks * hidden : 0}, dy.options().dtype(torch::kFloat32));
+    g.partial = partial.data_ptr<float>();
+    kernels::EmbSortArgs s = {};
+    s.idx = idx.data_ptr(), s.idx64 = idx.scalar_type() == torch::kInt64, s.num_tokens = num_tokens, s.num_rows = num_rows;
+    // a sum is written over the whole row, so only rows without a token need zeros
+    s.touched = accumulate ? nullptr : reinterpret_cast<uint32_t*>(ints.data_ptr<int>() + ints.numel() - bitmap_ints);
+    launch::embedding_sort(s, ints.data_ptr<int>(), &g.ids, &g.order, stream);
+    g.touched = s.touched;
+    launch::embedding_grad(g, in_type, out_type, stream);
+}
+
+inline void register_embedding(pybind11::module_& m) {
+    namespace py = pybind11;
+    m.def("embedding_lookup", &embedding_lookup, py::arg("table"), py::arg("idx"), py::arg("scale") = 1.0, py::arg("table_sf") = py::none());
+    m.def("embedding_grad", &embedding_grad, py::arg("dy"), py::arg("idx"), py::arg("scale"), py::arg("out"), py::arg("accumulate") = false);
+}
+
+}  // namespace deep_ep::ops

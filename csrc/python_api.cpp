@@ -10,6 +10,8 @@
 #include "buffers/pp.hpp"
 #include "comm/barrier.hpp"
 #include "comm/stream.hpp"
+#include "ops/embedding.hpp"
+#include "ops/grad_norm.hpp"
 #include "runtime/device.hpp"
 #include "runtime/jit.hpp"
 #include "runtime/specialize.hpp"
@@ -368,6 +370,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("block_quant_ue8m0", &block_quant_ue8m0, py::arg("w"), py::arg("transposed") = false);
     m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, py::arg("a"), py::arg("b"), py::arg("d"), py::arg("psum"), py::arg("count"),
           py::arg("num_sms") = 0, py::arg("accumulate") = true, py::arg("use_pairs") = false);
+
+    ops::register_embedding(m);
+    ops::register_grad_norm(m);
 
     py::class_<BufferBase, std::shared_ptr<BufferBase>>(m, "BufferBase")
         .def_readonly("main_context", &BufferBase::main_context)

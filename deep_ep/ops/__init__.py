@@ -6,5 +6,7 @@
 * `quant`, `jit`: run-time specialised kernels (per-token FP8 quantiser compiled for the hidden size in use).
 * `layout`: routing layout of a batch (`get_dispatch_layout`).
 * `dense`: the router's and the shared expert's dense products on the same tcgen05 kernels (one group).
+* `embedding`: embedding lookup with scaling (bf16 / fp16 / fp32 tables, e4m3 entries with 1x128 scales) and its gradient.
+* `grad_norm`: global gradient norm over many tensors and ranks, and clipping by it.
 """
-__all__ = ['dense', 'fp8_training', 'grouped_gemm', 'jit', 'layout', 'quant']
+__all__ = ['dense', 'embedding', 'fp8_training', 'grad_norm', 'grouped_gemm', 'jit', 'layout', 'quant']
