@@ -13,6 +13,7 @@
 #include <deep_ep/kernels/ep_layout_args.hpp>
 #include <deep_ep/kernels/grad_norm_args.hpp>
 #include <deep_ep/kernels/grouped_gemm_args.hpp>
+#include <deep_ep/kernels/lora_args.hpp>
 #include <deep_ep/kernels/misc_args.hpp>
 
 namespace deep_ep::launch {
@@ -102,6 +103,11 @@ int grad_norm_max_sums(int num_tensors);
 int grad_square_sums(const std::vector<GradTensor>& tensors, double* partial, cudaStream_t stream);
 void grad_norm_finish(const kernels::GradClipArgs& args, cudaStream_t stream);
 void grad_clip(const std::vector<GradTensor>& tensors, kernels::GradClipArgs args, cudaStream_t stream);
+
+// Adapters beside a shared projection (see lora.cuh); the launchers choose tiles, chunks and clusters.
+void lora_shrink(kernels::LoraShrinkArgs args, const void* x, const void* a, cudaStream_t stream);
+void lora_gemm(kernels::LoraGemmArgs args, const void* x, const void* w, cudaStream_t stream);
+void lora_wgrad(kernels::LoraWgradArgs args, const void* x, cudaStream_t stream);
 
 // Test hook: a one-warp kernel that waits (bounded) for a flag nobody sets and records the status.
 void bounded_wait_probe(layout::CommonSignals* cs, layout::HostStatus* host_status, long long timeout_ns,

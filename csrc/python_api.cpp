@@ -12,6 +12,7 @@
 #include "comm/stream.hpp"
 #include "ops/embedding.hpp"
 #include "ops/grad_norm.hpp"
+#include "ops/lora.hpp"
 #include "runtime/device.hpp"
 #include "runtime/jit.hpp"
 #include "runtime/specialize.hpp"
@@ -373,6 +374,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 
     ops::register_embedding(m);
     ops::register_grad_norm(m);
+    ops::register_lora(m);
 
     py::class_<BufferBase, std::shared_ptr<BufferBase>>(m, "BufferBase")
         .def_readonly("main_context", &BufferBase::main_context)

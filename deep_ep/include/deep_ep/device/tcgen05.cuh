@@ -37,6 +37,21 @@ EP_DEVICE void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr) : "memory");
 }
 
+// 32 lanes x one 32-bit column
+EP_DEVICE uint32_t tmem_ld_32x1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+    return r;
+}
+// 32 lanes x 16 consecutive 32-bit columns
+EP_DEVICE void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+
 // ---------------------------------------------------------------- MMA
 // Instruction descriptor of kind::f16 / kind::f8f6f4: fp32 accumulation, dense, no negation.
 //   [4,6) D format (1 = F32)   [7,10) A format   [10,13) B format   [15] A major   [16] B major (0 = K, 1 = MN)
@@ -121,6 +136,11 @@ EP_DEVICE void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y,
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(ptx::smem_addr(smem_dst)), "l"(map), "r"(x), "r"(y), "r"(ptx::smem_addr(bar)) : "memory");
+}
+EP_DEVICE void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(ptx::smem_addr(smem_dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(ptx::smem_addr(bar)) : "memory");
 }
 // Tiled 2-D store of a shared-memory box to global memory, and the same as an element-wise add into global memory
 // (the element type comes from the tensor map). Tracked by the issuing thread's bulk async-group. `x * element size`

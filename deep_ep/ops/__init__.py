@@ -8,5 +8,6 @@
 * `dense`: the router's and the shared expert's dense products on the same tcgen05 kernels (one group).
 * `embedding`: embedding lookup with scaling (bf16 / fp16 / fp32 tables, e4m3 entries with 1x128 scales) and its gradient.
 * `grad_norm`: global gradient norm over many tensors and ranks, and clipping by it.
+* `lora`: low-rank adapters of many requests beside one shared projection (`dense_linear` with an adapter per row).
 """
-__all__ = ['dense', 'embedding', 'fp8_training', 'grad_norm', 'grouped_gemm', 'jit', 'layout', 'quant']
+__all__ = ['dense', 'embedding', 'fp8_training', 'grad_norm', 'grouped_gemm', 'jit', 'layout', 'lora', 'quant']
