@@ -88,7 +88,7 @@ void block_quant_ue8m0(const void* w, void* q, void* sf, void* qt, void* sft, in
 void embedding_lookup(const kernels::EmbLookupArgs& args, kernels::EmbType type, cudaStream_t stream);
 int64_t embedding_sort_workspace_ints(int num_tokens);
 void embedding_sort(kernels::EmbSortArgs args, int* workspace, const int** ids, const int** order, cudaStream_t stream);
-int embedding_grad_chunk(int num_tokens);
+int embedding_grad_chunk(int num_tokens, int hidden);
 void embedding_grad(const kernels::EmbGradArgs& args, kernels::EmbType in, kernels::EmbType out, cudaStream_t stream);
 
 // Gradient norm and clipping over lists of dense tensors. `grad_square_sums` fills at most `grad_norm_max_sums` slots and

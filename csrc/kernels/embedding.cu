@@ -34,7 +34,7 @@ void launch_lookup(EmbLookupArgs a, cudaStream_t stream) {
 // Widest access that both the table's rows and the result's allow: 16 bytes, 4 bytes, one element.
 template <typename In, typename Out>
 void choose_lookup(const EmbLookupArgs& a, cudaStream_t stream) {
-    constexpr int kWide = 16 / sizeof(In), kHalf = 4 / sizeof(In);
+    constexpr int kWide = 16 / sizeof(Out), kHalf = 4 / sizeof(Out);
     const auto fits = [&](int elems) {
         return a.hidden % elems == 0 and aligned(a.table, a.table_stride * sizeof(In), elems * int(sizeof(In))) and
                aligned(a.out, int64_t(a.hidden) * sizeof(Out), std::min(16, elems * int(sizeof(Out))));
@@ -66,7 +66,7 @@ void embedding_lookup(const EmbLookupArgs& args, EmbType type, cudaStream_t stre
 // ---------------------------------------------------------------------------------------- sort
 namespace {
 
-constexpr int kSoloKeys = 8192;        // one CTA sorts up to this many keys, see `embedding_sort`
+constexpr int kClusterKeys = 8 * kEmbClusterThreads * kEmbClusterMaxRounds;      // 65536 keys in one launch
 constexpr int kKeysPerCta = 2048;
 
 int sort_ctas(int num_tokens) { return std::min(148, math::ceil_div(num_tokens, kKeysPerCta)); }
@@ -75,68 +75,91 @@ int sort_ctas(int num_tokens) { return std::min(148, math::ceil_div(num_tokens, 
 void choose_digits(EmbSortArgs& a, int most) {
     const int bits = std::max(1, int(std::bit_width(static_cast<unsigned>(a.num_rows))));
     a.num_passes = math::ceil_div(bits, most);
-    a.digit_bits = math::ceil_div(bits, a.num_passes);
+    a.digit_bits = std::max(1, math::ceil_div(bits, a.num_passes));
+}
+
+template <int kRounds>
+void sort_in_cluster(const EmbSortArgs& args, cudaStream_t stream) {
+    constexpr int kKeys = kEmbClusterThreads * kRounds;
+    const int bins = 1 << args.digit_bits;
+    int cluster = 1;
+    while (cluster * kKeys < args.num_tokens) cluster *= 2;
+    const int smem = 4 * kKeys * 4 + 3 * bins * 4 + (kEmbClusterThreads / 32) * bins * 2;
+    CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_cluster_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(cluster), config.blockDim = dim3(kEmbClusterThreads);
+    config.dynamicSmemBytes = smem, config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr, config.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&config, embedding_sort_cluster_kernel<kRounds>, args));
 }
 
 }  // namespace
 
 int64_t embedding_sort_workspace_ints(int num_tokens) {
     // two key and two value buffers, the counts of a pass
-    return 4ll * num_tokens + int64_t(sort_ctas(num_tokens)) * (1 << kEmbMaxDigitBits);
+    return num_tokens <= kClusterKeys ? 2ll * num_tokens : 4ll * num_tokens + int64_t(sort_ctas(num_tokens)) * (1 << kEmbMaxDigitBits);
 }
 
 void embedding_sort(EmbSortArgs args, int* workspace, const int** ids, const int** order, cudaStream_t stream) {
     const int n = args.num_tokens;
+    if (n <= kClusterKeys) {
+        choose_digits(args, kEmbClusterDigitBits);
+        args.keys[0] = workspace, args.vals[0] = workspace + n;
+        // as few keys per thread as eight CTAs allow
+        if (n <= 8 * kEmbClusterThreads) sort_in_cluster<1>(args, stream);
+        else if (n <= 16 * kEmbClusterThreads) sort_in_cluster<2>(args, stream);
+        else if (n <= 32 * kEmbClusterThreads) sort_in_cluster<4>(args, stream);
+        else sort_in_cluster<8>(args, stream);
+        *ids = args.keys[0], *order = args.vals[0];
+        return;
+    }
+    choose_digits(args, kEmbMaxDigitBits);
     args.keys[0] = workspace, args.keys[1] = workspace + n;
     args.vals[0] = workspace + 2ll * n, args.vals[1] = workspace + 3ll * n;
-    if (n <= kSoloKeys) {
-        choose_digits(args, 9);
-        args.keys_per_warp = std::max(32, math::align(math::ceil_div(n, kEmbSortSoloThreads / 32), 32));
-        const int bins = 1 << args.digit_bits;
-        const int smem = (kEmbSortSoloThreads / 32 + 1) * bins * 4 + 128;
-        CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_solo_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        embedding_sort_solo_kernel<<<1, kEmbSortSoloThreads, smem, stream>>>(args);
-        CUDA_CHECK(cudaGetLastError());
-    } else {
-        choose_digits(args, kEmbMaxDigitBits);
-        args.hist = workspace + 4ll * n;
-        const int ctas = sort_ctas(n), warps = kEmbSortThreads / 32, bins = 1 << args.digit_bits;
-        args.keys_per_warp = math::align(math::ceil_div(n, ctas * warps), 32);
-        const int smem = (warps + 2) * bins * 4 + 128;
-        for (args.pass = 0; args.pass < args.num_passes; ++args.pass) {
-            embedding_sort_count_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
-            embedding_sort_scatter_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
-        }
-        CUDA_CHECK(cudaGetLastError());
+    args.hist = workspace + 4ll * n;
+    const int ctas = sort_ctas(n), warps = kEmbSortThreads / 32, bins = 1 << args.digit_bits;
+    args.keys_per_warp = math::align(math::ceil_div(n, ctas * warps), 32);
+    const int smem = (warps + 2) * bins * 4 + 128;
+    for (args.pass = 0; args.pass < args.num_passes; ++args.pass) {
+        embedding_sort_count_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
+        embedding_sort_scatter_kernel<<<ctas, kEmbSortThreads, smem, stream>>>(args);
     }
+    CUDA_CHECK(cudaGetLastError());
     *ids = args.keys[(args.num_passes - 1) & 1], *order = args.vals[(args.num_passes - 1) & 1];
 }
 
 // ---------------------------------------------------------------------------------------- gradient
-int embedding_grad_chunk(int num_tokens) {
-    // 32 sorted positions per chunk; longer chunks for long inputs, so that a run over all of them is joined from at most
-    // about 2048 pieces
+int embedding_grad_chunk(int num_tokens, int hidden) {
+    // 32 sorted positions per chunk; fewer while that leaves SMs without warps; more for long inputs, so that a run over all of
+    // them is joined from at most 2048 pieces
     int chunk = 32;
+    while (chunk > 8 and int64_t(math::ceil_div(num_tokens, chunk)) * math::ceil_div(hidden, 128) < 148 * 16) chunk /= 2;
     while (math::ceil_div(num_tokens, chunk) > 2048) chunk *= 2;
     return chunk;
 }
 
 namespace {
 
-template <typename In, typename Out, int kElems>
+// A launch that may be set up while the kernel before it in the stream still runs; it waits for that one's results itself.
+void launch_early(void (*kernel)(EmbGradArgs), unsigned grid, cudaStream_t stream, const EmbGradArgs& args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid), config.blockDim = dim3(256), config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr, config.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args));
+}
+
+template <typename In, typename Out, int kElems, int kPacks, bool kAccumulate>
 void launch_grad(const EmbGradArgs& a, cudaStream_t stream) {
-    const int64_t slices = math::ceil_div(a.hidden, 32 * kElems);
+    const int64_t slices = math::ceil_div(a.hidden, 32 * kElems * kPacks);
     const int64_t sums = int64_t(a.num_chunks) * slices, fills = a.touched != nullptr ? a.num_rows : 0;
     EP_HOST_ASSERT(sums < (int64_t(1) << 31));
-    if (sums + fills > 0) {
-        embedding_grad_kernel<In, Out, kElems><<<static_cast<unsigned>((sums + fills + 7) / 8), 256, 0, stream>>>(a);
-        CUDA_CHECK(cudaGetLastError());
-    }
-    if (a.num_chunks > 1) {
-        const dim3 grid(a.num_chunks, static_cast<unsigned>(std::min<int64_t>(slices, 4)));
-        embedding_grad_join_kernel<Out, kElems><<<grid, 256, 0, stream>>>(a);
-        CUDA_CHECK(cudaGetLastError());
-    }
+    launch_early(embedding_grad_kernel<In, Out, kElems, kPacks, kAccumulate>, static_cast<unsigned>((sums + fills + 7) / 8), stream, a);
+    if (a.num_chunks > 1) launch_early(embedding_grad_join_kernel<Out, kElems, kAccumulate>, 148 * 6, stream, a);
 }
 
 template <typename In, typename Out>
@@ -146,9 +169,15 @@ void choose_grad(const EmbGradArgs& a, cudaStream_t stream) {
         return a.hidden % elems == 0 and aligned(a.dy, a.dy_stride * sizeof(In), elems * int(sizeof(In))) and
                aligned(a.out, a.out_stride * sizeof(Out), std::min(16, elems * int(sizeof(Out))));
     };
-    if (fits(kWide)) launch_grad<In, Out, kWide>(a, stream);
-    else if (kHalf > 1 and fits(kHalf)) launch_grad<In, Out, kHalf>(a, stream);
-    else launch_grad<In, Out, 1>(a, stream);
+    const auto go = [&]<int kElems, int kPacks>() {
+        if constexpr (sizeof(Out) == 4) {
+            if (a.accumulate) return launch_grad<In, Out, kElems, kPacks, true>(a, stream);
+        }
+        launch_grad<In, Out, kElems, kPacks, false>(a, stream);
+    };
+    if (fits(kWide)) go.template operator()<kWide, 1>();
+    else if (kHalf > 1 and fits(kHalf)) go.template operator()<kHalf, 2>();
+    else go.template operator()<1, 4>();
 }
 
 }  // namespace

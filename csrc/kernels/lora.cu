@@ -55,6 +55,12 @@ void launch_clusters(void (*kernel)(Params...), int64_t grid, int threads, int c
 }
 
 constexpr int64_t kRingBytes = 192 * 1024;
+// Up to this many products of x A^T, the kernel without tensor cores is ahead: its time is that of reading rows * rank * k
+// elements of A from L2, the other's starts at what setting up a tile costs.
+constexpr int64_t kFewProducts = int64_t(1) << 24;
+// Up to this many elements of t, the low-rank term is computed beside the shared product's stream of W instead of on the
+// tensor cores.
+constexpr int64_t kFewTerms = 4096;
 
 }  // namespace
 
@@ -62,6 +68,14 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
     const int rows = args.rows.num_rows, rank = args.rows.rank;
+    if (rows <= kLoraTileRows and int64_t(rows) * rank * args.k <= kFewProducts) {
+        // (an SM divides its memory between cache and shared memory by the kernels on it: with the default, the next kernel's
+        // CTAs, which need all of the latter, could not join before these have left)
+        CUDA_CHECK(cudaFuncSetAttribute(lora_shrink_rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+        lora_shrink_rows_kernel<<<rows * (rank / 4), 512, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), args);
+        CUDA_CHECK(cudaGetLastError());
+        return;
+    }
     const int rp = math::align(rank, args.mn_major ? 64 : 16);
     const int64_t tiles = math::ceil_div(rows, kLoraTileRows), sms = device_sms();
     const int distinct = std::min({args.rows.num_adapters, rows, kLoraTileRows});        // at most, per tile
@@ -72,10 +86,8 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
     args.cluster = choose_cluster(tiles, blocks, 4, static_cast<int>(sms));
     args.chunk = static_cast<int>(std::clamp<int64_t>(math::ceil_div<int64_t>(int64_t(distinct) * tiles * args.cluster, sms), 1, most));
     args.num_chunks = math::ceil_div(distinct, args.chunk);
-    args.stage_bytes = kLoraTileRows * kLoraBlockK * 2 + args.chunk * rp * 128;
-    args.num_stages = static_cast<int>(std::min<int64_t>(8, kRingBytes / args.stage_bytes));
-    const int64_t part = int64_t(kLoraTileRows) * (rp + 4) * 4;                          // overlays the ring
-    const int64_t smem = std::max<int64_t>(int64_t(args.num_stages) * args.stage_bytes, part) + 1024;
+    args.ring_bytes = kRingBytes;             // the partial sums of a cluster overlay it: at most 128 x 132 floats
+    const int64_t smem = kRingBytes + 1024;
     const CUtensorMap map_x = make_map_2d(x, rows, args.k, kLoraBlockK, kLoraTileRows);
     const CUtensorMap map_a = args.mn_major ? make_map_3d(a, args.rows.num_adapters, args.k, rank, 64, 64)
                                             : make_map_3d(a, args.rows.num_adapters, rank, args.k, kLoraBlockK, rp);
@@ -86,20 +98,51 @@ namespace {
 
 template <int BN>
 void launch_gemm(LoraGemmArgs args, const void* x, const void* w, int sms, cudaStream_t stream) {
-    constexpr int kStages = BN == 256 ? 4 : 6;
-    args.m_tiles = math::ceil_div(args.rows.num_rows, kLoraTileRows), args.n_tiles = math::ceil_div(args.n, BN);
+    const auto& r = args.rows;
+    args.m_tiles = math::ceil_div(r.num_rows, kLoraTileRows), args.n_tiles = math::ceil_div(args.n, BN);
     const int64_t tiles = int64_t(args.m_tiles) * args.n_tiles;
     EP_HOST_ASSERT_MSG(tiles < (int64_t(1) << 30), "too many tiles for one launch");
     args.cluster = BN == 128 ? choose_cluster(tiles, math::ceil_div(args.k, kLoraBlockK), 4, sms) : 1;
     const int64_t grid = args.cluster > 1 ? tiles * args.cluster : std::min<int64_t>(tiles, sms);
-    const int64_t smem = kStages * int64_t(kLoraTileRows + BN) * kLoraBlockK * 2 + 4 * 4096 + 1024;
-    const auto& r = args.rows;
     const CUtensorMap map_x = make_map_2d(x, r.num_rows, args.k, kLoraBlockK, kLoraTileRows);
     const CUtensorMap map_w = args.mn_major ? make_map_2d(w, args.k, args.n, 64, kLoraBlockK) : make_map_2d(w, args.n, args.k, kLoraBlockK, 128);
     const CUtensorMap map_v = args.mn_major ? make_map_3d(args.v, r.num_adapters, r.rank, args.n, 64, 64)
                                             : make_map_3d(args.v, r.num_adapters, args.n, r.rank, 64, 128);
     const CUtensorMap map_y = make_map_out(args.y, r.num_rows, args.n, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
-    launch_clusters(lora_gemm_kernel<BN>, grid, 320, args.cluster, smem, true, stream, map_x, map_w, map_v, map_y, args);
+    launch_clusters(lora_gemm_kernel<BN>, grid, 320, args.cluster, lora_gemm_smem_bytes<BN>(), true, stream, map_x, map_w, map_v, map_y, args);
+}
+
+// Few rows: columns per tile and CTAs per cluster by an estimate of the time. W comes from memory at 6.5 TB/s however it is
+// cut; a CTA takes in at most about 110 KB per us of W and of x, which every column tile reads again; and a cluster costs two
+// barriers (about 1 us) and the parts that each CTA sends to the others, at about 15 KB per us. Measured with W [4096, 7168]:
+// 64 columns by two CTAs took 15.1 / 15.4 / 17.1 us for 1 / 32 / 128 rows, 128 columns by four 14.8 / 17.1 / 18.5 us (32 columns and
+// no cluster 17.6 to 25 us: too many small blocks per CTA). Stages of up to 48 KB: fewer, larger steps leave the issuing warps
+// ahead of memory.
+bool launch_gemm_few(const LoraGemmArgs& g, const void* x, const void* w, int sms, cudaStream_t stream) {
+    LoraGemmFewArgs args = {};
+    args.rows = g.rows, args.k = g.k, args.n = g.n, args.mn_major = g.mn_major, args.t = g.t, args.v = g.v, args.y = g.y;
+    args.m_tiles = math::ceil_div(g.rows.num_rows, kLoraTileRows);
+    args.x_box_rows = args.m_tiles > 1 ? kLoraTileRows : math::align(g.rows.num_rows, 8);
+    const int blocks = math::ceil_div(g.k, kLoraBlockK);
+    double best = 0;
+    for (int bn = 64; bn <= 128; bn *= 2) {
+        const int64_t tiles = int64_t(args.m_tiles) * math::ceil_div(g.n, bn);
+        if (tiles > sms) continue;
+        const int block_bytes = (args.x_box_rows + bn) * kLoraBlockK * 2, sub = std::clamp(48 * 1024 / block_bytes, 1, 4);
+        const int cluster = choose_cluster(tiles, math::ceil_div(blocks, sub), 2, sms);
+        const double stream_us = std::max(double(g.n) * g.k * 2 / 6.5e6, double(block_bytes) * blocks / cluster / 110e3);
+        const double tail_us = cluster > 1 ? 1.0 + double(args.x_box_rows) * bn * 4 * (cluster - 1) / cluster / 15e3 : 0.0;
+        if (best == 0 or stream_us + tail_us < best) best = stream_us + tail_us, args.block_n = bn, args.cluster = cluster, args.stage_blocks = sub;
+    }
+    if (best == 0) return false;
+    const int64_t tiles = int64_t(args.m_tiles) * math::ceil_div(g.n, args.block_n);
+    const int64_t part_bytes = int64_t(kLoraTileRows) * args.block_n * 4, budget = 225 * 1024 - 1024 - part_bytes;
+    const int64_t stage = int64_t(args.stage_blocks) * (args.x_box_rows + args.block_n) * kLoraBlockK * 2;
+    args.num_stages = static_cast<int>(std::min<int64_t>(32, budget / stage));
+    const CUtensorMap map_x = make_map_2d(x, g.rows.num_rows, g.k, kLoraBlockK, args.x_box_rows);
+    const CUtensorMap map_w = g.mn_major ? make_map_2d(w, g.k, g.n, 64, kLoraBlockK) : make_map_2d(w, g.n, g.k, kLoraBlockK, args.block_n);
+    launch_clusters(lora_gemm_few_kernel, tiles * args.cluster, 320, args.cluster, args.num_stages * stage + part_bytes + 1024, true, stream, map_x, map_w, args);
+    return true;
 }
 
 }  // namespace
@@ -108,28 +151,29 @@ void lora_gemm(LoraGemmArgs args, const void* x, const void* w, cudaStream_t str
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
     const int sms = device_sms();
-    const int64_t wide = int64_t(math::ceil_div(args.rows.num_rows, kLoraTileRows)) * math::ceil_div(args.n, 256);
+    const int64_t rows = args.rows.num_rows, m_tiles = math::ceil_div<int64_t>(rows, kLoraTileRows);
+    if (rows * args.rows.rank <= kFewTerms and launch_gemm_few(args, x, w, sms, stream)) return;
     // 256 columns per tile as soon as that gives every SM a tile: half the shared-memory traffic per product
-    if (wide >= sms) launch_gemm<256>(args, x, w, sms, stream);
+    if (m_tiles * math::ceil_div(args.n, 256) >= sms) launch_gemm<256>(args, x, w, sms, stream);
     else launch_gemm<128>(args, x, w, sms, stream);
 }
 
 void lora_wgrad(LoraWgradArgs args, const void* x, cudaStream_t stream) {
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
-    const int rp = math::align(args.rows.rank, 64);
+    const int half = args.rows.rank <= 32 ? 32 : math::align(args.rows.rank, 64);         // columns of hi, as many of lo
     args.m_tiles = math::ceil_div(args.m, kLoraWgradColumns);
     args.row_tiles = math::ceil_div(args.rows.num_rows, kLoraTileRows);
     EP_HOST_ASSERT_MSG(args.row_tiles <= kLoraMaxTileWords * 32, "too many rows for one call");
     const int adapters = std::min(args.rows.num_adapters, args.rows.num_rows);           // that can have rows at all
     const int blocks = math::ceil_div(args.rows.num_rows, kLoraBlockK);
     args.cluster = choose_cluster(int64_t(args.m_tiles) * adapters, math::ceil_div(blocks, adapters), 2, device_sms());
-    args.stage_bytes = kLoraWgradColumns * kLoraBlockK * 2 + 2 * rp * 128;
+    args.stage_bytes = kLoraWgradColumns * kLoraBlockK * 2 + 2 * half * 128;
     args.num_stages = static_cast<int>(std::min<int64_t>(4, kRingBytes / args.stage_bytes));
-    const int64_t part = int64_t(kLoraWgradColumns) * (rp + 1) * 4;                      // overlays the ring
+    const int64_t part = int64_t(kLoraWgradColumns) * (math::align(args.rows.rank, 16) + 4) * 4;                      // overlays the ring
     const int64_t smem = std::max<int64_t>(int64_t(args.num_stages) * args.stage_bytes, part) + 1024;
     const CUtensorMap map_x = make_map_2d(x, args.rows.num_rows, args.m, 64, kLoraBlockK);
-    launch_clusters(lora_wgrad_kernel, int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 192, args.cluster, smem, false, stream, map_x, args);
+    launch_clusters(lora_wgrad_kernel, int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 320, args.cluster, smem, false, stream, map_x, args);
 }
 
 }  // namespace deep_ep::launch

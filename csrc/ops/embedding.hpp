@@ -36,7 +36,7 @@ inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
     EP_HOST_ASSERT_MSG(idx.device() == with.device(), "all tensors of a call lie on one device");
 }
 
-// [num_tokens, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
+// [*idx.shape, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
 inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale,
                                       const std::optional<torch::Tensor>& table_sf) {
     check_rows(table), check_ids(idx, table);
@@ -56,7 +56,9 @@ inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::T
                            "scales are fp32 [rows, hidden / 128], hidden a multiple of 128");
         a.table_sf = table_sf->data_ptr<float>(), a.sf_stride = table_sf->stride(0);
     }
-    auto out = torch::empty({a.num_tokens, a.hidden}, table.options().dtype(
+    auto shape = idx.sizes().vec();
+    shape.push_back(a.hidden);
+    auto out = torch::empty(shape, table.options().dtype(
         type == kernels::EmbType::kE4M3 ? torch::kBFloat16 : table.scalar_type()));
     a.out = out.data_ptr();
     launch::embedding_lookup(a, type, c10::cuda::getCurrentCUDAStream());
@@ -88,16 +90,17 @@ inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, do
         if (not accumulate) out.zero_();
         return;
     }
-    g.chunk = launch::embedding_grad_chunk(num_tokens), g.num_chunks = (num_tokens + g.chunk - 1) / g.chunk;
+    g.chunk = launch::embedding_grad_chunk(num_tokens, hidden), g.num_chunks = (num_tokens + g.chunk - 1) / g.chunk;
     // scratch of this call, from the caching allocator: freed in stream order, private to a graph that is being captured
-    const int64_t bitmap_ints = accumulate ? 0 : (num_rows + 31) / 32;
-    const auto ints = torch::empty({launch::embedding_sort_workspace_ints(num_tokens) + bitmap_ints}, idx.options().dtype(torch::kInt32));
+    const int64_t sort_ints = launch::embedding_sort_workspace_ints(num_tokens), bitmap_ints = accumulate ? 0 : (num_rows + 31) / 32;
+    const auto ints = torch::empty({sort_ints + bitmap_ints + 1 + g.num_chunks}, idx.options().dtype(torch::kInt32));
     const auto partial = torch::empty({g.num_chunks > 1 ? 2ll * g.num_chunks * hidden : 0}, dy.options().dtype(torch::kFloat32));
     g.partial = partial.data_ptr<float>();
     kernels::EmbSortArgs s = {};
     s.idx = idx.data_ptr(), s.idx64 = idx.scalar_type() == torch::kInt64, s.num_tokens = num_tokens, s.num_rows = num_rows;
     // a sum is written over the whole row, so only rows without a token need zeros
-    s.touched = accumulate ? nullptr : reinterpret_cast<uint32_t*>(ints.data_ptr<int>() + ints.numel() - bitmap_ints);
+    s.touched = accumulate ? nullptr : reinterpret_cast<uint32_t*>(ints.data_ptr<int>() + sort_ints);
+    s.num_crossing = g.num_crossing = ints.data_ptr<int>() + sort_ints + bitmap_ints, g.crossing = g.num_crossing + 1;
     launch::embedding_sort(s, ints.data_ptr<int>(), &g.ids, &g.order, stream);
     g.touched = s.touched;
     launch::embedding_grad(g, in_type, out_type, stream);

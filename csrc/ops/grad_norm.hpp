@@ -85,6 +85,9 @@ inline torch::Tensor grad_norm_finish(const torch::Tensor& sums) {
     return norm;
 }
 
+// the norm of one list
+inline torch::Tensor grad_norm(const std::vector<torch::Tensor>& grads) { return grad_norm_finish(grad_square_sums(grads)); }
+
 // outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), in place without `outs`; returns the norm
 inline torch::Tensor grad_clip(const std::vector<torch::Tensor>& grads, const std::optional<std::vector<torch::Tensor>>& outs,
                                const std::optional<torch::Tensor>& sums, double max_norm) {
@@ -105,6 +108,7 @@ inline void register_grad_norm(pybind11::module_& m) {
     namespace py = pybind11;
     m.def("grad_square_sums", &grad_square_sums, py::arg("grads"));
     m.def("grad_norm_finish", &grad_norm_finish, py::arg("sums"));
+    m.def("grad_norm", &grad_norm, py::arg("grads"));
     m.def("grad_clip", &grad_clip, py::arg("grads"), py::arg("outs"), py::arg("sums"), py::arg("max_norm"));
 }
 

@@ -15,16 +15,17 @@
 
 namespace deep_ep::ops {
 
-// A contiguous CUDA tensor on a 16-byte boundary, as the TMA reads it
-inline void check_operand(const torch::Tensor& t, int dims, const torch::Tensor& with, torch::ScalarType type = torch::kBFloat16) {
-    EP_HOST_ASSERT_MSG(t.is_cuda() and t.is_contiguous() and t.dim() == dims and t.scalar_type() == type, "contiguous CUDA tensors of the documented type and rank");
+// The tensor as the TMA reads it: contiguous, on a 16-byte boundary (a copy where a view is neither)
+inline torch::Tensor operand(const torch::Tensor& t, int dims, const torch::Tensor& with, torch::ScalarType type = torch::kBFloat16) {
+    EP_HOST_ASSERT_MSG(t.is_cuda() and t.dim() == dims and t.scalar_type() == type, "CUDA tensors of the documented types and shapes");
     EP_HOST_ASSERT_MSG(t.device() == with.device(), "all tensors of a call lie on one device");
-    EP_HOST_ASSERT_MSG(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "operands start on 16-byte boundaries");
     for (int i = 0; i < dims; ++i) EP_HOST_ASSERT_MSG(t.size(i) <= std::numeric_limits<int>::max() / 2, "sizes above 2^30");
+    const auto c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
 inline kernels::LoraRows adapter_rows(const torch::Tensor& idx, const torch::Tensor& with, int64_t num_adapters, int64_t rank) {
-    EP_HOST_ASSERT_MSG(idx.is_contiguous() and idx.dim() == 1 and idx.device() == with.device() and
+    EP_HOST_ASSERT_MSG(idx.dim() == 1 and (idx.size(0) <= 1 or idx.stride(0) == 1) and idx.device() == with.device() and
                        (idx.scalar_type() == torch::kInt32 or idx.scalar_type() == torch::kInt64), "adapter indices are int32 or int64 [rows]");
     EP_HOST_ASSERT_MSG(idx.size(0) == with.size(0), "one adapter index per row");
     EP_HOST_ASSERT_MSG(num_adapters >= 1 and rank >= 8 and rank % 8 == 0 and rank <= kernels::kLoraMaxRank, "ranks are multiples of 8 up to 128");
@@ -32,13 +33,13 @@ inline kernels::LoraRows adapter_rows(const torch::Tensor& idx, const torch::Ten
 }
 
 // (t fp32 [rows, rank] = scaling[e] * x . A_e^T, presence uint8 [row tiles, adapters] or nothing). `transposed`: A is [adapters, k, rank].
-inline std::tuple<torch::Tensor, std::optional<torch::Tensor>> lora_shrink(const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& idx,
-                                                                           const torch::Tensor& scaling, bool transposed, bool with_presence) {
-    check_operand(x, 2, x), check_operand(a, 3, x), check_operand(scaling, 1, x, torch::kFloat32);
+inline std::tuple<torch::Tensor, std::optional<torch::Tensor>> lora_shrink(const torch::Tensor& x_in, const torch::Tensor& a_in, const torch::Tensor& idx,
+                                                                           const torch::Tensor& scaling_in, bool transposed, bool with_presence) {
+    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
+    const auto x = operand(x_in, 2, x_in), a = operand(a_in, 3, x_in), scaling = operand(scaling_in, 1, x_in, torch::kFloat32);
     const int64_t k = x.size(1), rank = transposed ? a.size(2) : a.size(1);
     EP_HOST_ASSERT_MSG((transposed ? a.size(1) : a.size(2)) == k and k >= 8 and k % 8 == 0, "contraction lengths agree and are multiples of 8");
     EP_HOST_ASSERT_MSG(scaling.size(0) == a.size(0), "one scaling per adapter");
-    const c10::cuda::CUDAGuard guard(x.device());
     kernels::LoraShrinkArgs args = {};
     args.rows = adapter_rows(idx, x, a.size(0), rank);
     args.k = static_cast<int>(k), args.mn_major = transposed, args.scaling = scaling.data_ptr<float>();
@@ -54,13 +55,13 @@ inline std::tuple<torch::Tensor, std::optional<torch::Tensor>> lora_shrink(const
 }
 
 // y = x . W^T + t . V_e^T; `transposed`: W is [k, n] and V [adapters, rank, n] (the data gradient), else [n, k] and [adapters, n, rank]
-inline torch::Tensor lora_gemm(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& t, const torch::Tensor& v,
+inline torch::Tensor lora_gemm(const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& t_in, const torch::Tensor& v_in,
                                const torch::Tensor& idx, bool transposed) {
-    check_operand(x, 2, x), check_operand(w, 2, x), check_operand(v, 3, x), check_operand(t, 2, x, torch::kFloat32);
+    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
+    const auto x = operand(x_in, 2, x_in), w = operand(w_in, 2, x_in), t = operand(t_in, 2, x_in, torch::kFloat32), v = operand(v_in, 3, x_in);
     const int64_t k = x.size(1), n = transposed ? w.size(1) : w.size(0), rank = t.size(1);
     EP_HOST_ASSERT_MSG((transposed ? w.size(0) : w.size(1)) == k and k >= 8 and k % 8 == 0 and n >= 8 and n % 8 == 0, "dimensions agree and are multiples of 8");
     EP_HOST_ASSERT_MSG(t.size(0) == x.size(0) and (transposed ? v.size(1) : v.size(2)) == rank and (transposed ? v.size(2) : v.size(1)) == n, "adapter shapes agree");
-    const c10::cuda::CUDAGuard guard(x.device());
     kernels::LoraGemmArgs args = {};
     args.rows = adapter_rows(idx, x, v.size(0), rank);
     args.k = static_cast<int>(k), args.n = static_cast<int>(n), args.mn_major = transposed;
@@ -70,16 +71,26 @@ inline torch::Tensor lora_gemm(const torch::Tensor& x, const torch::Tensor& w, c
     return y;
 }
 
+// (y, t): both steps of the forward pass
+inline std::tuple<torch::Tensor, torch::Tensor> lora_forward(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& a, const torch::Tensor& b,
+                                                             const torch::Tensor& idx, const torch::Tensor& scaling) {
+    EP_HOST_ASSERT_MSG(a.dim() == 3 and b.dim() == 3 and a.size(0) == b.size(0), "as many A as B");
+    const auto t = std::get<0>(lora_shrink(x, a, idx, scaling, false, false));
+    return {lora_gemm(x, w, t, b, idx, false), t};
+}
+
 // out[e] (+)= sum over the rows of adapter e of t[row]^T x[row]: [adapters, rank, m] (`rank_major`) or [adapters, m, rank]
-inline void lora_wgrad(const torch::Tensor& x, const torch::Tensor& t, const torch::Tensor& idx, const torch::Tensor& presence,
+inline void lora_wgrad(const torch::Tensor& x_in, const torch::Tensor& t_in, const torch::Tensor& idx, const torch::Tensor& presence,
                        const torch::Tensor& out, bool rank_major, bool accumulate) {
-    check_operand(x, 2, x), check_operand(t, 2, x, torch::kFloat32), check_operand(presence, 2, x, torch::kUInt8);
-    check_operand(out, 3, x, out.scalar_type());
+    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
+    const auto x = operand(x_in, 2, x_in), t = operand(t_in, 2, x_in, torch::kFloat32);
+    EP_HOST_ASSERT_MSG(out.device() == x.device() and out.dim() == 3 and out.is_contiguous(), "a contiguous result on the operands' device");
+    EP_HOST_ASSERT_MSG(presence.device() == x.device() and presence.dim() == 2 and presence.is_contiguous() and presence.scalar_type() == torch::kUInt8, "presence of `lora_shrink`");
     const int64_t rank = t.size(1), m = x.size(1);
     EP_HOST_ASSERT_MSG(t.size(0) == x.size(0) and m >= 8 and m % 8 == 0, "one t per row, columns a multiple of 8");
     EP_HOST_ASSERT_MSG(out.size(1) == (rank_major ? rank : m) and out.size(2) == (rank_major ? m : rank), "the result's shape");
     EP_HOST_ASSERT_MSG(out.scalar_type() == torch::kFloat32 or (out.scalar_type() == torch::kBFloat16 and not accumulate), "fp32, or bf16 and overwritten");
-    const c10::cuda::CUDAGuard guard(x.device());
+    EP_HOST_ASSERT_MSG(out.scalar_type() == torch::kFloat32 or reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0, "a bf16 result starts on a 16-byte boundary");
     kernels::LoraWgradArgs args = {};
     args.rows = adapter_rows(idx, x, out.size(0), rank);
     EP_HOST_ASSERT(presence.size(1) == out.size(0) and presence.size(0) == (x.size(0) + kernels::kLoraTileRows - 1) / kernels::kLoraTileRows);
@@ -98,6 +109,7 @@ inline void register_lora(pybind11::module_& m) {
     m.def("lora_shrink", &lora_shrink, py::arg("x"), py::arg("a"), py::arg("idx"), py::arg("scaling"), py::arg("transposed") = false,
           py::arg("with_presence") = false);
     m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("v"), py::arg("idx"), py::arg("transposed") = false);
+    m.def("lora_forward", &lora_forward, py::arg("x"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling"));
     m.def("lora_wgrad", &lora_wgrad, py::arg("x"), py::arg("t"), py::arg("idx"), py::arg("presence"), py::arg("out"), py::arg("rank_major"),
           py::arg("accumulate") = false);
 }

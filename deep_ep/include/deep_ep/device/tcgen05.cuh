@@ -169,6 +169,9 @@ EP_DEVICE uint32_t cluster_ctarank() {
 EP_DEVICE void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// the same in two halves: what lies between may run before the others have arrived
+EP_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+EP_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // shared::cluster address of `local_ptr`'s counterpart in CTA `rank` of this cluster
 EP_DEVICE uint32_t map_to_cta(const void* local_ptr, uint32_t rank) {
     uint32_t out;

@@ -13,49 +13,109 @@
 
 #include <cuda_fp16.h>
 
-#include "../device/ptx.cuh"
+#include <type_traits>
+
+#include "../device/tcgen05.cuh"
 #include "embedding_args.hpp"
 
 namespace deep_ep::kernels {
 
 namespace emb_detail {
 
-template <int kBytes> struct RawOf;
-template <> struct RawOf<1> { using type = uint8_t; };
-template <> struct RawOf<2> { using type = uint16_t; };
-template <> struct RawOf<4> { using type = uint32_t; };
-template <> struct RawOf<8> { using type = uint2; };
-template <> struct RawOf<16> { using type = uint4; };
-
-EP_DEVICE float to_float(float v) { return v; }
-EP_DEVICE float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-EP_DEVICE float to_float(__half v) { return __half2float(v); }
-EP_DEVICE float to_float(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
-template <typename T> EP_DEVICE T from_float(float v);
-template <> EP_DEVICE float from_float<float>(float v) { return v; }
-template <> EP_DEVICE __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> EP_DEVICE __half from_float<__half>(float v) { return __float2half_rn(v); }
-
-// `kElems` consecutive elements that move as one access of up to 16 bytes (more than that: several of 16)
+// `kElems` consecutive elements as they move: one access of up to 16 bytes, or two of 16. Kept as raw words until they are used
+// (elements of 16 bits would otherwise take a register each).
 template <typename T, int kElems>
-struct alignas(kElems * sizeof(T) < 16 ? kElems * sizeof(T) : 16) Pack {
-    T v[kElems];
+struct Pack {
+    static constexpr int kBytes = kElems * int(sizeof(T)), kParts = kBytes > 16 ? kBytes / 16 : 1;
+    using Raw = std::conditional_t<kBytes >= 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, uint32_t,
+                std::conditional_t<kBytes == 2, uint16_t, uint8_t>>>>;
+    Raw raw[kParts];
+
+    EP_DEVICE uint32_t word(int i) const {
+        if constexpr (kBytes >= 16) {
+            const uint4& u = raw[i / 4];
+            return i % 4 == 0 ? u.x : i % 4 == 1 ? u.y : i % 4 == 2 ? u.z : u.w;
+        } else if constexpr (kBytes == 8) {
+            return i == 0 ? raw[0].x : raw[0].y;
+        } else {
+            return raw[0];
+        }
+    }
+    EP_DEVICE void set_word(int i, uint32_t w) {
+        if constexpr (kBytes >= 16) {
+            uint4& u = raw[i / 4];
+            (i % 4 == 0 ? u.x : i % 4 == 1 ? u.y : i % 4 == 2 ? u.z : u.w) = w;
+        } else if constexpr (kBytes == 8) {
+            (i == 0 ? raw[0].x : raw[0].y) = w;
+        } else {
+            raw[0] = static_cast<Raw>(w);
+        }
+    }
 };
+
 template <typename T, int kElems>
-EP_DEVICE Pack<T, kElems> load_pack(const T* p) {
-    using Raw = typename RawOf<(kElems * sizeof(T) < 16 ? kElems * sizeof(T) : 16)>::type;
-    constexpr int kParts = kElems * sizeof(T) / sizeof(Raw);
+EP_DEVICE Pack<T, kElems> load_pack(const T* p) {           // data that nobody writes during the kernel
     Pack<T, kElems> out;
     #pragma unroll
-    for (int i = 0; i < kParts; ++i) reinterpret_cast<Raw*>(&out)[i] = __ldg(reinterpret_cast<const Raw*>(p) + i);
+    for (int i = 0; i < Pack<T, kElems>::kParts; ++i) out.raw[i] = __ldg(reinterpret_cast<const typename Pack<T, kElems>::Raw*>(p) + i);
+    return out;
+}
+template <typename T, int kElems>
+EP_DEVICE Pack<T, kElems> load_written_pack(const T* p) {
+    Pack<T, kElems> out;
+    #pragma unroll
+    for (int i = 0; i < Pack<T, kElems>::kParts; ++i) out.raw[i] = reinterpret_cast<const typename Pack<T, kElems>::Raw*>(p)[i];
     return out;
 }
 template <typename T, int kElems>
 EP_DEVICE void store_pack(T* p, const Pack<T, kElems>& in) {
-    using Raw = typename RawOf<(kElems * sizeof(T) < 16 ? kElems * sizeof(T) : 16)>::type;
-    constexpr int kParts = kElems * sizeof(T) / sizeof(Raw);
     #pragma unroll
-    for (int i = 0; i < kParts; ++i) reinterpret_cast<Raw*>(p)[i] = reinterpret_cast<const Raw*>(&in)[i];
+    for (int i = 0; i < Pack<T, kElems>::kParts; ++i) reinterpret_cast<typename Pack<T, kElems>::Raw*>(p)[i] = in.raw[i];
+}
+
+template <typename T, int kElems>
+EP_DEVICE void unpack(const Pack<T, kElems>& in, float (&out)[kElems]) {
+    if constexpr (sizeof(T) == 4) {
+        #pragma unroll
+        for (int j = 0; j < kElems; ++j) out[j] = __uint_as_float(in.word(j));
+    } else if constexpr (sizeof(T) == 2) {
+        #pragma unroll
+        for (int j = 0; j < kElems; ++j) {
+            const uint32_t w = in.word(j / 2);
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) out[j] = __uint_as_float(j % 2 ? w & 0xffff0000u : w << 16);
+            else out[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(j % 2 ? w >> 16 : w & 0xffffu)));
+        }
+    } else if constexpr (kElems == 1) {
+        out[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(in.word(0)), __NV_E4M3)));
+    } else {
+        #pragma unroll
+        for (int j = 0; j < kElems; j += 2) {               // the hardware converts pairs
+            const uint32_t w = in.word(j / 4);
+            const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(j % 4 ? w >> 16 : w & 0xffffu), __NV_E4M3)));
+            out[j] = f.x, out[j + 1] = f.y;
+        }
+    }
+}
+// Rounds to the type
+template <typename T, int kElems>
+EP_DEVICE Pack<T, kElems> pack(const float (&v)[kElems]) {
+    Pack<T, kElems> out;
+    if constexpr (sizeof(T) == 4) {
+        #pragma unroll
+        for (int j = 0; j < kElems; ++j) out.set_word(j, __float_as_uint(v[j]));
+    } else {
+        #pragma unroll
+        for (int j = 0; j < kElems; j += 2) {
+            const float next = j + 1 < kElems ? v[j + 1 < kElems ? j + 1 : j] : 0.0f;
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                out.set_word(j / 2, ptx::float2_to_bf16x2(v[j], next));
+            } else {
+                const __half2 h = __floats2half2_rn(v[j], next);
+                out.set_word(j / 2, *reinterpret_cast<const uint32_t*>(&h));
+            }
+        }
+    }
+    return out;
 }
 
 EP_DEVICE int64_t load_id(const void* idx, int idx64, int64_t i) {
@@ -64,8 +124,9 @@ EP_DEVICE int64_t load_id(const void* idx, int idx64, int64_t i) {
 
 }  // namespace emb_detail
 
-// One warp per (token, slice of 32 * kElems * kUnroll columns). A warp keeps kUnroll accesses of up to 16 bytes per lane in
-// flight: four for large calls, where the 64 resident warps of an SM then cover the latency of HBM; one for small calls,
+// One warp per (token, slice of 32 * kElems * kUnroll columns). The side with the wider elements moves 16 bytes per lane and
+// access (8-bit entries are therefore read 8 bytes at a time: 16 would leave stores of half sectors). A warp keeps kUnroll
+// accesses per lane in flight: four for large calls, where the 64 resident warps of an SM then cover the latency of HBM; one for small calls,
 // which spreads a single row over more SMs.
 template <typename In, typename Out, int kElems, int kUnroll>
 __global__ void __launch_bounds__(256) embedding_lookup_kernel(const __grid_constant__ EmbLookupArgs a) {
@@ -94,15 +155,14 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const __grid_cons
     for (int u = 0; u < kUnroll; ++u) {
         const unsigned p = (slice * kUnroll + u) * 32 + lane;
         if (p >= packs) continue;
-        Pack<Out, kElems> o;
+        float v[kElems];
+        unpack<In, kElems>(in[u], v);
         #pragma unroll
         for (int j = 0; j < kElems; ++j) {
-            float v = 0.0f;
-            if (valid) v = to_float(in[u].v[j]);
-            if constexpr (sizeof(In) == 1) v *= sf[u];
-            o.v[j] = from_float<Out>(valid ? v * a.scale : 0.0f);
+            if constexpr (sizeof(In) == 1) v[j] *= sf[u];
+            v[j] = valid ? v[j] * a.scale : 0.0f;
         }
-        store_pack<Out, kElems>(out + int64_t(p) * kElems, o);
+        store_pack<Out, kElems>(out + int64_t(p) * kElems, pack<Out, kElems>(v));
     }
 }
 
@@ -211,34 +271,114 @@ EP_DEVICE void prefix_over_warps(int* counters, int* totals, int bins) {
 
 }  // namespace emb_detail
 
-// All passes in one CTA: no launch gaps between the passes. For the batches whose keys one CTA ranks faster than the four
-// launches of the form below take.
-__global__ void __launch_bounds__(kEmbSortSoloThreads) embedding_sort_solo_kernel(const __grid_constant__ EmbSortArgs a) {
+// All passes in one launch: up to eight CTAs of a cluster hold the keys in their shared memory. Per pass every warp ranks its
+// keys (in registers) per digit, the CTAs exchange their counts, and each key goes straight into the shared memory of the CTA
+// that owns its place (the last pass writes to memory). The time is latency (match, barriers), not work, so the keys are
+// spread over the cluster even when one CTA could hold them: a warp then has one or two rounds of 32 keys.
+template <int kRounds>
+__global__ void __launch_bounds__(kEmbClusterThreads, 1) embedding_sort_cluster_kernel(const __grid_constant__ EmbSortArgs a) {
     using namespace emb_detail;
-    constexpr int kWarps = kEmbSortSoloThreads / 32;
-    extern __shared__ int sort_smem[];                 // counters [kWarps][bins], totals [bins], warp sums [32]
+    constexpr int kWarps = kEmbClusterThreads / 32, kKeys = kEmbClusterThreads * kRounds;       // keys of a CTA, a power of two
+    extern __shared__ int sort_smem[];
+    __shared__ int warp_sums[32];
     const int bins = 1 << a.digit_bits, lane = ptx::lane_id(), warp = threadIdx.x / 32;
-    int *totals = sort_smem + kWarps * bins, *warp_sums = totals + bins;
-    int* mine = sort_smem + warp * bins;
-    const int begin = min(warp * a.keys_per_warp, a.num_tokens), end = min(begin + a.keys_per_warp, a.num_tokens);
+    const int rank = int(tc::cluster_ctarank()), ctas = int(gridDim.x);
+    int* keys[2] = {sort_smem, sort_smem + kKeys};
+    int* vals[2] = {sort_smem + 2 * kKeys, sort_smem + 3 * kKeys};
+    int *hist = sort_smem + 4 * kKeys, *base = hist + bins, *totals = base + bins;
+    uint16_t* counters = reinterpret_cast<uint16_t*>(totals + bins);                            // [kWarps][bins]
+    uint16_t* mine = counters + warp * bins;
+    const int count = min(max(a.num_tokens - rank * kKeys, 0), kKeys);                          // this CTA's keys
+
+    cudaTriggerProgrammaticLaunchCompletion();                  // the kernel of the sums may be set up meanwhile
+    if (rank == 0 and threadIdx.x == 0) *a.num_crossing = 0;
     if (a.touched != nullptr)
-        for (int i = threadIdx.x; i < (a.num_rows + 31) / 32; i += kEmbSortSoloThreads) a.touched[i] = 0;
+        for (int i = rank * kEmbClusterThreads + threadIdx.x; i < (a.num_rows + 31) / 32; i += ctas * kEmbClusterThreads) a.touched[i] = 0;
+    int key[kRounds], val[kRounds];
+    #pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const int i = (warp * kRounds + r) * 32 + lane;
+        val[r] = rank * kKeys + i;
+        key[r] = i < count ? sort_key(a, 0, val[r]) : a.num_rows;
+    }
+    if (a.touched != nullptr) {
+        // (the bitmap is zero once every CTA of the cluster has passed here)
+        __threadfence();
+        tc::cluster_sync();
+        #pragma unroll
+        for (int r = 0; r < kRounds; ++r)
+            if ((warp * kRounds + r) * 32 + lane < count and key[r] < a.num_rows) atomicOr(a.touched + (key[r] >> 5), 1u << (key[r] & 31));
+    }
     for (int pass = 0; pass < a.num_passes; ++pass) {
-        for (int i = threadIdx.x; i < kWarps * bins; i += kEmbSortSoloThreads) sort_smem[i] = 0;
+        const int shift = pass * a.digit_bits;
+        if (pass > 0) {
+            #pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int i = (warp * kRounds + r) * 32 + lane;
+                if (i < count) key[r] = keys[pass & 1][i], val[r] = vals[pass & 1][i];
+            }
+        }
+        for (int i = threadIdx.x; i < kWarps * bins / 2; i += kEmbClusterThreads) reinterpret_cast<uint32_t*>(counters)[i] = 0;
         __syncthreads();
-        sort_count(a, pass, mine, begin, end, lane);
+        int place[kRounds];                   // among this warp's keys of the same digit
+        #pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const bool active = (warp * kRounds + r) * 32 + lane < count;
+            const int digit = active ? (key[r] >> shift) & (bins - 1) : bins;
+            const unsigned peers = __match_any_sync(0xffffffffu, digit);
+            const int before = __popc(peers & ptx::lanemask_lt());
+            place[r] = active ? mine[digit] + before : 0;
+            __syncwarp();
+            if (active and before == 0) mine[digit] += uint16_t(__popc(peers));
+            __syncwarp();
+        }
         __syncthreads();
-        prefix_over_warps<kWarps>(sort_smem, totals, bins);
-        block_exclusive_scan<kEmbSortSoloThreads>(totals, bins, warp_sums);
-        for (int i = threadIdx.x; i < kWarps * bins; i += kEmbSortSoloThreads) sort_smem[i] += totals[i % bins];
+        for (int b = threadIdx.x; b < bins; b += kEmbClusterThreads) {
+            int run = 0;
+            #pragma unroll 8
+            for (int w = 0; w < kWarps; ++w) {
+                const int c = counters[w * bins + b];
+                counters[w * bins + b] = uint16_t(run);
+                run += c;
+            }
+            hist[b] = run;
+        }
+        tc::cluster_sync();
+        for (int b = threadIdx.x; b < bins; b += kEmbClusterThreads) {
+            int all = 0, earlier = 0;
+            int v[8];
+            #pragma unroll
+            for (int q = 0; q < 8; ++q)       // all in flight at once
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[q]) : "r"(tc::map_to_cta(hist + b, min(q, ctas - 1))));
+            #pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                all += q < ctas ? v[q] : 0;
+                earlier += q < rank ? v[q] : 0;
+            }
+            totals[b] = all, base[b] = earlier;
+        }
         __syncthreads();
-        sort_scatter(a, pass, mine, begin, end, lane);
-        __syncthreads();
+        block_exclusive_scan<kEmbClusterThreads>(totals, bins, warp_sums);
+        const bool last = pass + 1 == a.num_passes;
+        #pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            if ((warp * kRounds + r) * 32 + lane >= count) continue;
+            const int digit = (key[r] >> shift) & (bins - 1);
+            const int at = totals[digit] + base[digit] + mine[digit] + place[r];
+            if (last) {
+                a.keys[0][at] = key[r], a.vals[0][at] = val[r];
+            } else {
+                const int q = at / kKeys, i = at % kKeys, to = (pass + 1) & 1;
+                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(keys[to] + i, q)), "r"(key[r]) : "memory");
+                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(vals[to] + i, q)), "r"(val[r]) : "memory");
+            }
+        }
+        tc::cluster_sync();                   // keys are in place, and nobody still reads a neighbour's counts
     }
 }
 
-// The same over many CTAs, two launches per pass: counts per CTA, then the scatter (which adds up the counts of the smaller
-// digits and of the CTAs before it).
+// Longer inputs: any number of CTAs, two launches per pass (counts per CTA, then the scatter, which adds up the counts of the
+// smaller digits and of the CTAs before it), keys in memory.
 __global__ void __launch_bounds__(kEmbSortThreads) embedding_sort_count_kernel(const __grid_constant__ EmbSortArgs a) {
     using namespace emb_detail;
     constexpr int kWarps = kEmbSortThreads / 32;
@@ -248,6 +388,7 @@ __global__ void __launch_bounds__(kEmbSortThreads) embedding_sort_count_kernel(c
     const int64_t first = (int64_t(blockIdx.x) * kWarps + warp) * a.keys_per_warp;
     const int begin = int(min(first, int64_t(a.num_tokens))), end = int(min(first + a.keys_per_warp, int64_t(a.num_tokens)));
     for (int i = threadIdx.x; i < kWarps * bins; i += kEmbSortThreads) sort_smem[i] = 0;
+    if (a.pass == 0 and blockIdx.x == 0 and threadIdx.x == 0) *a.num_crossing = 0;
     if (a.pass == 0 and a.touched != nullptr)
         for (int i = blockIdx.x * kEmbSortThreads + threadIdx.x; i < (a.num_rows + 31) / 32; i += gridDim.x * kEmbSortThreads)
             a.touched[i] = 0;
@@ -292,144 +433,165 @@ __global__ void __launch_bounds__(kEmbSortThreads) embedding_sort_scatter_kernel
 namespace emb_detail {
 
 template <typename Out, int kElems>
-EP_DEVICE void write_sum(const EmbGradArgs& a, int id, int column, const float (&acc)[kElems]) {
-    Out* out = reinterpret_cast<Out*>(a.out) + int64_t(id) * a.out_stride + column;
-    Pack<Out, kElems> o;
-    if constexpr (sizeof(Out) == 4) {
-        if (a.accumulate) {
-            o = *reinterpret_cast<const Pack<Out, kElems>*>(out);
-            #pragma unroll
-            for (int j = 0; j < kElems; ++j) o.v[j] += a.scale * acc[j];
-            store_pack<Out, kElems>(out, o);
-            return;
-        }
-    }
+EP_DEVICE void write_sum(Out* out, float scale, const float (&acc)[kElems]) {
+    float v[kElems];
     #pragma unroll
-    for (int j = 0; j < kElems; ++j) o.v[j] = from_float<Out>(a.scale * acc[j]);
-    store_pack<Out, kElems>(out, o);
+    for (int j = 0; j < kElems; ++j) v[j] = scale * acc[j];
+    store_pack<Out, kElems>(out, pack<Out, kElems>(v));
 }
-
+// The same added to what was there (`old`, read ahead)
 template <int kElems>
-EP_DEVICE void write_partial(float* p, const float (&acc)[kElems]) {
-    Pack<float, kElems> o;
+EP_DEVICE void add_sum(float* out, float scale, const float (&acc)[kElems], const Pack<float, kElems>& old) {
+    float v[kElems];
+    unpack<float, kElems>(old, v);
     #pragma unroll
-    for (int j = 0; j < kElems; ++j) o.v[j] = acc[j];
-    store_pack<float, kElems>(p, o);
+    for (int j = 0; j < kElems; ++j) v[j] += scale * acc[j];
+    store_pack<float, kElems>(out, pack<float, kElems>(v));
 }
 
 }  // namespace emb_detail
 
-// One warp per (chunk of sorted positions, slice of 32 * kElems columns): the rows of a run are added in registers, kAhead
-// loads in flight. Further warps write the zero rows of a dense gradient, whose bytes are most of the work when the table is
-// much larger than the batch.
-template <typename In, typename Out, int kElems>
-__global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_constant__ EmbGradArgs a) {
+// One warp per (chunk of sorted positions, slice of 32 * kElems * kPacks columns): the rows of a run are added in registers,
+// kAhead rows in flight. When the sums are added to a buffer, the rows that end in the group of kAhead are read ahead too:
+// a read at the end of each run would be a round trip to memory per id. Further warps write the zero rows of a dense gradient,
+// whose bytes are most of the work when the table is much larger than the batch.
+template <typename In, typename Out, int kElems, int kPacks, bool kAccumulate>
+__global__ void __launch_bounds__(256, 3) embedding_grad_kernel(const __grid_constant__ EmbGradArgs a) {
     using namespace emb_detail;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = kAccumulate ? 4 : 8;
     const int lane = ptx::lane_id();
-    const unsigned slices = math::ceil_div(unsigned(a.hidden), 32u * kElems);
+    cudaTriggerProgrammaticLaunchCompletion();                  // the join kernel may be set up meanwhile
+    cudaGridDependencySynchronize();                            // the sort is done
+    const unsigned slices = math::ceil_div(unsigned(a.hidden), 32u * kElems * kPacks);
     const int64_t item = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
     const int64_t sum_items = int64_t(a.num_chunks) * slices;
     if (item >= sum_items) {
         // ---- rows without a token
         const int64_t row = item - sum_items;
         if (a.touched == nullptr or row >= a.num_rows or ((a.touched[row >> 5] >> (row & 31)) & 1u)) return;
-        Pack<Out, kElems> zero;
-        #pragma unroll
-        for (int j = 0; j < kElems; ++j) zero.v[j] = from_float<Out>(0.0f);
+        const float nothing[kElems] = {};
+        const Pack<Out, kElems> zero = pack<Out, kElems>(nothing);
         for (int c = lane * kElems; c < a.hidden; c += 32 * kElems)
             store_pack<Out, kElems>(reinterpret_cast<Out*>(a.out) + row * a.out_stride + c, zero);
         return;
     }
     const int chunk = int(unsigned(item) / slices), slice = int(unsigned(item) - unsigned(chunk) * slices);
-    const int column = (slice * 32 + lane) * kElems;
-    const bool mine = column < a.hidden;
-    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.num_tokens);
-    int run = a.ids[begin];
-    bool from_before = begin > 0 and a.ids[begin - 1] == run;
-    const int next = end < a.num_tokens ? a.ids[end] : a.num_rows;
-    float acc[kElems];
+    constexpr int kWidth = 32 * kElems;                         // columns from one pack of a lane to its next
+    const int column = slice * (kWidth * kPacks) + lane * kElems;
+    bool mine[kPacks];
     #pragma unroll
-    for (int j = 0; j < kElems; ++j) acc[j] = 0.0f;
-
-    auto flush = [&](bool goes_on) {
-        if (run >= a.num_rows or not mine) return;
-        if (from_before) write_partial<kElems>(a.partial + (int64_t(chunk) * 2) * a.hidden + column, acc);
-        else if (goes_on) write_partial<kElems>(a.partial + (int64_t(chunk) * 2 + 1) * a.hidden + column, acc);
-        else write_sum<Out, kElems>(a, run, column, acc);
-    };
+    for (int p = 0; p < kPacks; ++p) mine[p] = column + p * kWidth < a.hidden;
+    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.num_tokens);
+    bool from_before = begin > 0 and a.ids[begin - 1] == a.ids[begin];
+    const In* dy = reinterpret_cast<const In*>(a.dy) + column;
+    float* partial = a.partial + int64_t(chunk) * 2 * a.hidden + column;
+    float acc[kPacks][kElems] = {};
 
     for (int base = begin; base < end; base += 32) {
         const int count = min(32, end - base);
         const int my_id = lane < count ? a.ids[base + lane] : a.num_rows;
         const int my_row = lane < count ? a.order[base + lane] : 0;
-        if (__shfl_sync(0xffffffffu, my_id, 0) >= a.num_rows and run >= a.num_rows) return;    // only masked positions follow
-        for (int j0 = 0; j0 < count; j0 += kAhead) {
-            Pack<In, kElems> in[kAhead];
+        const int behind = base + count < a.num_tokens ? a.ids[base + count] : a.num_rows;
+        // positions with an id (they come first), and those that end a run
+        const int valid = __popc(__ballot_sync(0xffffffffu, my_id < a.num_rows));
+        int after = __shfl_down_sync(0xffffffffu, my_id, 1);
+        if (lane == count - 1) after = behind;
+        const unsigned ends = __ballot_sync(0xffffffffu, after != my_id);
+        for (int j0 = 0; j0 < valid; j0 += kAhead) {
+            Pack<In, kElems> in[kAhead][kPacks];
+            Pack<float, kAccumulate ? kElems : 1> old[kAhead][kPacks];
             #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int id = __shfl_sync(0xffffffffu, my_id, j0 + u), row = __shfl_sync(0xffffffffu, my_row, j0 + u);
-                if (id < a.num_rows and mine)
-                    in[u] = load_pack<In, kElems>(reinterpret_cast<const In*>(a.dy) + int64_t(row) * a.dy_stride + column);
+                if (j0 + u >= valid) break;
+                const In* src = dy + int64_t(__shfl_sync(0xffffffffu, my_row, j0 + u)) * a.dy_stride;
+                #pragma unroll
+                for (int p = 0; p < kPacks; ++p)
+                    if (mine[p]) in[u][p] = load_pack<In, kElems>(src + p * kWidth);
+                if constexpr (kAccumulate) {
+                    if ((ends >> (j0 + u)) & 1u) {
+                        const float* out = reinterpret_cast<const float*>(a.out) + int64_t(__shfl_sync(0xffffffffu, my_id, j0 + u)) * a.out_stride + column;
+                        #pragma unroll
+                        for (int p = 0; p < kPacks; ++p)
+                            if (mine[p]) old[u][p] = load_written_pack<float, kElems>(out + p * kWidth);
+                    }
+                }
             }
             #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int id = __shfl_sync(0xffffffffu, my_id, j0 + u);
-                if (j0 + u >= count) break;
-                if (id != run) {
-                    flush(false);
-                    run = id, from_before = false;
+                if (j0 + u >= valid) break;
+                #pragma unroll
+                for (int p = 0; p < kPacks; ++p) {
+                    float v[kElems];
+                    unpack<In, kElems>(in[u][p], v);
                     #pragma unroll
-                    for (int j = 0; j < kElems; ++j) acc[j] = 0.0f;
+                    for (int j = 0; j < kElems; ++j) acc[p][j] += v[j];
                 }
-                if (id < a.num_rows and mine) {
+                const bool run_ends = (ends >> (j0 + u)) & 1u, last = base + j0 + u == end - 1;
+                if (not run_ends and not last) continue;
+                if (from_before or not run_ends) {
+                    // a piece of a run that crosses a chunk border; one that begins here and goes on enters the list for the
+                    // join kernel (in whatever order: runs do not meet)
                     #pragma unroll
-                    for (int j = 0; j < kElems; ++j) acc[j] += to_float(in[u].v[j]);
+                    for (int p = 0; p < kPacks; ++p)
+                        if (mine[p]) store_pack<float, kElems>(partial + (from_before ? 0 : a.hidden) + p * kWidth, pack<float, kElems>(acc[p]));
+                    if (not from_before and slice == 0 and lane == 0) a.crossing[atomicAdd(a.num_crossing, 1)] = chunk;
+                } else {
+                    Out* out = reinterpret_cast<Out*>(a.out) + int64_t(__shfl_sync(0xffffffffu, my_id, j0 + u)) * a.out_stride + column;
+                    #pragma unroll
+                    for (int p = 0; p < kPacks; ++p) {
+                        if (not mine[p]) continue;
+                        if constexpr (kAccumulate) add_sum<kElems>(out + p * kWidth, a.scale, acc[p], old[u][p]);
+                        else write_sum<Out, kElems>(out + p * kWidth, a.scale, acc[p]);
+                    }
                 }
+                from_before = false;
+                #pragma unroll
+                for (int p = 0; p < kPacks; ++p)
+                    #pragma unroll
+                    for (int j = 0; j < kElems; ++j) acc[p][j] = 0.0f;
             }
         }
+        if (valid < count) return;            // only masked positions follow
     }
-    flush(end < a.num_tokens and next == run);
 }
 
-// Runs that cross chunk borders. The CTA of the chunk in which such a run begins adds its pieces: eight warps take consecutive
-// ranges of them, and the eight sums are added in order.
-template <typename Out, int kElems>
-__global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_constant__ EmbGradArgs a) {
+// Runs that cross chunk borders: one CTA per (such run, column slice) adds its pieces, eight warps take consecutive ranges of
+// them, and the eight sums are added in order.
+template <typename Out, int kElems, bool kAccumulate>
+__global__ void __launch_bounds__(256, 6) embedding_grad_join_kernel(const __grid_constant__ EmbGradArgs a) {
     using namespace emb_detail;
     __shared__ float sums[8][32 * kElems];
-    const int lane = ptx::lane_id(), warp = threadIdx.x / 32, chunk = blockIdx.x;
-    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.num_tokens);
-    if (end >= a.num_tokens) return;
-    const int id = a.ids[end - 1];
-    if (id >= a.num_rows or a.ids[end] != id) return;                               // nothing goes on
-    if (begin > 0 and a.ids[begin] == id and a.ids[begin - 1] == id) return;        // it began earlier
-    // last chunk whose first position still belongs to the run
-    int lo = chunk + 1, hi = a.num_chunks - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.ids[int64_t(mid) * a.chunk] == id) lo = mid; else hi = mid - 1;
-    }
-    const int pieces = lo - chunk;                                                  // pieces in the chunks chunk + 1 .. lo
-    const int per_warp = math::ceil_div(pieces, 8);
-    const int first = min(warp * per_warp, pieces), last = min(first + per_warp, pieces);
+    const int lane = ptx::lane_id(), warp = threadIdx.x / 32;
     const int slices = math::ceil_div(a.hidden, 32 * kElems);
-    for (int slice = blockIdx.y; slice < slices; slice += gridDim.y) {
+    cudaGridDependencySynchronize();          // launched before the sums are done
+    const int64_t items = int64_t(*a.num_crossing) * slices;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int chunk = a.crossing[item / slices], slice = int(item % slices);
+        const int id = a.ids[int64_t(chunk + 1) * a.chunk];
+        // pieces: the chunks behind this one whose first position still belongs to the run, 32 looked at per step
+        int pieces = 0;
+        for (bool more = true; more; ) {
+            const int c = chunk + 1 + pieces + lane;
+            const unsigned same = __ballot_sync(0xffffffffu, c < a.num_chunks and a.ids[int64_t(c) * a.chunk] == id);
+            pieces += __popc(same);
+            more = same == 0xffffffffu;
+        }
+        const int per_warp = math::ceil_div(pieces, 8);
+        const int first = min(warp * per_warp, pieces), last = min(first + per_warp, pieces);
         const int column = (slice * 32 + lane) * kElems;
         float acc[kElems];
         #pragma unroll
         for (int j = 0; j < kElems; ++j) acc[j] = 0.0f;
         if (column < a.hidden) {
             if (warp == 0) {
-                const auto head = *reinterpret_cast<const Pack<float, kElems>*>(a.partial + (int64_t(chunk) * 2 + 1) * a.hidden + column);
-                #pragma unroll
-                for (int j = 0; j < kElems; ++j) acc[j] = head.v[j];
+                unpack<float, kElems>(load_written_pack<float, kElems>(a.partial + (int64_t(chunk) * 2 + 1) * a.hidden + column), acc);
             }
             #pragma unroll 4
             for (int i = first; i < last; ++i) {
-                const auto p = *reinterpret_cast<const Pack<float, kElems>*>(a.partial + (int64_t(chunk + 1 + i) * 2) * a.hidden + column);
+                float v[kElems];
+                unpack<float, kElems>(load_written_pack<float, kElems>(a.partial + (int64_t(chunk + 1 + i) * 2) * a.hidden + column), v);
                 #pragma unroll
-                for (int j = 0; j < kElems; ++j) acc[j] += p.v[j];
+                for (int j = 0; j < kElems; ++j) acc[j] += v[j];
             }
         }
         #pragma unroll
@@ -442,7 +604,9 @@ __global__ void __launch_bounds__(256) embedding_grad_join_kernel(const __grid_c
                 #pragma unroll
                 for (int j = 0; j < kElems; ++j) acc[j] += sums[w][lane * kElems + j];
             }
-            write_sum<Out, kElems>(a, id, column, acc);
+            Out* out = reinterpret_cast<Out*>(a.out) + int64_t(id) * a.out_stride + column;
+            if constexpr (kAccumulate) add_sum<kElems>(out, a.scale, acc, load_written_pack<float, kElems>(out));
+            else write_sum<Out, kElems>(out, a.scale, acc);
         }
         __syncthreads();
     }

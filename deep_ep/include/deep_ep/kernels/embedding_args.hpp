@@ -28,15 +28,19 @@ struct EmbSortArgs {
     int idx64;
     int num_tokens, num_rows;
     int digit_bits, num_passes;
-    int pass;                 // multi-CTA form: the pass of this launch
-    int keys_per_warp;        // contiguous keys of one warp (multiple of 32)
-    int *keys[2], *vals[2];   // ping-pong buffers [num_tokens]; pass p reads buffer (p + 1) % 2 (pass 0: `idx`) and writes p % 2
-    int* hist;                // multi-CTA form: [2^digit_bits][num_ctas] counts of this pass
+    int pass;                 // form of many launches: the pass of this one
+    int keys_per_warp;        // form of many launches: contiguous keys of one warp (multiple of 32)
+    int *keys[2], *vals[2];   // [num_tokens]; many launches: pass p reads buffer (p + 1) % 2 (pass 0: `idx`) and writes p % 2;
+                              // one launch: the result goes to buffer 0
+    int* hist;                // form of many launches: [num_ctas][2^digit_bits] counts of this pass
     uint32_t* touched;        // optional bitmap over the rows (bit set = the row receives a gradient), zeroed by pass 0
+    int* num_crossing;        // set to 0 for the kernels that follow
 };
 
-constexpr int kEmbSortThreads = 256;          // multi-CTA form: eight warps
-constexpr int kEmbSortSoloThreads = 1024;     // one-CTA form
+constexpr int kEmbSortThreads = 256;          // form of many launches: eight warps
+constexpr int kEmbClusterThreads = 1024;      // form of one launch: a cluster of up to eight CTAs ...
+constexpr int kEmbClusterMaxRounds = 8;       // ... with up to this many keys per thread
+constexpr int kEmbClusterDigitBits = 9;
 constexpr int kEmbMaxDigitBits = 10;
 
 // Sum of the gradient rows of every id over the sorted order, in two steps: chunks of `chunk` sorted positions are reduced
@@ -52,6 +56,7 @@ struct EmbGradArgs {
     int64_t out_stride;
     int accumulate;           // fp32 `out`: add to its contents; otherwise overwrite
     const uint32_t* touched;  // overwrite: rows without a set bit are written as zeros
+    int *num_crossing, *crossing;   // list of the chunks in which a run begins that goes on in the next
 };
 
 }  // namespace deep_ep::kernels

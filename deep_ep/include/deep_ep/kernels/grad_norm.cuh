@@ -5,8 +5,9 @@
 // and writes everything, and when the factor is 1 in place it touches nothing. It walks the chunks from the end, so
 // that what the first sweep read last is still in L2 (126 MB).
 //
-// Sums: the squares of 16 bytes of elements are added in fp32, everything above that in fp64. Squares that leave fp32's range
-// (an element beyond about 1e18, or all of them below 1e-14) are taken in fp64 instead, so neither huge nor tiny
+// Sums: the squares of 64 bytes of elements are added in fp32 (at most ten roundings on the way of each), everything above
+// that in fp64, whose units would otherwise be the bound for 16-bit gradients. Squares that leave fp32's range (an element
+// beyond about 1e18, or all of them below 1e-14) are taken in fp64 instead, so neither huge nor tiny
 // gradients lose the norm. Each CTA takes a fixed set of chunks and its sum has a fixed slot: the same bits every time.
 #pragma once
 
@@ -51,13 +52,17 @@ struct Unpacked {
 };
 
 template <typename T>
-EP_DEVICE double square_sum(const uint4& raw) {
+EP_DEVICE float square_sum(const uint4& raw) {
     const Unpacked<T> e(raw);
     float s = 0.0f;
     #pragma unroll
     for (int i = 0; i < Unpacked<T>::kCount; ++i) s = fmaf(e.v[i], e.v[i], s);
-    if (s > 1e-28f and s < 1e36f) return double(s);
-    double d = 0.0;                           // zeros, or a range that fp32 squares do not have (NaN and infinity included)
+    return s;
+}
+template <typename T>
+EP_DEVICE double square_sum_exact(const uint4& raw) {
+    const Unpacked<T> e(raw);
+    double d = 0.0;
     #pragma unroll
     for (int i = 0; i < Unpacked<T>::kCount; ++i) d += double(e.v[i]) * double(e.v[i]);
     return d;
@@ -83,10 +88,15 @@ __device__ __noinline__ double sum_range(const T* p, int n) {
         uint4 e[kAhead];
         #pragma unroll
         for (int u = 0; u < kAhead; ++u) e[u] = __ldg(body + i + u * kGradThreads);
-        #pragma unroll
-        for (int u = 0; u < kAhead; ++u) acc += square_sum<T>(e[u]);
+        const float s = (square_sum<T>(e[0]) + square_sum<T>(e[1])) + (square_sum<T>(e[2]) + square_sum<T>(e[3]));
+        if (s > 1e-28f and s < 1e36f) {
+            acc += double(s);
+        } else {                              // zeros, or a range that fp32 squares do not have (NaN and infinity included)
+            #pragma unroll 1
+            for (int u = 0; u < kAhead; ++u) acc += square_sum_exact<T>(u == 0 ? e[0] : u == 1 ? e[1] : u == 2 ? e[2] : e[3]);
+        }
     }
-    for (; i < packs; i += kGradThreads) acc += square_sum<T>(__ldg(body + i));
+    for (; i < packs; i += kGradThreads) acc += square_sum_exact<T>(__ldg(body + i));
     return acc;
 }
 
@@ -194,7 +204,7 @@ EP_DEVICE float clip_factor(float norm, float max_norm) {
 }  // namespace grad_detail
 
 template <int kTensors>
-__global__ void __launch_bounds__(kGradThreads, 2) grad_square_sum_kernel(const __grid_constant__ GradTable<kTensors> t, GradNormArgs a) {
+__global__ void __launch_bounds__(kGradThreads, kGradCtasPerSm) grad_square_sum_kernel(const __grid_constant__ GradTable<kTensors> t, GradNormArgs a) {
     using namespace grad_detail;
     cudaTriggerProgrammaticLaunchCompletion();
     const int chunks = t.first_chunk[t.num_tensors];
@@ -224,7 +234,7 @@ __global__ void __launch_bounds__(kGradThreads) grad_norm_finish_kernel(const __
 }
 
 template <int kTensors>
-__global__ void __launch_bounds__(kGradThreads, 2) grad_clip_kernel(const __grid_constant__ GradTable<kTensors> t,
+__global__ void __launch_bounds__(kGradThreads, 4) grad_clip_kernel(const __grid_constant__ GradTable<kTensors> t,
                                                                     const __grid_constant__ GradClipArgs a) {
     using namespace grad_detail;
     cudaGridDependencySynchronize();

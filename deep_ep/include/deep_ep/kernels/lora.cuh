@@ -108,6 +108,71 @@ EP_DEVICE int ld_cluster_int(uint32_t addr) {
     return v;
 }
 
+// A row of the accumulator (`columns` fp32, a multiple of 32) to shared memory at `to`, possibly of another CTA of the cluster.
+// Its 16-byte units are swizzled by the row, so that neither side has bank conflicts. Called by a whole warp.
+EP_DEVICE void send_part(uint32_t to, uint32_t taddr, int columns, int row, bool valid) {
+    for (int c = 0; c < columns; c += 32) {
+        uint32_t r[32];
+        tc::tmem_ld_32x32(taddr + c, r);
+        tc::wait_ld();
+        if (not valid) continue;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(to + (((c / 4 + i) ^ (row & 7)) << 4)), "r"(r[4 * i]), "r"(r[4 * i + 1]), "r"(r[4 * i + 2]), "r"(r[4 * i + 3]) : "memory");
+    }
+}
+// Adds columns c .. c + 7 of a row over the parts of all ranks, in rank order
+EP_DEVICE void add_parts(float (&v)[8], const uint8_t* parts, int part_bytes, int ranks, int row_offset, int c, int row) {
+    #pragma unroll 4
+    for (int q = 0; q < ranks; ++q) {
+        const uint8_t* line = parts + q * part_bytes + row_offset;
+        const float4 x = *reinterpret_cast<const float4*>(line + (((c / 4) ^ (row & 7)) << 4));
+        const float4 y = *reinterpret_cast<const float4*>(line + (((c / 4 + 1) ^ (row & 7)) << 4));
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+}
+EP_DEVICE void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(ptx::float2_to_bf16x2(v[0], v[1]), ptx::float2_to_bf16x2(v[2], v[3]),
+                                              ptx::float2_to_bf16x2(v[4], v[5]), ptx::float2_to_bf16x2(v[6], v[7]));
+}
+
+// One lane of a converged warp, always the same. The loops that feed the tensor cores are run by a whole warp and let this lane
+// issue: their counters and descriptors then stay in uniform registers, which is what the instructions take. Run by a single
+// lane of a diverged warp, a step of such a loop cost about twice as much.
+EP_DEVICE bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
+}
+// Wait for a phase: false when somebody gave up (`error_flag`), or when this wait itself ran out (about 10 s), which sets the flag.
+// The flag is looked at only when the barrier is not ready.
+EP_DEVICE bool wait(uint64_t* bar, uint32_t parity, volatile int* error_flag) {
+    if (ptx::mbarrier_try_wait(bar, parity)) return true;
+    #pragma unroll 1
+    for (int i = 0; i < 100; ++i) {
+        if (*error_flag) return false;
+        if (ptx::mbarrier_wait(bar, parity, 1 << 20, 100000000ull)) return true;
+    }
+    *error_flag = 1;
+    return false;
+}
+EP_DEVICE bool wait_all_lanes(uint64_t* bar, uint32_t parity, volatile int* error_flag) {
+    return __all_sync(0xffffffffu, wait(bar, parity, error_flag));
+}
+// this thread's copies into the last stages of a ring have landed
+EP_DEVICE void drain(uint64_t* full_bar, int issued, int stages) {
+    for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbarrier_wait(&full_bar[i % stages], (i / stages) & 1);
+}
+// Position in a ring of stages
+struct Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    EP_DEVICE void advance(int stages) {
+        if (++slot == stages) slot = 0, phase ^= 1;
+    }
+};
+
 EP_DEVICE uint8_t* align_1024(uint8_t* p) { return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023)); }
 
 EP_DEVICE void report(bool failed, int* status) {
@@ -135,18 +200,18 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     __shared__ volatile int error_flag;
 
     cudaTriggerProgrammaticLaunchCompletion();
-    const int warp = threadIdx.x / 32, lane = ptx::lane_id();
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = blockIdx.x % cluster;
     const int chunk = (blockIdx.x / cluster) % a.num_chunks, tile = blockIdx.x / cluster / a.num_chunks;
     const int m0 = tile * kLoraTileRows;
     // columns of the accumulator per adapter: the rank, padded (by zeros that the TMA fills in) to what the operand's layout has
-    const int rp = math::align(a.rows.rank, a.mn_major ? 64 : 16), stages = a.num_stages;
+    const int rp = math::align(a.rows.rank, a.mn_major ? 64 : 16);
     uint8_t* smem = align_1024(smem_raw);
     constexpr uint32_t kXBytes = kLoraTileRows * kLoraBlockK * 2;
     const uint32_t slot_bytes = rp * 128u;    // one adapter's block of a stage
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1);
+        for (int s = 0; s < kMaxStages; ++s) ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1);
         ptx::mbarrier_init(&done_bar, 1);
         ptx::fence_mbarrier_init();
         error_flag = 0;
@@ -176,6 +241,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     __syncthreads();
     const int n = list_size;
     if (n == 0) return;                       // the same for all CTAs of the cluster
+    // the ring is cut by the adapters that are there: fewer adapters, more stages in flight
+    const int stage_bytes = int(kXBytes + n * slot_bytes), stages = min(kMaxStages, a.ring_bytes / stage_bytes);
     uint32_t columns = 32;
     while (columns < uint32_t(a.chunk * rp)) columns *= 2;
     if (warp == 1) tc::tmem_alloc(&tmem_slot, columns);
@@ -188,45 +255,45 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     const int kb0 = min(rank * per, blocks), kb1 = min(kb0 + per, blocks);
 
     if (warp == 0) {
-        if (lane == 0) {
-            int issued = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                const int s = issued % stages;
-                if (not ptx::mbarrier_wait(&empty_bar[s], ((issued / stages) & 1) ^ 1)) { error_flag = 1; break; }
-                uint8_t* stage = smem + size_t(s) * a.stage_bytes;
-                ptx::mbarrier_arrive_expect_tx(&full_bar[s], kXBytes + n * slot_bytes);
-                tc::tma_load_2d(stage, &map_x, kb * kLoraBlockK, m0, &full_bar[s]);
+        Ring ring;
+        int issued = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++issued, ring.advance(stages)) {
+            if (not wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag)) break;
+            if (elect_one()) {
+                uint64_t* bar = &full_bar[ring.slot];
+                uint8_t* stage = smem + size_t(ring.slot) * stage_bytes;
+                ptx::mbarrier_arrive_expect_tx(bar, kXBytes + n * slot_bytes);
+                tc::tma_load_2d(stage, &map_x, kb * kLoraBlockK, m0, bar);
                 for (int j = 0; j < n; ++j) {
                     uint8_t* dst = stage + kXBytes + j * slot_bytes;
                     if (a.mn_major) {
-                        for (int c = 0; c * 64 < rp; ++c) tc::tma_load_3d(dst + c * 8192, &map_a, c * 64, kb * kLoraBlockK, list[j], &full_bar[s]);
+                        for (int c = 0; c * 64 < rp; ++c) tc::tma_load_3d(dst + c * 8192, &map_a, c * 64, kb * kLoraBlockK, list[j], bar);
                     } else {
-                        tc::tma_load_3d(dst, &map_a, kb * kLoraBlockK, 0, list[j], &full_bar[s]);
+                        tc::tma_load_3d(dst, &map_a, kb * kLoraBlockK, 0, list[j], bar);
                     }
                 }
             }
-            // its own copies have landed before this thread leaves, also when somebody gave up
-            for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbarrier_wait(&full_bar[i % stages], (i / stages) & 1);
         }
+        drain(full_bar, issued, stages);      // its own copies have landed before this warp leaves, also when somebody gave up
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, kLoraTileRows, rp, false, a.mn_major);
-            const uint32_t b_lead = a.mn_major ? 8192 : 16, b_k = (a.mn_major ? 2048 : 32) >> 4;
-            const uint64_t desc_x = tc::make_smem_desc(smem, 16, 1024), desc_a = tc::make_smem_desc(smem + kXBytes, b_lead, 1024);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int i = kb - kb0, s = i % stages;
-                if (error_flag or not ptx::mbarrier_wait(&full_bar[s], (i / stages) & 1)) { error_flag = 1; break; }
-                tc::fence_after_thread_sync();
-                const uint64_t step = uint64_t(s) * (a.stage_bytes >> 4);
+        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, kLoraTileRows, rp, false, a.mn_major);
+        const uint32_t b_lead = a.mn_major ? 8192 : 16, b_k = (a.mn_major ? 2048 : 32) >> 4;
+        const uint64_t desc_x = tc::make_smem_desc(smem, 16, 1024), desc_a = tc::make_smem_desc(smem + kXBytes, b_lead, 1024);
+        Ring ring;
+        for (int kb = kb0; kb < kb1; ++kb, ring.advance(stages)) {
+            wait(&full_bar[ring.slot], ring.phase, &error_flag);
+            tc::fence_after_thread_sync();
+            if (elect_one()) {
+                const uint64_t step = uint64_t(ring.slot) * (stage_bytes >> 4);
                 for (int j = 0; j < n; ++j) {
                     #pragma unroll
                     for (int k = 0; k < kLoraBlockK / 16; ++k)
-                        tc::mma_f16(tmem + j * rp, desc_x + step + k * 2, desc_a + step + uint64_t(j) * (slot_bytes >> 4) + k * b_k, idesc, i > 0 or k > 0);
+                        tc::mma_f16(tmem + j * rp, desc_x + step + k * 2, desc_a + step + uint64_t(j) * (slot_bytes >> 4) + k * b_k, idesc, kb > kb0 or k > 0);
                 }
-                tc::commit(&empty_bar[s]);
+                tc::commit(&empty_bar[ring.slot]);
             }
-            tc::commit(&done_bar);
         }
+        if (elect_one()) tc::commit(&done_bar);
     }
     // ---- every row picks its adapter's columns: straight to memory, or through shared memory and the cluster
     const int pitch = rp + 4;                 // floats per row of the staging area
@@ -237,7 +304,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         int slot = -1;
         for (int j = 0; j < n; ++j)
             if (list[j] == mine) slot = j;
-        if (not ptx::mbarrier_wait(&done_bar, 0)) error_flag = 1;
+        wait_all_lanes(&done_bar, 0, &error_flag);
         tc::fence_after_thread_sync();
         const float scale = slot >= 0 ? a.scaling[mine] : 0.0f;
         for (int j = 0; j < n; ++j) {
@@ -289,49 +356,122 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     if (threadIdx.x == 0) report(error_flag != 0, a.rows.status);
 }
 
+// The same for a few rows (decode): one CTA per (row, four rank columns), plain fp32 products. A tile of the kernel above would
+// be mostly empty, and its setup (tensor maps, tensor memory, a cluster) costs more than these products; the adapters are
+// read once per row, from L2. Its time is that of round trips to memory, those for its instructions among them: between two
+// calls a decode step streams more weights than L2 holds, so the code is cold. Hence many threads with a short loop each
+// instead of unrolled ones (which took 8.6 us for one row of 7168, of which 5 went to fetching instructions).
+__global__ void __launch_bounds__(512, 3)
+lora_shrink_rows_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a_all, const __grid_constant__ LoraShrinkArgs a) {
+    using namespace lora_detail;
+    constexpr int kColumns = 4, kThreads = 512;
+    __shared__ float sums[kThreads / 32][kColumns];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int groups = a.rows.rank / kColumns, row = blockIdx.x / groups, r0 = blockIdx.x % groups * kColumns;
+    const int warp = threadIdx.x / 32, lane = ptx::lane_id();
+    const int e = adapter_of(a.rows, row);
+    if (a.presence != nullptr and r0 == 0 and row % kLoraTileRows == 0) {
+        for (int p = warp; p < a.rows.num_adapters; p += kThreads / 32) {
+            bool here = false;
+            #pragma unroll 1
+            for (int i = 0; i < 4; ++i) here = here or adapter_of(a.rows, row + lane + 32 * i) == p;
+            here = __any_sync(0xffffffffu, here);
+            if (lane == 0) a.presence[int64_t(row / kLoraTileRows) * a.rows.num_adapters + p] = here;
+        }
+    }
+    if (e < 0) return;
+    const float scale = a.scaling[e];
+    const __nv_bfloat16* xr = x + int64_t(row) * a.k;
+    const __nv_bfloat16* ae = a_all + int64_t(e) * a.rows.rank * a.k;
+    float acc[kColumns] = {};
+    if (a.mn_major) {
+        // A_e [k, rank]: a thread takes single k with the columns of this CTA
+        #pragma unroll 2
+        for (int k = threadIdx.x; k < a.k; k += kThreads) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(ae + int64_t(k) * a.rows.rank + r0));
+            const float v = __bfloat162float(xr[k]);
+            const float2 f = ptx::bf16x2_to_float2(u.x), g = ptx::bf16x2_to_float2(u.y);
+            acc[0] = fmaf(v, f.x, acc[0]), acc[1] = fmaf(v, f.y, acc[1]), acc[2] = fmaf(v, g.x, acc[2]), acc[3] = fmaf(v, g.y, acc[3]);
+        }
+    } else {
+        // A_e [rank, k]: a thread takes eight k of each of the rows
+        ae += int64_t(r0) * a.k;
+        #pragma unroll 1
+        for (int k = threadIdx.x * 8; k < a.k; k += kThreads * 8) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(xr + k));
+            uint4 v[kColumns];
+            #pragma unroll
+            for (int r = 0; r < kColumns; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(ae + int64_t(r) * a.k + k));
+            const uint32_t xw[4] = {u.x, u.y, u.z, u.w};
+            #pragma unroll
+            for (int r = 0; r < kColumns; ++r) {
+                const uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+                #pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 f = ptx::bf16x2_to_float2(w[q]), g = ptx::bf16x2_to_float2(xw[q]);
+                    acc[r] = fmaf(g.x, f.x, acc[r]), acc[r] = fmaf(g.y, f.y, acc[r]);
+                }
+            }
+        }
+    }
+    // four sums over 32 lanes: two steps halve the number of sums a lane carries (lane bits 4 and 3 say which), three add the rest
+    const bool upper = lane & 16, odd = lane & 8;
+    const float p0 = (upper ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, upper ? acc[0] : acc[2], 16);
+    const float p1 = (upper ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, upper ? acc[1] : acc[3], 16);
+    float sum = (odd ? p1 : p0) + __shfl_xor_sync(0xffffffffu, odd ? p0 : p1, 8);
+    #pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane % 8 == 0) sums[warp][lane / 8] = sum;
+    __syncthreads();
+    if (threadIdx.x < kColumns) {
+        float total = 0.0f;
+        #pragma unroll 4
+        for (int w = 0; w < kThreads / 32; ++w) total += sums[w][threadIdx.x];
+        a.t[int64_t(row) * a.rows.rank + r0 + threadIdx.x] = total * scale;
+    }
+}
+
 // ---------------------------------------------------------------------------------------- shared product + adapters
-// Tiles of 128 rows x BN columns. Many tiles: persistent CTAs, two accumulators in tensor memory, so that the stores of one tile
-// overlap the products of the next. Few tiles (decode): a cluster shares the tile's contraction, so that all SMs pull on W,
-// and adds its parts through distributed shared memory in rank order.
+// Tiles of 128 rows x BN columns.
 //   warp 0      TMA producer: K blocks of x and W, then the V blocks of the tile's adapters
 //   warp 1      MMA issuer
 //   warps 2-5   epilogue
 //   warps 6-9   writers: the A operand of the adapters' K blocks (t as bf16 hi | lo, zeros in the rows of others)
+// Many tiles: persistent CTAs, two accumulators in tensor memory, so that the stores of one tile overlap the products of the
+// next. Few tiles (decode): a cluster shares the tile's contraction, so that all SMs pull on W; its CTAs send their parts
+// of a row to the CTA that owns the row, which adds them in rank order.
+constexpr int kLoraSplitBytes = 128 * 128 * 4;             // parts of the rows a CTA owns, BN = 128
+
+template <int BN>
+constexpr int lora_gemm_stages() { return BN == 256 ? 4 : 5; }
+template <int BN>
+constexpr int lora_gemm_smem_bytes() {
+    return lora_gemm_stages<BN>() * (kLoraTileRows + BN) * kLoraBlockK * 2 + (BN == 256 ? 4 * 4096 : kLoraSplitBytes) + 1024;
+}
+
 template <int BN>
 __global__ void __launch_bounds__(320, 1)
 lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_y, const __grid_constant__ LoraGemmArgs a) {
     using namespace lora_detail;
     extern __shared__ uint8_t smem_raw[];
-    constexpr int kStages = BN == 256 ? 4 : 6, kGroupM = 16;
+    constexpr int kStages = lora_gemm_stages<BN>(), kGroupM = 16;
     constexpr uint32_t kABytes = kLoraTileRows * kLoraBlockK * 2, kBBytes = BN * kLoraBlockK * 2;
-    constexpr int kPoisonSlots = 8;           // more tiles than the ring can run ahead
+    constexpr int kPoisonSlots = 8;           // more tiles than the writers can be ahead of the epilogue
     __shared__ uint64_t full_bar[kStages], empty_bar[kStages], grant_bar[kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ uint64_t list_full_bar[2], list_empty_bar[2];
+    __shared__ int list[2][kLoraTileRows], list_size[2];       // the adapters of a tile
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int error_flag, poison[kPoisonSlots];
 
-    const int warp = threadIdx.x / 32, lane = ptx::lane_id();
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = cluster > 1 ? int(blockIdx.x) % cluster : 0;
     const int num_tiles = a.m_tiles * a.n_tiles;
     const int first_tile = int(blockIdx.x) / cluster, tile_step = int(gridDim.x) / cluster;
+    const bool split = cluster > 1;                            // parts are exchanged; one tile per cluster
     uint8_t* smem_a = align_1024(smem_raw);
     uint8_t* smem_b = smem_a + kStages * kABytes;
-    uint8_t* smem_out = smem_b + kStages * kBBytes;            // 4 x 4 KB, one chunk of 32 rows x 64 columns per epilogue warp
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s)
-            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&grant_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 4);
-        for (int i = 0; i < 2; ++i) ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 4);
-        ptx::fence_mbarrier_init();
-        error_flag = 0;
-        for (int i = 0; i < kPoisonSlots; ++i) poison[i] = 0;
-        tc::prefetch_tensormap(&map_x), tc::prefetch_tensormap(&map_w), tc::prefetch_tensormap(&map_v), tc::prefetch_tensormap(&map_y);
-    }
-    if (warp == 1) tc::tmem_alloc(&tmem_slot, 2 * BN);
-    tc::fence_before_thread_sync();
-    __syncthreads();
-    tc::fence_after_thread_sync();
-    const uint32_t tmem = tmem_slot;
+    uint8_t* smem_out = smem_b + kStages * kBBytes;            // a chunk of 32 rows x 64 columns per epilogue warp, or the parts
 
     const int blocks = math::ceil_div(a.k, kLoraBlockK), per = math::ceil_div(blocks, cluster);
     const int kb0 = min(rank * per, blocks), kb1 = min(kb0 + per, blocks);        // never empty, see the launcher
@@ -343,186 +483,41 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         const int local = tile - group * kGroupM * a.n_tiles;
         m0 = (first_m + local % gm) * kLoraTileRows, n0 = local / gm * BN;
     };
+    const auto load_block = [&](unsigned s, int m0, int n0, int kb) {
+        ptx::mbarrier_arrive_expect_tx(&full_bar[s], kABytes + kBBytes);
+        const int k0 = kb * kLoraBlockK;
+        tc::tma_load_2d(smem_a + s * kABytes, &map_x, k0, m0, &full_bar[s]);
+        uint8_t* sb = smem_b + s * kBBytes;
+        if (a.mn_major) {
+            #pragma unroll
+            for (int i = 0; i < BN / 64; ++i) tc::tma_load_2d(sb + i * 8192, &map_w, n0 + 64 * i, k0, &full_bar[s]);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d(sb + i * 16384, &map_w, k0, n0 + 128 * i, &full_bar[s]);
+        }
+    };
 
-    if (warp == 0) {
-        // ------------------------------------------------------------------ TMA producer
-        unsigned it = 0;
-        bool ok = true;
-        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step) {
-            int m0, n0;
-            origin(tile, m0, n0);
-            TileAdapters rows;
-            rows.load(a.rows, m0, lane);
-            if (lane == 0) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const unsigned s = it % kStages;
-                    if (error_flag or not ptx::mbarrier_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1)) { error_flag = 1, ok = false; break; }
-                    ptx::mbarrier_arrive_expect_tx(&full_bar[s], kABytes + kBBytes);
-                    const int k0 = kb * kLoraBlockK;
-                    tc::tma_load_2d(smem_a + s * kABytes, &map_x, k0, m0, &full_bar[s]);
-                    uint8_t* sb = smem_b + s * kBBytes;
-                    if (a.mn_major) {
-                        #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tc::tma_load_2d(sb + i * 8192, &map_w, n0 + 64 * i, k0, &full_bar[s]);
-                    } else {
-                        #pragma unroll
-                        for (int i = 0; i < BN / 128; ++i) tc::tma_load_2d(sb + i * 16384, &map_w, k0, n0 + 128 * i, &full_bar[s]);
-                    }
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0), it = __shfl_sync(0xffffffffu, it, 0);
-            int turn = 0;
-            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
-                if (turn % cluster != rank) continue;
-                for (int c = 0; c < rank_chunks and ok; ++c) {
-                    const unsigned s = it % kStages;
-                    if (lane == 0) {
-                        if (error_flag or not ptx::mbarrier_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1)) {
-                            error_flag = 1, ok = false;
-                        } else {
-                            ptx::mbarrier_arrive(&grant_bar[s]);            // the writers may fill the A slot
-                            ptx::mbarrier_arrive_expect_tx(&full_bar[s], kBBytes);
-                            uint8_t* sb = smem_b + s * kBBytes;
-                            if (a.mn_major) {
-                                #pragma unroll
-                                for (int i = 0; i < BN / 64; ++i) tc::tma_load_3d(sb + i * 8192, &map_v, n0 + 64 * i, 32 * c, e, &full_bar[s]);
-                            } else {
-                                #pragma unroll
-                                for (int i = 0; i < BN / 128; ++i) tc::tma_load_3d(sb + i * 16384, &map_v, 32 * c, n0 + 128 * i, e, &full_bar[s]);
-                            }
-                        }
-                    }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                    it += ok;
-                }
-            }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s)
+            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&grant_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 4);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 4);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], 2);
         }
-        // its own copies have landed before this warp leaves, also when somebody gave up
-        if (lane == 0)
-            for (unsigned i = it > kStages ? it - kStages : 0; i < it; ++i) ptx::mbarrier_wait(&full_bar[i % kStages], (i / kStages) & 1);
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
-        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, kLoraTileRows, BN, false, a.mn_major);
-        const uint32_t b_lead = a.mn_major ? 8192 : 16, b_k = (a.mn_major ? 2048 : 32) >> 4;
-        const uint64_t desc_a0 = tc::make_smem_desc(smem_a, 16, 1024), desc_b0 = tc::make_smem_desc(smem_b, b_lead, 1024);
-        unsigned it = 0, ext_phase = 0;
-        int local = 0;
-        bool ok = true;
-        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
-            int m0, n0;
-            origin(tile, m0, n0);
-            TileAdapters rows;
-            rows.load(a.rows, m0, lane);
-            const int acc = local & 1;
-            const uint32_t d = tmem + acc * BN;
-            if (lane == 0) {
-                if (not ptx::mbarrier_wait(&tmem_empty_bar[acc], ((local >> 1) & 1) ^ 1)) error_flag = 1, ok = false;
-                tc::fence_after_thread_sync();
-                for (int kb = kb0; kb < kb1 and ok; ++kb, ++it) {
-                    const unsigned s = it % kStages;
-                    if (error_flag or not ptx::mbarrier_wait(&full_bar[s], (it / kStages) & 1)) { error_flag = 1, ok = false; break; }
-                    tc::fence_after_thread_sync();
-                    const uint64_t da = desc_a0 + uint64_t(s * (kABytes >> 4)), db = desc_b0 + uint64_t(s * (kBBytes >> 4));
-                    #pragma unroll
-                    for (int k = 0; k < kLoraBlockK / 16; ++k) tc::mma_f16(d, da + k * 2, db + k * b_k, idesc, kb > kb0 or k > 0);
-                    tc::commit(&empty_bar[s]);
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0), it = __shfl_sync(0xffffffffu, it, 0);
-            int turn = 0;
-            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
-                if (turn % cluster != rank) continue;
-                for (int c = 0; c < rank_chunks and ok; ++c, ++it) {
-                    const unsigned s = it % kStages;
-                    if (lane == 0) {
-                        if (error_flag or not ptx::mbarrier_wait(&full_bar[s], (it / kStages) & 1) or
-                            not ptx::mbarrier_wait(&ext_bar[s], (ext_phase >> s) & 1)) {
-                            error_flag = 1, ok = false;
-                        } else {
-                            tc::fence_after_thread_sync();
-                            const uint64_t da = desc_a0 + uint64_t(s * (kABytes >> 4)), db = desc_b0 + uint64_t(s * (kBBytes >> 4));
-                            for (int k = 0; k < 2 and 32 * c + 16 * k < a.rows.rank; ++k) {
-                                tc::mma_f16(d, da + k * 2, db + k * b_k, idesc, true);             // hi
-                                tc::mma_f16(d, da + 4 + k * 2, db + k * b_k, idesc, true);         // lo
-                            }
-                            tc::commit(&empty_bar[s]);
-                        }
-                    }
-                    ext_phase ^= 1u << s;
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
-                }
-            }
-            if (lane == 0 and ok) tc::commit(&tmem_full_bar[acc]);
-        }
-    } else if (warp >= 6) {
-        // ------------------------------------------------------------------ writers of the adapters' A operand
-        cudaGridDependencySynchronize();      // t comes from the kernel before, which this one does not wait for until here
-        const int row = threadIdx.x - 192;
-        // These warps do not follow the ring through the K blocks of x, so they cannot tell from a slot's own barriers (which
-        // show a phase's parity only) whether it is free for THIS block: the producer, which can, grants it.
-        unsigned it = 0, granted = 0;
-        int local = 0;
-        bool ok = true;
-        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
-            int m0, n0;
-            origin(tile, m0, n0);
-            TileAdapters rows;
-            rows.load(a.rows, m0, lane);
-            const int mine = adapter_of(a.rows, m0 + row);
-            it += kb1 - kb0;
-            int turn = 0;
-            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
-                if (turn % cluster != rank) continue;
-                const bool shared_tile = rows.others_than(e);
-                for (int c = 0; c < rank_chunks and ok; ++c, ++it) {
-                    const unsigned s = it % kStages, phase = (it / kStages) & 1;
-                    float v[4][8];
-                    #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const bool there = mine == e and 32 * c + 8 * u < a.rows.rank;
-                        if (there) load8(a.t + int64_t(m0 + row) * a.rows.rank + 32 * c + 8 * u, v[u]);
-                        #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[u][j] = there ? v[u][j] : 0.0f;
-                    }
-                    ok = ptx::mbarrier_wait(&grant_bar[s], (granted >> s) & 1);
-                    granted ^= 1u << s;
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (not ok) { error_flag = 1; break; }
-                    uint8_t* line = smem_a + s * kABytes + row * 128;
-                    #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint4 hi, lo;
-                        split8(v[u], hi, lo);
-                        // 16-byte unit u of row r sits at unit u ^ (r % 8) of its 128-byte line
-                        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = hi;
-                        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = lo;
-                    }
-                    if (shared_tile) {
-                        // infinities and NaN of this adapter must not meet the zeros of other rows
-                        ok = ok and ptx::mbarrier_wait(&full_bar[s], phase);
-                        uint8_t* sb = smem_b + s * kBBytes;
-                        // the part of the block that the products read: 32 columns of BN lines, or 32 lines of each 64-column block
-                        const auto look = [&](uint8_t* at) {
-                            uint4* unit = reinterpret_cast<uint4*>(at);
-                            if (has_non_finite(*unit)) *unit = make_uint4(0, 0, 0, 0), poison[local % kPoisonSlots] = local + 1;
-                        };
-                        if (a.mn_major) {
-                            for (int i = row; i < BN / 64 * 32 * 8; i += 128) look(sb + (i / 256) * 8192 + (i % 256) * 16);
-                        } else {
-                            for (int i = row; i < BN * 4; i += 128) look(sb + (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4));
-                        }
-                    }
-                    ptx::fence_proxy_async_smem();
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (not ok) { error_flag = 1; break; }
-                    if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
-                }
-            }
-            ok = ok and not __any_sync(0xffffffffu, error_flag != 0);
-        }
+        ptx::fence_mbarrier_init();
+        error_flag = 0;
+        for (int i = 0; i < kPoisonSlots; ++i) poison[i] = 0;
     }
+    if (threadIdx.x == 64) tc::prefetch_tensormap(&map_x), tc::prefetch_tensormap(&map_w), tc::prefetch_tensormap(&map_v), tc::prefetch_tensormap(&map_y);
+    if (warp == 1) tc::tmem_alloc(&tmem_slot, split ? BN : 2 * BN);
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    tc::fence_after_thread_sync();
+    const uint32_t tmem = tmem_slot;
+    if (split) tc::cluster_arrive();          // (waited for before the first access to another CTA's shared memory)
 
-    // products of an adapter's infinities and NaN (whole units of eight V elements that hold one) with this row's t
+    // product of this row's t with what the writers have kept from the tensor cores at column n: infinities and NaN of the row's
+    // adapter, by whole units of eight V elements
     const auto poisoned = [&](int row, int n) {
         const int e = adapter_of(a.rows, row);
         if (e < 0) return 0.0f;
@@ -544,6 +539,176 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         return sum;
     };
 
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer
+        Ring ring;
+        int issued = 0, local = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
+            int m0, n0;
+            origin(tile, m0, n0);
+            for (int kb = kb0; kb < kb1 and ok; ++kb) {
+                ok = wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag);
+                if (not ok) break;
+                if (elect_one()) load_block(ring.slot, m0, n0, kb);
+                ++issued, ring.advance(kStages);
+            }
+            const int slot = local & 1;
+            ok = ok and wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
+            if (not ok) break;
+            const int size = list_size[slot];
+            for (int i = rank; i < size and ok; i += cluster) {
+                const int e = list[slot][i];
+                for (int c = 0; c < rank_chunks; ++c) {
+                    ok = wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag);
+                    if (not ok) break;
+                    if (elect_one()) {
+                        uint64_t* bar = &full_bar[ring.slot];
+                        ptx::mbarrier_arrive(&grant_bar[ring.slot]);    // the writers may fill the A slot
+                        ptx::mbarrier_arrive_expect_tx(bar, kBBytes);
+                        uint8_t* sb = smem_b + ring.slot * kBBytes;
+                        if (a.mn_major) {
+                            #pragma unroll
+                            for (int j = 0; j < BN / 64; ++j) tc::tma_load_3d(sb + j * 8192, &map_v, n0 + 64 * j, 32 * c, e, bar);
+                        } else {
+                            #pragma unroll
+                            for (int j = 0; j < BN / 128; ++j) tc::tma_load_3d(sb + j * 16384, &map_v, 32 * c, n0 + 128 * j, e, bar);
+                        }
+                    }
+                    ++issued, ring.advance(kStages);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
+        }
+        drain(full_bar, issued, kStages);     // its own copies have landed before this warp leaves, also when somebody gave up
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, kLoraTileRows, BN, false, a.mn_major);
+        const uint32_t b_lead = a.mn_major ? 8192 : 16, b_k = (a.mn_major ? 2048 : 32) >> 4;
+        const uint64_t desc_a0 = tc::make_smem_desc(smem_a, 16, 1024), desc_b0 = tc::make_smem_desc(smem_b, b_lead, 1024);
+        Ring ring;
+        unsigned ext_phase = 0;
+        int local = 0;
+        for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++local) {
+            const int acc = local & 1, slot = local & 1;
+            const uint32_t d = tmem + acc * BN;
+            wait(&tmem_empty_bar[acc], ((local >> 1) & 1) ^ 1, &error_flag);
+            tc::fence_after_thread_sync();
+            for (int kb = kb0; kb < kb1; ++kb, ring.advance(kStages)) {
+                wait(&full_bar[ring.slot], ring.phase, &error_flag);
+                tc::fence_after_thread_sync();
+                if (elect_one()) {
+                    const uint64_t da = desc_a0 + uint64_t(ring.slot * (kABytes >> 4)), db = desc_b0 + uint64_t(ring.slot * (kBBytes >> 4));
+                    #pragma unroll
+                    for (int k = 0; k < kLoraBlockK / 16; ++k) tc::mma_f16(d, da + k * 2, db + k * b_k, idesc, kb > kb0 or k > 0);
+                    tc::commit(&empty_bar[ring.slot]);
+                }
+            }
+            const int size = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag) ? list_size[slot] : 0;
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
+            for (int i = rank; i < size; i += cluster) {
+                for (int c = 0; c < rank_chunks; ++c, ring.advance(kStages)) {
+                    wait(&full_bar[ring.slot], ring.phase, &error_flag);
+                    wait(&ext_bar[ring.slot], (ext_phase >> ring.slot) & 1, &error_flag);
+                    ext_phase ^= 1u << ring.slot;
+                    tc::fence_after_thread_sync();
+                    if (elect_one()) {
+                        const uint64_t da = desc_a0 + uint64_t(ring.slot * (kABytes >> 4)), db = desc_b0 + uint64_t(ring.slot * (kBBytes >> 4));
+                        for (int k = 0; k < 2 and 32 * c + 16 * k < a.rows.rank; ++k) {
+                            tc::mma_f16(d, da + k * 2, db + k * b_k, idesc, true);             // hi
+                            tc::mma_f16(d, da + 4 + k * 2, db + k * b_k, idesc, true);         // lo
+                        }
+                        tc::commit(&empty_bar[ring.slot]);
+                    }
+                }
+            }
+            if (elect_one()) tc::commit(&tmem_full_bar[acc]);
+        }
+    } else if (warp >= 6) {
+        // ------------------------------------------------------------------ writers of the adapters' A operand
+        cudaGridDependencySynchronize();      // t comes from the kernel before, which this one does not wait for until here
+        const int row = threadIdx.x - 192;
+        // These warps do not follow the ring through the K blocks of x, so they cannot tell from a slot's own barriers (which
+        // show a phase's parity only) whether it is free for THIS block: the producer, which can, grants it.
+        unsigned it = 0, granted = 0;
+        int local = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
+            int m0, n0;
+            origin(tile, m0, n0);
+            TileAdapters rows;
+            rows.load(a.rows, m0, lane);
+            const int mine = adapter_of(a.rows, m0 + row), slot = local & 1;
+            if (warp == 6) {
+                // the tile's adapters for the producer and the MMA issuer
+                ok = wait_all_lanes(&list_empty_bar[slot], ((local >> 1) & 1) ^ 1, &error_flag);
+                int size = 0;
+                for (int e = rows.next(-1); e != kNone; e = rows.next(e), ++size)
+                    if (lane == 0) list[slot][size] = e;
+                if (lane == 0) list_size[slot] = size;
+                if (not ok) break;
+                if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
+            }
+            it += kb1 - kb0;
+            // this row's t, 32 columns as bf16 hi and lo: read before the ring has room for it, and once per tile when the rank
+            // is not larger (with many adapters per tile, a read per adapter would be a round trip to L2 each)
+            uint4 hi[4], lo[4];
+            const auto read = [&](int c) {
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float v[8];
+                    const bool there = mine >= 0 and 32 * c + 8 * u < a.rows.rank;
+                    if (there) load8(a.t + int64_t(m0 + row) * a.rows.rank + 32 * c + 8 * u, v);
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = there ? v[j] : 0.0f;
+                    split8(v, hi[u], lo[u]);
+                }
+            };
+            if (rank_chunks == 1) read(0);
+            int turn = 0;
+            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
+                if (turn % cluster != rank) continue;
+                const bool shared_tile = rows.others_than(e);
+                for (int c = 0; c < rank_chunks and ok; ++c, ++it) {
+                    const unsigned s = it % kStages, phase = (it / kStages) & 1;
+                    if (rank_chunks > 1 and mine == e) read(c);
+                    ok = wait_all_lanes(&grant_bar[s], (granted >> s) & 1, &error_flag);
+                    granted ^= 1u << s;
+                    if (not ok) break;
+                    uint8_t* line = smem_a + s * kABytes + row * 128;
+                    const uint4 zero = make_uint4(0, 0, 0, 0);
+                    #pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        // 16-byte unit u of row r sits at unit u ^ (r % 8) of its 128-byte line
+                        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = mine == e ? hi[u] : zero;
+                        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = mine == e ? lo[u] : zero;
+                    }
+                    if (shared_tile) {
+                        // infinities and NaN of this adapter must not meet the zeros of other rows
+                        ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
+                        if (not ok) break;
+                        uint8_t* sb = smem_b + s * kBBytes;
+                        // the part of the block that the products read: 32 columns of BN lines, or 32 lines of each 64-column block
+                        const auto look = [&](uint8_t* at) {
+                            uint4* unit = reinterpret_cast<uint4*>(at);
+                            if (has_non_finite(*unit)) *unit = make_uint4(0, 0, 0, 0), poison[local % kPoisonSlots] = local + 1;
+                        };
+                        if (a.mn_major) {
+                            for (int i = row; i < BN / 64 * 32 * 8; i += 128) look(sb + (i / 256) * 8192 + (i % 256) * 16);
+                        } else {
+                            for (int i = row; i < BN * 4; i += 128) look(sb + (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4));
+                        }
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
+                }
+            }
+        }
+    }
+
     if (warp >= 2 and warp < 6) {
         // ------------------------------------------------------------------ epilogue
         const int quarter = warp & 3, row = quarter * 32 + lane;
@@ -553,60 +718,60 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             int m0, n0;
             origin(tile, m0, n0);
             const int acc = local & 1;
-            if (error_flag or not ptx::mbarrier_wait(&tmem_full_bar[acc], (local >> 1) & 1)) { error_flag = 1; break; }
+            if (not wait_all_lanes(&tmem_full_bar[acc], (local >> 1) & 1, &error_flag)) {
+                if (split) tc::cluster_wait();
+                break;
+            }
             tc::fence_after_thread_sync();
             const uint32_t taddr = tmem + acc * BN + (uint32_t(quarter * 32) << 16);
-            if (cluster > 1) {
-                // fp32 parts to this CTA's shared memory (the ring is idle: every product that read it has completed)
-                float* part = reinterpret_cast<float*>(smem_a) + row * (BN + 4);
-                for (int c = 0; c < BN; c += 32) {
-                    uint32_t r[32];
-                    tc::tmem_ld_32x32(taddr + c, r);
+            if (split) {
+                tc::cluster_wait();
+                // fp32 parts to the CTA that owns the row: [rank][row][column], 16-byte units swizzled by the row
+                if (m0 + quarter * 32 < a.rows.num_rows) {
+                    const int share = kLoraTileRows / cluster;
+                    send_part(tc::map_to_cta(smem_out + (rank * share + row % share) * (BN * 4), row / share), taddr, BN, row, m0 + row < a.rows.num_rows);
+                }
+                tc::fence_before_thread_sync();
+                break;                        // one tile per cluster
+            }
+            const bool fix = poison[local % kPoisonSlots] == local + 1;          // rare; the same for the whole warp
+            if (fix) cudaGridDependencySynchronize();
+            for (int c = 0; c < BN; c += 64) {
+                uint8_t* line = buffer + lane * 128;
+                if (lane == 0) ptx::bulk_wait_read<0>();
+                __syncwarp();
+                if (not fix) {
+                    uint32_t lo[32], hi[32];
+                    tc::tmem_ld_32x32(taddr + c, lo);
+                    tc::tmem_ld_32x32(taddr + c + 32, hi);
                     tc::wait_ld();
                     #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(part + c + 4 * i) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-                }
-            } else {
-                const bool fix = poison[local % kPoisonSlots] == local + 1;          // rare; the same for the whole warp
-                if (fix) cudaGridDependencySynchronize();
-                for (int c = 0; c < BN; c += 64) {
-                    uint8_t* line = buffer + lane * 128;
-                    if (lane == 0) ptx::bulk_wait_read<0>();
-                    __syncwarp();
-                    if (not fix) {
-                        uint32_t lo[32], hi[32];
-                        tc::tmem_ld_32x32(taddr + c, lo);
-                        tc::tmem_ld_32x32(taddr + c + 32, hi);
-                        tc::wait_ld();
+                    for (int u = 0; u < 4; ++u) {
+                        uint32_t w[4], w2[4];
                         #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            uint32_t w[4], w2[4];
-                            #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                w[j] = ptx::float2_to_bf16x2(__uint_as_float(lo[8 * u + 2 * j]), __uint_as_float(lo[8 * u + 2 * j + 1]));
-                                w2[j] = ptx::float2_to_bf16x2(__uint_as_float(hi[8 * u + 2 * j]), __uint_as_float(hi[8 * u + 2 * j + 1]));
-                            }
-                            *reinterpret_cast<uint4*>(line + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(line + (((4 + u) ^ (lane & 7)) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+                        for (int j = 0; j < 4; ++j) {
+                            w[j] = ptx::float2_to_bf16x2(__uint_as_float(lo[8 * u + 2 * j]), __uint_as_float(lo[8 * u + 2 * j + 1]));
+                            w2[j] = ptx::float2_to_bf16x2(__uint_as_float(hi[8 * u + 2 * j]), __uint_as_float(hi[8 * u + 2 * j + 1]));
                         }
-                    } else {
-                        for (int j = 0; j < 64; ++j) {
-                            const uint32_t r = tc::tmem_ld_32x1(taddr + c + j);
-                            tc::wait_ld();
-                            float v = __uint_as_float(r);
-                            if (m0 + row < a.rows.num_rows and n0 + c + j < a.n) v += poisoned(m0 + row, n0 + c + j);
-                            __syncwarp();
-                            *reinterpret_cast<__nv_bfloat16*>(line + (((j / 8) ^ (lane & 7)) << 4) + (j % 8) * 2) = __float2bfloat16_rn(v);
-                        }
+                        *reinterpret_cast<uint4*>(line + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (lane & 7)) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
                     }
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    // rows and columns beyond the matrix are cut off by the store itself
-                    if (lane == 0 and m0 + quarter * 32 < a.rows.num_rows and n0 + c < a.n) {
-                        tc::tma_store_2d(&map_y, n0 + c, m0 + quarter * 32, buffer);
-                        ptx::bulk_commit();
+                } else {
+                    for (int j = 0; j < 64; ++j) {
+                        const uint32_t r = tc::tmem_ld_32x1(taddr + c + j);
+                        tc::wait_ld();
+                        float v = __uint_as_float(r);
+                        if (m0 + row < a.rows.num_rows and n0 + c + j < a.n) v += poisoned(m0 + row, n0 + c + j);
+                        __syncwarp();
+                        *reinterpret_cast<__nv_bfloat16*>(line + (((j / 8) ^ (lane & 7)) << 4) + (j % 8) * 2) = __float2bfloat16_rn(v);
                     }
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                // rows and columns beyond the matrix are cut off by the store itself
+                if (lane == 0 and m0 + quarter * 32 < a.rows.num_rows and n0 + c < a.n) {
+                    tc::tma_store_2d(&map_y, n0 + c, m0 + quarter * 32, buffer);
+                    ptx::bulk_commit();
                 }
             }
             tc::fence_before_thread_sync();
@@ -617,40 +782,223 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         __syncwarp();
     }
 
-    if (cluster > 1) {
-        __syncwarp();
-        tc::cluster_sync();
+    if (split) {
+        // ------------------------------------------------------------------ sum of the parts
         int m0, n0;
         origin(first_tile, m0, n0);
+        const int share = kLoraTileRows / cluster;
+        __syncwarp();
+        if (warp < 2 or warp >= 6) tc::cluster_wait();         // (the epilogue warps have done so)
+        tc::cluster_sync();
         bool fix = false;
         for (int q = 0; q < cluster; ++q) fix = fix or ld_cluster_int(tc::map_to_cta(const_cast<const int*>(&poison[0]), q)) != 0;
         if (fix) cudaGridDependencySynchronize();
-        const int share = kLoraTileRows / cluster;
-        const float* part = reinterpret_cast<const float*>(smem_a);
         for (int item = threadIdx.x; item < share * (BN / 8); item += 320) {
             const int row = rank * share + item / (BN / 8), c = item % (BN / 8) * 8;
             if (m0 + row >= a.rows.num_rows or n0 + c >= a.n) continue;
             float v[8] = {};
-            for (int q = 0; q < cluster; ++q) {
-                const uint32_t at = tc::map_to_cta(part + row * (BN + 4) + c, q);
-                const float4 x = ld_cluster_v4(at), y = ld_cluster_v4(at + 16);
-                v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
-            }
-            if (fix) {
+            add_parts(v, smem_out, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
+            if (fix)
                 for (int j = 0; j < 8; ++j) v[j] += poisoned(m0 + row, n0 + c + j);
-            }
-            uint4 packed = make_uint4(ptx::float2_to_bf16x2(v[0], v[1]), ptx::float2_to_bf16x2(v[2], v[3]),
-                                      ptx::float2_to_bf16x2(v[4], v[5]), ptx::float2_to_bf16x2(v[6], v[7]));
-            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c) = packed;
+            store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c, v);
         }
-        tc::cluster_sync();                   // nobody leaves while others read its shared memory
+        tc::cluster_sync();                   // nobody leaves while others look at its flag
     }
 
     tc::fence_before_thread_sync();
     __syncthreads();
     if (warp == 1) {
         tc::fence_after_thread_sync();
-        tc::tmem_dealloc(tmem, 2 * BN);
+        tc::tmem_dealloc(tmem, split ? BN : 2 * BN);
+    }
+    if (threadIdx.x == 0) report(error_flag != 0, a.rows.status);
+}
+
+// ---------------------------------------------------------------------------------------- shared product + adapters, few rows
+// Decode: the time is that of reading W once. A cluster shares the contraction of (row tile, block_n columns of Y), so that
+// every SM pulls on W with all the shared memory it has in flight; rows of x that do not exist are not loaded (the products read
+// whatever lies behind them, into accumulator rows that are never stored). The low-rank term is too small for tensor-core
+// blocks of its own (a block per adapter costs about a microsecond, and every row may have another adapter): eight warps, idle
+// while W streams in, compute it in fp32 for the rows their CTA owns and add it to the parts of the shared product.
+//   warp 0      TMA producer     warp 1      MMA issuer
+//   warps 2-9   low-rank term; warps 2-5 then send the accumulator's rows to their owners, and all eight add and store
+// One tile per CTA. The wait for the kernel that computes t comes after W is under way.
+__global__ void __launch_bounds__(320, 1)
+lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ LoraGemmFewArgs a) {
+    using namespace lora_detail;
+    extern __shared__ uint8_t smem_raw[];
+    constexpr int kMaxStages = 32;
+    __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], done_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int error_flag;
+
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
+    const int cluster = a.cluster, rank = cluster > 1 ? int(blockIdx.x) % cluster : 0, tile = int(blockIdx.x) / cluster;
+    const int BN = a.block_n, stages = a.num_stages, sub = a.stage_blocks;       // a stage holds `sub` K blocks
+    const int m0 = tile % a.m_tiles * kLoraTileRows, n0 = tile / a.m_tiles * BN;
+    const int blocks = math::ceil_div(a.k, kLoraBlockK), per = math::align(math::ceil_div(blocks, cluster), sub);
+    const int kb0 = min(rank * per, blocks), kb1 = min(kb0 + per, blocks), steps = math::ceil_div(kb1 - kb0, sub);
+    const uint32_t x_bytes = a.x_box_rows * kLoraBlockK * 2, w_bytes = BN * kLoraBlockK * 2;       // of one K block
+    uint8_t* smem_a = align_1024(smem_raw);
+    uint8_t* smem_b = smem_a + stages * sub * x_bytes;
+    uint8_t* smem_part = smem_b + stages * sub * w_bytes;
+
+    const auto load = [&](int step, int s) {
+        ptx::mbarrier_arrive_expect_tx(&full_bar[s], sub * (x_bytes + w_bytes));
+        for (int i = 0; i < sub; ++i) {
+            // (blocks behind the contraction's end read zeros; behind this CTA's share they are not multiplied)
+            const int k0 = (kb0 + step * sub + i) * kLoraBlockK;
+            tc::tma_load_2d(smem_a + (s * sub + i) * x_bytes, &map_x, k0, m0, &full_bar[s]);
+            uint8_t* sb = smem_b + (s * sub + i) * w_bytes;
+            if (a.mn_major) for (int c = 0; c < BN / 64; ++c) tc::tma_load_2d(sb + c * 8192, &map_w, n0 + 64 * c, k0, &full_bar[s]);
+            else tc::tma_load_2d(sb, &map_w, k0, n0, &full_bar[s]);
+        }
+    };
+    if (threadIdx.x == 32) tc::prefetch_tensormap(&map_x), tc::prefetch_tensormap(&map_w);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1);
+        ptx::mbarrier_init(&done_bar, 1);
+        ptx::fence_mbarrier_init();
+        error_flag = 0;
+        for (int i = 0; i < min(stages, steps); ++i) load(i, i);
+    }
+    if (warp == 1) tc::tmem_alloc(&tmem_slot, BN);
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    tc::fence_after_thread_sync();
+    const uint32_t tmem = tmem_slot;
+    tc::cluster_arrive();                     // (waited for before the first access to another CTA's shared memory)
+
+    const int share = kLoraTileRows / cluster, units = BN / 8;                    // an item: eight columns of one row
+    float low[2][8];
+    if (warp == 0) {
+        Ring ring;
+        int issued = min(stages, steps);
+        for (; issued < steps; ++issued, ring.advance(stages)) {
+            if (not wait_all_lanes(&empty_bar[ring.slot], ring.phase, &error_flag)) break;
+            if (elect_one()) load(issued, ring.slot);
+        }
+        drain(full_bar, issued, stages);      // its own copies have landed before this warp leaves, also when somebody gave up
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, kLoraTileRows, BN, false, a.mn_major);
+        const uint32_t b_k = (a.mn_major ? 2048 : 32) >> 4;
+        const uint64_t desc_a0 = tc::make_smem_desc(smem_a, 16, 1024), desc_b0 = tc::make_smem_desc(smem_b, a.mn_major ? 8192 : 16, 1024);
+        Ring ring;
+        for (int step = 0; step < steps; ++step, ring.advance(stages)) {
+            wait(&full_bar[ring.slot], ring.phase, &error_flag);
+            tc::fence_after_thread_sync();
+            if (elect_one()) {
+                for (int i = 0; i < sub and kb0 + step * sub + i < kb1; ++i) {
+                    const uint64_t da = desc_a0 + uint64_t((ring.slot * sub + i) * (x_bytes >> 4)), db = desc_b0 + uint64_t((ring.slot * sub + i) * (w_bytes >> 4));
+                    #pragma unroll
+                    for (int k = 0; k < kLoraBlockK / 16; ++k) tc::mma_f16(tmem, da + k * 2, db + k * b_k, idesc, step > 0 or i > 0 or k > 0);
+                }
+                tc::commit(&empty_bar[ring.slot]);
+            }
+        }
+        if (elect_one()) tc::commit(&done_bar);
+        __syncwarp();
+    }
+    const int id = int(threadIdx.x) - 64;
+    const auto place = [&](int item, int& row, int& c) {                         // false: not part of the result
+        row = rank * share + item / units, c = item % units * 8;
+        return item < share * units and m0 + row < a.rows.num_rows and n0 + c < a.n;
+    };
+    // low-rank terms of two items at once, in fp32
+    const auto low_rank = [&](int first, float (&v)[2][8]) {
+        const __nv_bfloat16* base[2];
+        const float* t[2];
+        bool there[2];
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int row, c;
+            there[i] = place(first + 256 * i, row, c);
+            const int e = there[i] ? adapter_of(a.rows, m0 + row) : -1;
+            there[i] = e >= 0;
+            base[i] = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(max(e, 0)) * a.n * a.rows.rank + (a.mn_major ? n0 + c : int64_t(n0 + c) * a.rows.rank);
+            t[i] = a.t + int64_t(m0 + row) * a.rows.rank;
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        }
+        const int64_t pitch = a.mn_major ? a.n : a.rows.rank;
+        // four 16-byte units of V per item and step. mn_major: eight columns of the rank rows r .. r + 3; else eight rank columns of
+        // four of the columns
+        for (int step = 0; step < a.rows.rank / 4; ++step) {
+            const int r = a.mn_major ? step * 4 : step / 2 * 8, j0 = a.mn_major ? 0 : step % 2 * 4;
+            float f[2][8];
+            uint4 u[2][4];
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (not there[i]) continue;
+                if (a.mn_major) {
+                    const float4 g = *reinterpret_cast<const float4*>(t[i] + r);
+                    f[i][0] = g.x, f[i][1] = g.y, f[i][2] = g.z, f[i][3] = g.w;
+                } else {
+                    load8(t[i] + r, f[i]);
+                }
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) u[i][j] = *reinterpret_cast<const uint4*>(base[i] + (a.mn_major ? (r + j) * pitch : (j0 + j) * pitch + r));
+            }
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (not there[i]) continue;
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w[4] = {u[i][j].x, u[i][j].y, u[i][j].z, u[i][j].w};
+                    float sum = 0.0f;
+                    #pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 g = ptx::bf16x2_to_float2(w[q]);
+                        if (a.mn_major) v[i][2 * q] = fmaf(f[i][j], g.x, v[i][2 * q]), v[i][2 * q + 1] = fmaf(f[i][j], g.y, v[i][2 * q + 1]);
+                        else sum = fmaf(f[i][2 * q], g.x, sum), sum = fmaf(f[i][2 * q + 1], g.y, sum);
+                    }
+                    if (not a.mn_major) {
+                        if (j0 == 0) v[i][j] += sum; else v[i][4 + j] += sum;
+                    }
+                }
+            }
+        }
+    };
+    if (warp >= 2) {
+        cudaGridDependencySynchronize();      // t comes from the kernel before
+        low_rank(id, low);
+        __syncwarp();
+    }
+    if (warp >= 2 and warp < 6) {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        wait_all_lanes(&done_bar, 0, &error_flag);
+        tc::fence_after_thread_sync();
+        tc::cluster_wait();
+        if (m0 + quarter * 32 < a.rows.num_rows and quarter * 32 < a.x_box_rows)
+            send_part(tc::map_to_cta(smem_part + (rank * share + row % share) * (BN * 4), row / share), tmem + (uint32_t(quarter * 32) << 16), BN, row,
+                      m0 + row < a.rows.num_rows);
+        tc::fence_before_thread_sync();
+        __syncwarp();
+    } else {
+        tc::cluster_wait();
+    }
+    tc::cluster_sync();                       // all parts have arrived; nobody touches another CTA's shared memory after this
+    if (warp >= 2) {
+        for (int first = id; first < share * units; first += 512) {
+            if (first != id) low_rank(first, low);
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                int row, c;
+                if (not place(first + 256 * i, row, c)) continue;
+                float v[8] = {};
+                add_parts(v, smem_part, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += low[i][j];
+                store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c, v);
+            }
+        }
+    }
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after_thread_sync();
+        tc::tmem_dealloc(tmem, BN);
     }
     if (threadIdx.x == 0) report(error_flag != 0, a.rows.status);
 }
@@ -658,11 +1006,15 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // ---------------------------------------------------------------------------------------- weight gradients
 // A cluster owns (adapter, 256 columns of X); its CTAs take the adapter's row tiles in turn and add their sums through
 // distributed shared memory in rank order. X is the A operand (its columns are the M of the product), t the B operand, written
-// into shared memory by the epilogue warps as hi and lo. Row tiles in which the adapter does not occur are never read.
+// into shared memory as hi and lo side by side: one product gives both sums, which are added at the end. Row tiles in which the adapter does not occur are never read.
+//   warp 0      TMA producer     warp 1      MMA issuer
+//   warps 2-9   writers of t, two groups that take the blocks in turn; warps 2-5 read the accumulator
+// A block of 64 tokens is little work for the tensor cores, so the writers set the pace: each asks for the index two blocks
+// ahead and for t one block ahead. (One group that read both when it needed them took 1.4 us per block.)
 constexpr int kLoraWgradColumns = 256;
 constexpr int kLoraMaxTileWords = 2048;       // bitmap of row tiles: 2048 * 32 tiles of 128 rows
 
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(320, 1)
 lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LoraWgradArgs a) {
     using namespace lora_detail;
     extern __shared__ uint8_t smem_raw[];
@@ -672,12 +1024,13 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     __shared__ uint32_t tmem_slot, tile_bits[kLoraMaxTileWords];
     __shared__ volatile int error_flag;
 
-    const int warp = threadIdx.x / 32, lane = ptx::lane_id();
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = blockIdx.x % cluster, item = blockIdx.x / cluster;
     const int m_tile = item % a.m_tiles, e = item / a.m_tiles, m0 = m_tile * kM;
-    const int rp = math::align(a.rows.rank, 64), stages = a.num_stages;       // t's columns come in blocks of 64
-    const uint32_t t_bytes = rp * 128u;       // hi; lo follows
-    const int words = math::ceil_div(a.row_tiles, 32);
+    // columns of t: hi in [0, half), lo in [half, 2 * half); those beyond the rank hold whatever is there, and so do the columns of
+    // the accumulator that they make, which nobody reads
+    const int half = a.rows.rank <= 32 ? 32 : math::align(a.rows.rank, 64), stages = a.num_stages;
+    const int words = math::ceil_div(a.row_tiles, 32), pitch = math::align(a.rows.rank, 16) + 4;      // floats per column of X, staged
     uint8_t* smem = align_1024(smem_raw);
 
     if (threadIdx.x == 0) {
@@ -687,13 +1040,13 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         error_flag = 0;
         tc::prefetch_tensormap(&map_x);
     }
-    for (int w = warp; w < words; w += 6) {
+    for (int w = warp; w < words; w += 10) {
         const int tile = w * 32 + lane;
         const unsigned bits = __ballot_sync(0xffffffffu, tile < a.row_tiles and a.presence[int64_t(tile) * a.rows.num_adapters + e] != 0);
         if (lane == 0) tile_bits[w] = bits;
     }
     uint32_t columns = 32;
-    while (columns < uint32_t(2 * rp)) columns *= 2;
+    while (columns < uint32_t(4 * half)) columns *= 2;
     if (warp == 1) tc::tmem_alloc(&tmem_slot, columns);
     tc::fence_before_thread_sync();
     __syncthreads();
@@ -713,90 +1066,133 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 
     int count = 0;                            // blocks of this CTA
     if (warp == 0) {
-        if (lane == 0) {
-            walk([&](int token) {
-                const int s = count % stages;
-                if (error_flag or not ptx::mbarrier_wait(&empty_bar[s], ((count / stages) & 1) ^ 1)) { error_flag = 1; return false; }
-                ptx::mbarrier_arrive_expect_tx(&full_bar[s], kXBytes);
-                uint8_t* stage = smem + size_t(s) * a.stage_bytes;
-                for (int i = 0; i < kM / 64; ++i) tc::tma_load_2d(stage + i * 8192, &map_x, m0 + 64 * i, token, &full_bar[s]);
-                ++count;
-                return true;
-            });
-            for (int i = max(0, count - stages); i < count; ++i) ptx::mbarrier_wait(&full_bar[i % stages], (i / stages) & 1);
-        }
+        Ring ring;
+        walk([&](int token) {
+            if (not wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag)) return false;
+            if (elect_one()) {
+                ptx::mbarrier_arrive_expect_tx(&full_bar[ring.slot], kXBytes);
+                uint8_t* stage = smem + size_t(ring.slot) * a.stage_bytes;
+                #pragma unroll
+                for (int i = 0; i < kM / 64; ++i) tc::tma_load_2d(stage + i * 8192, &map_x, m0 + 64 * i, token, &full_bar[ring.slot]);
+            }
+            ++count, ring.advance(stages);
+            return true;
+        });
+        drain(full_bar, count, stages);       // its own copies have landed before this warp leaves, also when somebody gave up
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, 128, rp, true, true);
-            const uint64_t desc_x = tc::make_smem_desc(smem, 8192, 1024), desc_t = tc::make_smem_desc(smem + kXBytes, 8192, 1024);
-            walk([&](int) {
-                const int s = count % stages, phase = (count / stages) & 1;
-                if (error_flag or not ptx::mbarrier_wait(&full_bar[s], phase) or not ptx::mbarrier_wait(&ext_bar[s], phase)) { error_flag = 1; return false; }
-                tc::fence_after_thread_sync();
-                const uint64_t step = uint64_t(s) * (a.stage_bytes >> 4);
+        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, 128, 2 * half, true, true);
+        const uint64_t desc_x = tc::make_smem_desc(smem, 8192, 1024), desc_t = tc::make_smem_desc(smem + kXBytes, 8192, 1024);
+        Ring ring;
+        walk([&](int) {
+            wait(&full_bar[ring.slot], ring.phase, &error_flag);
+            wait(&ext_bar[ring.slot], ring.phase, &error_flag);
+            tc::fence_after_thread_sync();
+            if (elect_one()) {
+                const uint64_t step = uint64_t(ring.slot) * (a.stage_bytes >> 4);
                 #pragma unroll
                 for (int k = 0; k < kLoraBlockK / 16; ++k) {
                     #pragma unroll
-                    for (int m = 0; m < 2; ++m) {               // 128 columns of X each, 16 KB apart
-                        tc::mma_f16(tmem + m * rp, desc_x + step + m * 1024 + k * 128, desc_t + step + k * 128, idesc, count > 0 or k > 0);
-                        tc::mma_f16(tmem + m * rp, desc_x + step + m * 1024 + k * 128, desc_t + step + (t_bytes >> 4) + k * 128, idesc, true);
-                    }
+                    for (int m = 0; m < 2; ++m)                 // 128 columns of X each, 16 KB apart
+                        tc::mma_f16(tmem + m * 2 * half, desc_x + step + m * 1024 + k * 128, desc_t + step + k * 128, idesc, count > 0 or k > 0);
                 }
-                tc::commit(&empty_bar[s]);
-                ++count;
-                return true;
-            });
-            tc::commit(&done_bar);
-        }
+                tc::commit(&empty_bar[ring.slot]);
+            }
+            ++count, ring.advance(stages);
+            return true;
+        });
+        if (elect_one()) tc::commit(&done_bar);
     } else {
         // ------------------------------------------------------------------ writers of the B operand, then the epilogue
-        const int id = threadIdx.x - 64, line = id & 63, side = id >> 6;
-        bool ok = true;
-        walk([&](int token) {
-            const int s = count % stages, phase = (count / stages) & 1, row = token + line;
-            const bool mine = adapter_of(a.rows, row) == e;
+        const int id = (threadIdx.x - 64) & 127, group = (warp - 2) / 4, line = id & 63, side = id >> 6;
+        constexpr int kUnits = kLoraMaxRank / 8 / 2;            // units of eight rank columns, dealt out to two threads per row
+        // a block's index is asked for in one step, its t in the next, and it is written in the one after that
+        int first = -1, first_turn = 0, first32 = -1;           // block whose index has been asked for: first token, number, index as read
+        int64_t first64 = -1;
+        int third = -1, third_turn = 0, turn = 0;               // block in registers as hi and lo
+        bool third_mine = false;
+        float next[kUnits][8];
+        uint4 hi[kUnits], lo[kUnits];
+        const auto write = [&]() {
+            const int s = third_turn % stages, phase = (third_turn / stages) & 1;
             uint8_t* stage = smem + size_t(s) * a.stage_bytes;
-            ok = __all_sync(0xffffffffu, ptx::mbarrier_wait(&empty_bar[s], phase ^ 1));
-            if (not ok) { error_flag = 1; return false; }
-            for (int u = side; u < rp / 8; u += 2) {            // units of eight rank columns, shared by two threads
-                float v[8];
-                const bool there = mine and 8 * u < a.rows.rank;
-                if (there) load8(a.t + int64_t(row) * a.rows.rank + 8 * u, v);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = there ? v[j] : 0.0f;
-                uint4 hi, lo;
-                split8(v, hi, lo);
-                uint8_t* at = stage + kXBytes + (u / 8) * 8192 + line * 128 + (((u % 8) ^ (line & 7)) << 4);
-                *reinterpret_cast<uint4*>(at) = hi;
-                *reinterpret_cast<uint4*>(at + t_bytes) = lo;
+            if (not wait_all_lanes(&empty_bar[s], phase ^ 1, &error_flag)) return false;
+            const auto place = [&](int column) {                // 16-byte unit of this row's line in its block of 64 columns
+                return reinterpret_cast<uint4*>(stage + kXBytes + (column / 64) * 8192 + line * 128 + (((column % 64 / 8) ^ (line & 7)) << 4));
+            };
+            #pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = 8 * (2 * i + side);
+                if (r < a.rows.rank) *place(r) = hi[i], *place(half + r) = lo[i];
             }
             // rows of other requests in this block: zeros instead of whatever they hold (0 * inf would be NaN)
-            ok = ok and ptx::mbarrier_wait(&full_bar[s], phase);
-            if (not mine and row < a.rows.num_rows)
-                for (int i = side; i < kM / 64; i += 2)
-                    for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stage + i * 8192 + line * 128 + u * 16) = make_uint4(0, 0, 0, 0);
-            ptx::fence_proxy_async_smem();
-            ok = __all_sync(0xffffffffu, ok);
-            if (not ok) { error_flag = 1; return false; }
-            if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
-            ++count;
-            return not __any_sync(0xffffffffu, error_flag != 0);
-        });
-        if (not ptx::mbarrier_wait(&done_bar, 0)) error_flag = 1;
-        tc::fence_after_thread_sync();
-        const int quarter = warp & 3;
-        float* part = reinterpret_cast<float*>(smem);
-        for (int m = 0; m < 2; ++m) {
-            float* out = part + (m * 128 + quarter * 32 + lane) * (rp + 1);
-            for (int c = 0; c < a.rows.rank; c += 16) {
-                uint32_t r[16];
-                tc::tmem_ld_32x16(tmem + (uint32_t(quarter * 32) << 16) + m * rp + c, r);
-                tc::wait_ld();
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) out[c + i] = count > 0 ? __uint_as_float(r[i]) : 0.0f;
+            const bool foreign = not third_mine and third + line < a.rows.num_rows;
+            if (__any_sync(0xffffffffu, foreign)) {
+                if (not wait_all_lanes(&full_bar[s], phase, &error_flag)) return false;
+                if (foreign)
+                    for (int i = side; i < kM / 64; i += 2)
+                        for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stage + i * 8192 + line * 128 + u * 16) = make_uint4(0, 0, 0, 0);
             }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
+            return true;
+        };
+        // one step of the pipeline: `token` enters (-1: none), what leaves it is written
+        const auto step = [&](int token, int token_turn) {
+            // (compared with the adapter in the next step: a comparison here would wait for the read)
+            int new32 = -1;
+            int64_t new64 = -1;
+            if (token >= 0 and token + line < a.rows.num_rows) {
+                if (a.rows.idx64) new64 = reinterpret_cast<const int64_t*>(a.rows.idx)[token + line];
+                else new32 = reinterpret_cast<const int*>(a.rows.idx)[token + line];
+            }
+            const bool mine = a.rows.idx64 ? first64 == e : first32 == e;
+            #pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int u = 2 * i + side;
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) next[i][j] = 0.0f;
+                if (mine and 8 * u < a.rows.rank) load8(a.t + int64_t(first + line) * a.rows.rank + 8 * u, next[i]);
+            }
+            if (third >= 0 and not write()) return false;
+            third = first, third_mine = mine, third_turn = first_turn;
+            #pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                if (8 * (2 * i + side) < a.rows.rank) split8(next[i], hi[i], lo[i]);
+            first = token, first32 = new32, first64 = new64, first_turn = token_turn;
+            return true;
+        };
+        walk([&](int token) {
+            const int this_turn = turn++;
+            count = turn;
+            return this_turn % 2 != group or step(token, this_turn);
+        });
+        if (step(-1, 0)) step(-1, 0);
+        if (warp < 6) {
+            wait_all_lanes(&done_bar, 0, &error_flag);
+            tc::fence_after_thread_sync();
+            const int quarter = warp & 3;
+            float* part = reinterpret_cast<float*>(smem);
+            for (int m = 0; m < 2; ++m) {
+                float* out = part + (m * 128 + quarter * 32 + lane) * pitch;
+                for (int c = 0; c < a.rows.rank; c += 16) {
+                    uint32_t r[16], q[16];
+                    const uint32_t at = tmem + (uint32_t(quarter * 32) << 16) + m * 2 * half + c;
+                    tc::tmem_ld_32x16(at, r);
+                    tc::tmem_ld_32x16(at + half, q);
+                    tc::wait_ld();
+                    #pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (count > 0)
+                            v = make_float4(__uint_as_float(r[i]) + __uint_as_float(q[i]), __uint_as_float(r[i + 1]) + __uint_as_float(q[i + 1]),
+                                            __uint_as_float(r[i + 2]) + __uint_as_float(q[i + 2]), __uint_as_float(r[i + 3]) + __uint_as_float(q[i + 3]));
+                        *reinterpret_cast<float4*>(out + c + i) = v;
+                    }
+                }
+            }
+            tc::fence_before_thread_sync();
         }
-        tc::fence_before_thread_sync();
     }
     __syncthreads();
     if (cluster > 1) tc::cluster_sync();
@@ -804,20 +1200,41 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     for (int w = 0; w < words; ++w) any = any or tile_bits[w] != 0;
     if (any or not a.accumulate) {
         const float* part = reinterpret_cast<const float*>(smem);
-        const int share = kM / cluster, first = rank * share, r_count = a.rows.rank;
-        for (int i = threadIdx.x; i < share * r_count; i += 192) {
-            // neighbouring threads write neighbouring addresses in either layout
-            const int m = first + (a.rank_major ? i % share : i / r_count), r = a.rank_major ? i / share : i % r_count;
+        const int share = kM / cluster, first = rank * share, units = a.rows.rank / 4;
+        for (int i = threadIdx.x; i < share * units; i += 320) {
+            // an item is four rank columns of one column of X; neighbouring threads write neighbouring addresses in either layout
+            const int m = first + (a.rank_major ? i % share : i / units), r = (a.rank_major ? i / share : i % units) * 4;
             if (m0 + m >= a.m) continue;
-            float sum = 0.0f;
-            if (cluster > 1) for (int q = 0; q < cluster; ++q) sum += ld_cluster(tc::map_to_cta(part + m * (rp + 1) + r, q));
-            else sum = part[m * (rp + 1) + r];
-            const int64_t at = a.rank_major ? (int64_t(e) * r_count + r) * a.m + m0 + m : (int64_t(e) * a.m + m0 + m) * r_count + r;
-            if (a.out_fp32) {
-                float* d = reinterpret_cast<float*>(a.d) + at;
-                *d = a.accumulate ? *d + sum : sum;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float* line = part + m * pitch + r;
+            for (int q = 0; q < cluster; ++q) {
+                const float4 v = cluster > 1 ? ld_cluster_v4(tc::map_to_cta(line, q)) : *reinterpret_cast<const float4*>(line);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            if (a.rank_major) {
+                const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+                const int64_t at = (int64_t(e) * a.rows.rank + r) * a.m + m0 + m;
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (a.out_fp32) {
+                        float* d = reinterpret_cast<float*>(a.d) + at + int64_t(j) * a.m;
+                        *d = a.accumulate ? *d + v[j] : v[j];
+                    } else {
+                        reinterpret_cast<__nv_bfloat16*>(a.d)[at + int64_t(j) * a.m] = __float2bfloat16_rn(v[j]);
+                    }
+                }
             } else {
-                reinterpret_cast<__nv_bfloat16*>(a.d)[at] = __float2bfloat16_rn(sum);
+                const int64_t at = (int64_t(e) * a.m + m0 + m) * a.rows.rank + r;
+                if (a.out_fp32) {
+                    // (a buffer of the caller's may lie on any 4-byte boundary)
+                    float* d = reinterpret_cast<float*>(a.d) + at;
+                    if (a.accumulate) sum.x += d[0], sum.y += d[1], sum.z += d[2], sum.w += d[3];
+                    if (reinterpret_cast<uintptr_t>(d) % 16 == 0) *reinterpret_cast<float4*>(d) = sum;
+                    else d[0] = sum.x, d[1] = sum.y, d[2] = sum.z, d[3] = sum.w;
+                } else {
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.d) + at) =
+                        make_uint2(ptx::float2_to_bf16x2(sum.x, sum.y), ptx::float2_to_bf16x2(sum.z, sum.w));
+                }
             }
         }
     }

@@ -24,7 +24,7 @@ struct LoraShrinkArgs {
     int k;                                // contraction length
     int mn_major;                         // 0: A_e is [rank, k] (k contiguous); 1: [k, rank] (rank contiguous)
     int chunk, num_chunks;                // adapters per CTA, CTAs per row tile (times the cluster)
-    int cluster, num_stages, stage_bytes;
+    int cluster, ring_bytes;
     const float* scaling;                 // [num_adapters]
     float* t;
     uint8_t* presence;                    // optional [row tiles][num_adapters]: 1 = some row of the tile has the adapter
@@ -39,6 +39,19 @@ struct LoraGemmArgs {
     int m_tiles, n_tiles;
     const float* t;                       // fp32 [num_rows, rank], scaled
     const void* v;                        // V, read directly only where it holds infinities or NaN
+    void* y;
+};
+
+// The same for few rows and a small rank
+struct LoraGemmFewArgs {
+    LoraRows rows;
+    int k, n, mn_major, cluster;
+    int m_tiles;
+    int block_n;                          // columns of Y per tile: 64 or 128
+    int stage_blocks, num_stages;         // K blocks per stage, stages
+    int x_box_rows;                       // rows of X that a load brings (a whole tile, or all rows there are)
+    const float* t;
+    const void* v;
     void* y;
 };
 

@@ -20,16 +20,15 @@ _TABLE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _lookup(table: torch.Tensor, idx: torch.Tensor, scale: float, table_sf: Optional[torch.Tensor]) -> torch.Tensor:
-    flat = idx.reshape(-1)
     if table.is_cuda:
-        out = _C.embedding_lookup(table, flat.contiguous(), scale, table_sf)
-    else:
-        valid = (flat >= 0) & (flat < table.size(0))
-        rows = table.new_zeros((flat.numel(), table.size(1)), dtype=torch.float32)
-        rows[valid] = table[flat[valid].long()].float()
-        if table_sf is not None:
-            rows[valid] = rows[valid] * table_sf[flat[valid].long()].repeat_interleave(128, dim=1)
-        out = (rows * scale).to(torch.bfloat16 if table_sf is not None else table.dtype)
+        return _C.embedding_lookup(table, idx.contiguous(), scale, table_sf)
+    flat = idx.reshape(-1)
+    valid = (flat >= 0) & (flat < table.size(0))
+    rows = table.new_zeros((flat.numel(), table.size(1)), dtype=torch.float32)
+    rows[valid] = table[flat[valid].long()].float()
+    if table_sf is not None:
+        rows[valid] = rows[valid] * table_sf[flat[valid].long()].repeat_interleave(128, dim=1)
+    out = (rows * scale).to(torch.bfloat16 if table_sf is not None else table.dtype)
     return out.view(*idx.shape, table.size(1))
 
 
@@ -71,7 +70,7 @@ def embedding_lookup(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0,
         return _lookup(table.detach(), idx, float(scale), table_sf.detach())
     assert table.dtype in _TABLE_TYPES, 'the table is bf16, fp16 or fp32, or e4m3 with `table_sf`'
     if not (torch.is_grad_enabled() and table.requires_grad):
-        return _lookup(table.detach(), idx, float(scale), None)
+        return _lookup(table, idx, float(scale), None)
     return _Lookup.apply(table, idx, float(scale))
 
 

@@ -38,13 +38,14 @@ def _total(tensors: List[torch.Tensor], replicated: List[torch.Tensor], group: O
 
 
 def _checked(grads: Sequence[torch.Tensor], replicated: Sequence[torch.Tensor]):
-    if isinstance(grads, torch.Tensor):
-        grads = [grads]
-    tensors, replicated = [t.detach() for t in grads], [t.detach() for t in replicated]
-    for t in tensors + replicated:
+    tensors, replicated = [grads] if isinstance(grads, torch.Tensor) else list(grads), list(replicated)
+    everything = tensors + replicated
+    if everything and everything[0].is_cuda:
+        return tensors, replicated, everything         # the native call looks at types, devices and layouts, tensor by tensor
+    for t in everything:
         assert t.dtype in (torch.bfloat16, torch.float16, torch.float32), 'gradients are bf16, fp16 or fp32'
-        assert t.device == (tensors or replicated)[0].device, 'gradients lie on one device'
-    return tensors, replicated
+        assert t.device == everything[0].device, 'gradients lie on one device'
+    return tensors, replicated, everything
 
 
 def grad_norm(grads: Sequence[torch.Tensor], group: Optional[dist.ProcessGroup] = None,
@@ -54,7 +55,9 @@ def grad_norm(grads: Sequence[torch.Tensor], group: Optional[dist.ProcessGroup] 
     Tensors are dense (contiguous, or a permutation of it). With `group` the squares of `grads` are added over its ranks,
     a collective call even for a rank whose list is empty (give it a tensor in `replicated`, or an empty tensor, so that the
     device is known); `replicated` is counted once. NaN or infinity in a gradient shows in the norm."""
-    tensors, replicated = _checked(grads, replicated)
+    tensors, replicated, everything = _checked(grads, replicated)
+    if everything and everything[0].is_cuda and group is None and not replicated:
+        return _C.grad_norm(tensors)
     sums = _total(tensors, replicated, group)
     return _C.grad_norm_finish(sums) if sums.is_cuda else sums.sum().sqrt().float()
 
@@ -69,20 +72,21 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, group: Optio
     gradients are written there instead and `grads` stay as they are: fp32 accumulators become clipped bf16 gradients in
     one sweep. Tensors that are written may not share memory with one another."""
     assert max_norm >= 0, 'max_norm is not negative'
-    tensors, replicated = _checked(grads, replicated)
-    everything = tensors + replicated
+    tensors, replicated, everything = _checked(grads, replicated)
     if out is not None:
-        out = [out] if isinstance(out, torch.Tensor) else [o.detach() for o in out]
-        assert len(out) == len(everything) and all(o.shape == g.shape for o, g in zip(out, everything)), 'one output per gradient, of its shape'
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        assert len(out) == len(everything), 'one output per gradient'
     if not everything:
         return grad_norm(tensors, group)
-    simple = group is None and not replicated
     if everything[0].is_cuda:
         # (without other ranks and one list, the sums are taken inside the call)
+        simple = group is None and not replicated
         return _C.grad_clip(everything, out, None if simple else _total(tensors, replicated, group), float(max_norm))
+    assert out is None or all(o.shape == g.shape for o, g in zip(out, everything)), 'an output has its gradient\'s shape'
     sums = _total(tensors, replicated, group)
     norm = sums.sum().sqrt().float()
     factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
-    for o, g in zip(everything if out is None else out, everything):
-        o.copy_(g.float() * factor)
+    with torch.no_grad():
+        for o, g in zip(everything if out is None else out, everything):
+            o.copy_(g.float() * factor)
     return norm

@@ -16,9 +16,6 @@ from .._C_loader import _C
 
 __all__ = ['lora_linear']
 
-MAX_RANK = 128
-
-
 def _reference(x, w, lora_a, lora_b, idx, scaling):
     """Plain form in fp32 (CPU): rows are picked by adapter, so one adapter's values never meet another's rows."""
     dtype = x.dtype
@@ -41,8 +38,7 @@ def _weight_grad(x, t, idx, presence, parameter, rank_major):
 class _LoraLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, lora_a, lora_b, idx, scaling):
-        t, _ = _C.lora_shrink(x, lora_a, idx, scaling)
-        y = _C.lora_gemm(x, w, t, lora_b, idx)
+        y, t = _C.lora_forward(x, w, lora_a, lora_b, idx, scaling)
         ctx.save_for_backward(x, w, lora_a, lora_b, idx, scaling, t)
         return y
 
@@ -66,7 +62,7 @@ class _LoraLinear(torch.autograd.Function):
             from .grouped_gemm import grouped_gemm_wgrad
             one = _one_group(x.size(0), x.device)
             dw = torch.empty((1, *w.shape), dtype=w.dtype, device=w.device)
-            grouped_gemm_wgrad(dy, x, dw, one, one, accumulate=False)
+            grouped_gemm_wgrad(dy, x.contiguous(), dw, one, one, accumulate=False)
             dw = dw[0]
         return dx, dw, da, db, None, None
 
@@ -83,30 +79,23 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     Gradients reach `x`, `lora_a` and `lora_b` (or their fp32 `main_grad`), and `w` if it wants one (K and N multiples of
     128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to.
     """
+    if not isinstance(scaling, torch.Tensor):
+        scaling = torch.full((lora_a.size(0),), float(scaling), dtype=torch.float32, device=x.device)
+    assert not scaling.requires_grad, 'scaling receives no gradient'
+    if x.is_cuda:
+        if adapter_idx.dim() == 1 and adapter_idx.size(0) > 1 and adapter_idx.stride(0) != 1:
+            adapter_idx = adapter_idx.contiguous()
+        if not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or lora_a.requires_grad or lora_b.requires_grad)):
+            return _C.lora_forward(x, w, lora_a, lora_b, adapter_idx, scaling)[0]       # (which looks at every argument)
+        if w.requires_grad:
+            assert w.size(0) % 128 == 0 and w.size(1) % 128 == 0, 'the gradient of w needs K and N to be multiples of 128'
+        return _LoraLinear.apply(x, w, lora_a, lora_b, adapter_idx, scaling)
     assert x.dim() == 2 and w.dim() == 2 and lora_a.dim() == 3 and lora_b.dim() == 3, 'x [rows, K], w [N, K], lora_a [E, rank, K], lora_b [E, N, rank]'
     rows, k = x.shape
     n, adapters, rank = w.size(0), lora_a.size(0), lora_a.size(1)
     assert w.size(1) == k and lora_a.size(2) == k and lora_b.shape == (adapters, n, rank), 'shapes of x, w, lora_a and lora_b do not agree'
     assert adapter_idx.shape == (rows,) and adapter_idx.dtype in (torch.int32, torch.int64), 'one int32 or int64 adapter index per row'
     assert all(t.dtype == torch.bfloat16 for t in (x, w, lora_a, lora_b)), 'operands are bf16'
-    assert all(t.device == x.device for t in (w, lora_a, lora_b, adapter_idx)), 'all tensors of a call lie on one device'
-    if isinstance(scaling, torch.Tensor):
-        assert scaling.shape == (adapters,) and scaling.dtype == torch.float32 and scaling.device == x.device, 'scaling is a number or fp32 [adapters]'
-        assert not scaling.requires_grad, 'scaling receives no gradient'
-    else:
-        scaling = torch.full((adapters,), float(scaling), dtype=torch.float32, device=x.device)
-    if not x.is_cuda:
-        return _reference(x, w, lora_a, lora_b, adapter_idx, scaling)
-    assert adapters >= 1 and k % 8 == 0 and n % 8 == 0 and k > 0 and n > 0, 'K and N are multiples of 8'
-    assert rank % 8 == 0 and 0 < rank <= MAX_RANK, 'the rank is a multiple of 8 up to 128'
-    operands = [t.contiguous() for t in (x, w, lora_a, lora_b)]
-    operands = [t if t.data_ptr() % 16 == 0 else t.clone() for t in operands]      # views on odd addresses
-    idx, scaling = adapter_idx.contiguous(), scaling.contiguous()
-    if scaling.data_ptr() % 16:
-        scaling = scaling.clone()
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in operands)):
-        t, _ = _C.lora_shrink(operands[0], operands[2], idx, scaling)
-        return _C.lora_gemm(operands[0], operands[1], t, operands[3], idx)
-    if w.requires_grad:
-        assert k % 128 == 0 and n % 128 == 0, 'the gradient of w needs K and N to be multiples of 128'
-    return _LoraLinear.apply(*operands, idx, scaling)
+    assert all(t.device == x.device for t in (w, lora_a, lora_b, adapter_idx, scaling)), 'all tensors of a call lie on one device'
+    assert scaling.shape == (adapters,) and scaling.dtype == torch.float32, 'scaling is a number or fp32 [adapters]'
+    return _reference(x, w, lora_a, lora_b, adapter_idx, scaling)

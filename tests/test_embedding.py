@@ -167,7 +167,8 @@ def test_strided_and_unaligned_tables(offset, pitch):
 @pytest.mark.gpu
 @pytest.mark.parametrize('kind', ['any', 'same', 'few', 'masked', 'outside'])
 @pytest.mark.parametrize('tokens,rows,hidden', [(1, 1, 8), (31, 100, 1003), (33, 40, 130), (2049, 70000, 64), (8192, 300, 96),
-                                                (8193, 1200, 256), (40000, 129280, 64)])
+                                                (8193, 1200, 256), (17000, 511, 64), (40000, 129280, 64),
+                                                (70001, 300000, 24)])
 def test_gradient(tokens, rows, hidden, kind):
     ids = make_ids(tokens, rows, kind, torch.int64, 'cuda', seed=tokens)
     for dtype, out_type in ((torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)):

@@ -115,7 +115,8 @@ def test_refusals():
     (1, 64, 64, 8, 1, 'same'), (1, 7168, 4096, 16, 4, 'same'), (3, 8, 8, 8, 2, 'mixed'), (130, 200, 136, 24, 5, 'mixed'),
     (127, 1000, 520, 40, 3, 'runs'), (128, 512, 256, 128, 3, 'mixed'), (96, 2048, 1024, 16, 64, 'mixed'), (300, 1024, 392, 64, 200, 'mixed'),
     (257, 640, 384, 32, 2, 'none'), (1025, 512, 2048, 48, 4, 'runs'), (2500, 1096, 2056, 72, 3, 'runs'), (5000, 256, 4096, 8, 6, 'mixed'),
-    (1, 256, 128, 8, 1, 'none')])
+    (1, 256, 128, 8, 1, 'none'), (128, 1024, 512, 32, 7, 'mixed'), (129, 1024, 512, 32, 7, 'mixed'), (500, 2048, 200, 8, 3, 'mixed'),
+    (120, 4096, 1000, 64, 2, 'mixed'), (1, 128, 16384, 64, 2, 'same'), (64, 7168, 64, 128, 3, 'runs')])
 def test_forward_and_gradients(rows, k, n, rank, adapters, order):
     args = make(rows, k, n, rank, adapters, 'cuda', order, seed=rows)
     results = run_all(args)
@@ -228,12 +229,17 @@ def test_two_streams_at_once():
 
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
+    import deep_ep
+    refused = pytest.raises((AssertionError, deep_ep.EPException))
     for k, n, rank in ((12, 16, 8), (16, 12, 8), (16, 16, 12), (16, 16, 136)):
         x, w, a, b, dy, idx, s = make(5, k, n, rank, 2, 'cuda')
-        with pytest.raises(AssertionError):
+        with refused:
             lora_linear(x, w, a, b, idx, s)
     x, w, a, b, dy, idx, s = make(5, 64, 64, 8, 2, 'cuda')
-    with pytest.raises(AssertionError):
-        lora_linear(x, w.requires_grad_(), a, b, idx, s)
-    with pytest.raises(AssertionError):
-        lora_linear(x, w.detach(), a, b, idx.cpu(), s)
+    for bad in (lambda: lora_linear(x, w.clone().requires_grad_(), a, b, idx, s), lambda: lora_linear(x, w, a, b, idx.cpu(), s),
+                lambda: lora_linear(x.float(), w, a, b, idx, s), lambda: lora_linear(x, w[:, :32], a, b, idx, s), lambda: lora_linear(x, w, a, b[:1], idx, s),
+                lambda: lora_linear(x, w, a, b[:, :32], idx, s), lambda: lora_linear(x, w, a, b, idx[:4], s), lambda: lora_linear(x, w, a, b, idx.float(), s),
+                lambda: lora_linear(x, w, a, b, idx, s[:1]), lambda: lora_linear(x, w, a, b, idx, s.double()), lambda: lora_linear(x[0], w, a, b, idx, s),
+                lambda: lora_linear(x, w, a[0], b, idx, s), lambda: lora_linear(x, w.cpu(), a, b, idx, s)):
+        with refused:
+            bad()
