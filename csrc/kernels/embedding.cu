@@ -105,12 +105,19 @@ int64_t embedding_sort_workspace_ints(int num_tokens) {
 
 void embedding_sort(EmbSortArgs args, int* workspace, const int** ids, const int** order, cudaStream_t stream) {
     const int n = args.num_tokens;
+    if (args.touched != nullptr) CUDA_CHECK(cudaMemsetAsync(args.touched, 0, (args.num_rows + 31ll) / 32 * 4, stream));
+    if (n <= kEmbRankKeys) {
+        args.keys[0] = workspace, args.vals[0] = workspace + n;
+        embedding_rank_kernel<<<math::ceil_div(n, 32), kEmbRankThreads, math::align(n, 32) * 4, stream>>>(args);
+        CUDA_CHECK(cudaGetLastError());
+        *ids = args.keys[0], *order = args.vals[0];
+        return;
+    }
     if (n <= kClusterKeys) {
         choose_digits(args, kEmbClusterDigitBits);
         args.keys[0] = workspace, args.vals[0] = workspace + n;
         // as few keys per thread as eight CTAs allow
-        if (n <= 8 * kEmbClusterThreads) sort_in_cluster<1>(args, stream);
-        else if (n <= 16 * kEmbClusterThreads) sort_in_cluster<2>(args, stream);
+        if (n <= 16 * kEmbClusterThreads) sort_in_cluster<2>(args, stream);
         else if (n <= 32 * kEmbClusterThreads) sort_in_cluster<4>(args, stream);
         else sort_in_cluster<8>(args, stream);
         *ids = args.keys[0], *order = args.vals[0];
@@ -156,7 +163,7 @@ void launch_early(void (*kernel)(EmbGradArgs), unsigned grid, cudaStream_t strea
 template <typename In, typename Out, int kElems, int kPacks, bool kAccumulate>
 void launch_grad(const EmbGradArgs& a, cudaStream_t stream) {
     const int64_t slices = math::ceil_div(a.hidden, 32 * kElems * kPacks);
-    const int64_t sums = int64_t(a.num_chunks) * slices, fills = a.touched != nullptr ? a.num_rows : 0;
+    const int64_t sums = int64_t(a.num_chunks) * slices, fills = a.accumulate ? 0 : a.num_rows;
     EP_HOST_ASSERT(sums < (int64_t(1) << 31));
     launch_early(embedding_grad_kernel<In, Out, kElems, kPacks, kAccumulate>, static_cast<unsigned>((sums + fills + 7) / 8), stream, a);
     if (a.num_chunks > 1) launch_early(embedding_grad_join_kernel<Out, kElems, kAccumulate>, 148 * 6, stream, a);

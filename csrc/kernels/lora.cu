@@ -96,20 +96,35 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
 
 namespace {
 
-template <int BN>
+struct GemmMaps {
+    CUtensorMap x, w, v, y;
+};
+
+// Boxes of 64 (K) x 128 over x and over K-major W and V; 64 x 64 where the columns of Y are contiguous
+GemmMaps gemm_maps(const LoraGemmArgs& a, const void* x, const void* w) {
+    const auto& r = a.rows;
+    return {make_map_2d(x, r.num_rows, a.k, kLoraBlockK, kLoraTileRows),
+            a.mn_major ? make_map_2d(w, a.k, a.n, 64, kLoraBlockK) : make_map_2d(w, a.n, a.k, kLoraBlockK, 128),
+            a.mn_major ? make_map_3d(a.v, r.num_adapters, r.rank, a.n, 64, 64) : make_map_3d(a.v, r.num_adapters, a.n, r.rank, 64, 128),
+            make_map_out(a.y, r.num_rows, a.n, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2)};
+}
+
 void launch_gemm(LoraGemmArgs args, const void* x, const void* w, int sms, cudaStream_t stream) {
-    const auto& r = args.rows;
-    args.m_tiles = math::ceil_div(r.num_rows, kLoraTileRows), args.n_tiles = math::ceil_div(args.n, BN);
+    args.m_tiles = math::ceil_div(args.rows.num_rows, kLoraTileRows), args.n_tiles = math::ceil_div(args.n, kLoraGemmColumns);
     const int64_t tiles = int64_t(args.m_tiles) * args.n_tiles;
     EP_HOST_ASSERT_MSG(tiles < (int64_t(1) << 30), "too many tiles for one launch");
-    args.cluster = BN == 128 ? choose_cluster(tiles, math::ceil_div(args.k, kLoraBlockK), 4, sms) : 1;
+    args.cluster = choose_cluster(tiles, math::ceil_div(args.k, kLoraBlockK), 4, sms);
     const int64_t grid = args.cluster > 1 ? tiles * args.cluster : std::min<int64_t>(tiles, sms);
-    const CUtensorMap map_x = make_map_2d(x, r.num_rows, args.k, kLoraBlockK, kLoraTileRows);
-    const CUtensorMap map_w = args.mn_major ? make_map_2d(w, args.k, args.n, 64, kLoraBlockK) : make_map_2d(w, args.n, args.k, kLoraBlockK, 128);
-    const CUtensorMap map_v = args.mn_major ? make_map_3d(args.v, r.num_adapters, r.rank, args.n, 64, 64)
-                                            : make_map_3d(args.v, r.num_adapters, args.n, r.rank, 64, 128);
-    const CUtensorMap map_y = make_map_out(args.y, r.num_rows, args.n, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2);
-    launch_clusters(lora_gemm_kernel<BN>, grid, 320, args.cluster, lora_gemm_smem_bytes<BN>(), true, stream, map_x, map_w, map_v, map_y, args);
+    const auto maps = gemm_maps(args, x, w);
+    launch_clusters(lora_gemm_kernel, grid, 320, args.cluster, kLoraGemmSmemBytes, true, stream, maps.x, maps.w, maps.v, maps.y, args);
+}
+
+void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, cudaStream_t stream) {
+    args.m_tiles = math::ceil_div(args.rows.num_rows, 2 * kLoraTileRows), args.n_tiles = math::ceil_div(args.n, 256), args.cluster = 1;
+    const int64_t tiles = int64_t(args.m_tiles) * args.n_tiles;
+    EP_HOST_ASSERT_MSG(tiles < (int64_t(1) << 30), "too many tiles for one launch");
+    const auto maps = gemm_maps(args, x, w);
+    launch_clusters(lora_gemm_pair_kernel, 2 * std::min<int64_t>(tiles, sms / 2), 320, 2, kLoraPairSmemBytes, true, stream, maps.x, maps.w, maps.v, maps.y, args);
 }
 
 // Few rows: columns per tile and CTAs per cluster by an estimate of the time. W comes from memory at 6.5 TB/s however it is
@@ -151,11 +166,12 @@ void lora_gemm(LoraGemmArgs args, const void* x, const void* w, cudaStream_t str
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
     const int sms = device_sms();
-    const int64_t rows = args.rows.num_rows, m_tiles = math::ceil_div<int64_t>(rows, kLoraTileRows);
+    const int64_t rows = args.rows.num_rows;
     if (rows * args.rows.rank <= kFewTerms and launch_gemm_few(args, x, w, sms, stream)) return;
-    // 256 columns per tile as soon as that gives every SM a tile: half the shared-memory traffic per product
-    if (m_tiles * math::ceil_div(args.n, 256) >= sms) launch_gemm<256>(args, x, w, sms, stream);
-    else launch_gemm<128>(args, x, w, sms, stream);
+    // 256 x 256 tiles by pairs of CTAs as soon as every pair has one; smaller tiles keep more SMs busy before that
+    const int64_t pair_tiles = math::ceil_div<int64_t>(rows, 2 * kLoraTileRows) * math::ceil_div(args.n, 256);
+    if (rows > kLoraTileRows and sms >= 2 and pair_tiles >= sms / 2) launch_gemm_pair(args, x, w, sms, stream);
+    else launch_gemm(args, x, w, sms, stream);
 }
 
 void lora_wgrad(LoraWgradArgs args, const void* x, cudaStream_t stream) {

@@ -100,9 +100,9 @@ inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, do
     s.idx = idx.data_ptr(), s.idx64 = idx.scalar_type() == torch::kInt64, s.num_tokens = num_tokens, s.num_rows = num_rows;
     // a sum is written over the whole row, so only rows without a token need zeros
     s.touched = accumulate ? nullptr : reinterpret_cast<uint32_t*>(ints.data_ptr<int>() + sort_ints);
+    g.touched = s.touched;
     s.num_crossing = g.num_crossing = ints.data_ptr<int>() + sort_ints + bitmap_ints, g.crossing = g.num_crossing + 1;
     launch::embedding_sort(s, ints.data_ptr<int>(), &g.ids, &g.order, stream);
-    g.touched = s.touched;
     launch::embedding_grad(g, in_type, out_type, stream);
 }
 

@@ -181,6 +181,16 @@ EP_DEVICE uint32_t map_to_cta(const void* local_ptr, uint32_t rank) {
 EP_DEVICE void mbarrier_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// One poll for a phase that another CTA of the cluster takes part in
+EP_DEVICE bool mbarrier_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(ptx::smem_addr(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 EP_DEVICE void tmem_alloc_pair(uint32_t* smem_slot, uint32_t num_columns) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(ptx::smem_addr(smem_slot)), "r"(num_columns) : "memory");

@@ -169,6 +169,11 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const __grid_cons
 // ---------------------------------------------------------------------------------------- stable sort by id
 namespace emb_detail {
 
+// (the bitmap is zero before the sort begins)
+EP_DEVICE void mark_touched(const EmbSortArgs& a, int key) {
+    if (a.touched != nullptr and key < a.num_rows) atomicOr(a.touched + (key >> 5), 1u << (key & 31));
+}
+
 // Key of position i in pass `pass`: the id itself in the first pass (ids outside the table become `num_rows`), the previous
 // pass's output afterwards.
 EP_DEVICE int sort_key(const EmbSortArgs& a, int pass, int i) {
@@ -205,7 +210,7 @@ EP_DEVICE void sort_scatter(const EmbSortArgs& a, int pass, int* counters, int b
             const int place = counters[digit] + __popc(peers & ptx::lanemask_lt());
             out_keys[place] = key;
             out_vals[place] = pass > 0 ? a.vals[(pass + 1) & 1][i] : i;
-            if (pass == 0 and a.touched != nullptr and key < a.num_rows) atomicOr(a.touched + (key >> 5), 1u << (key & 31));
+            if (pass == 0) mark_touched(a, key);
         }
         __syncwarp();
         if (active and (peers & ptx::lanemask_lt()) == 0) counters[digit] += __popc(peers);
@@ -271,6 +276,45 @@ EP_DEVICE void prefix_over_warps(int* counters, int* totals, int bins) {
 
 }  // namespace emb_detail
 
+// Small batches: the place of a key is the number of keys before it (smaller, or equal and earlier), counted outright. A CTA
+// counts for 32 keys, its 32 warps over a part of all keys each. n^2 comparisons are 67 million for 8192 keys, 2 us of this
+// GPU, and there is nothing to wait for in between; a radix sort has a chain of barriers per digit.
+__global__ void __launch_bounds__(kEmbRankThreads) embedding_rank_kernel(const __grid_constant__ EmbSortArgs a) {
+    using namespace emb_detail;
+    extern __shared__ int sort_smem[];                 // all keys, padded to a multiple of 32 with the largest number
+    __shared__ int counts[32];
+    constexpr int kWarps = kEmbRankThreads / 32;
+    const int lane = ptx::lane_id(), warp = threadIdx.x / 32, n = a.num_tokens, padded = math::align(n, 32);
+    cudaTriggerProgrammaticLaunchCompletion();         // the kernel of the sums may be set up meanwhile
+    if (blockIdx.x == 0 and threadIdx.x == 0) *a.num_crossing = 0;
+    if (threadIdx.x < 32) counts[threadIdx.x] = 0;
+    #pragma unroll 8
+    for (int i = threadIdx.x; i < padded; i += kEmbRankThreads) sort_smem[i] = i < n ? sort_key(a, 0, i) : 0x7fffffff;
+    __syncthreads();
+    const int first = blockIdx.x * 32, mine = first + lane, key = sort_smem[mine];
+    const int per_warp = math::align(math::ceil_div(padded, kWarps), 32);
+    const int begin = min(warp * per_warp, padded), end = min(begin + per_warp, padded);
+    int count = 0;
+    // in groups of 32: those before this CTA's count smaller or equal keys, those behind it smaller ones, its own equal ones in
+    // lower lanes too
+    #pragma unroll 1
+    for (int group = begin; group < end; group += 32) {
+        const int limit = group < first ? key + 1 : key;
+        #pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const int4 k = *reinterpret_cast<const int4*>(sort_smem + group + j);
+            count += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+        }
+        if (group == first) count += __popc(__match_any_sync(0xffffffffu, key) & ptx::lanemask_lt());
+    }
+    atomicAdd(&counts[lane], count);
+    __syncthreads();
+    if (warp == 0 and mine < n) {
+        a.keys[0][counts[lane]] = key, a.vals[0][counts[lane]] = mine;
+        mark_touched(a, key);
+    }
+}
+
 // All passes in one launch: up to eight CTAs of a cluster hold the keys in their shared memory. Per pass every warp ranks its
 // keys (in registers) per digit, the CTAs exchange their counts, and each key goes straight into the shared memory of the CTA
 // that owns its place (the last pass writes to memory). The time is latency (match, barriers), not work, so the keys are
@@ -292,22 +336,13 @@ __global__ void __launch_bounds__(kEmbClusterThreads, 1) embedding_sort_cluster_
 
     cudaTriggerProgrammaticLaunchCompletion();                  // the kernel of the sums may be set up meanwhile
     if (rank == 0 and threadIdx.x == 0) *a.num_crossing = 0;
-    if (a.touched != nullptr)
-        for (int i = rank * kEmbClusterThreads + threadIdx.x; i < (a.num_rows + 31) / 32; i += ctas * kEmbClusterThreads) a.touched[i] = 0;
     int key[kRounds], val[kRounds];
     #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
         const int i = (warp * kRounds + r) * 32 + lane;
         val[r] = rank * kKeys + i;
         key[r] = i < count ? sort_key(a, 0, val[r]) : a.num_rows;
-    }
-    if (a.touched != nullptr) {
-        // (the bitmap is zero once every CTA of the cluster has passed here)
-        __threadfence();
-        tc::cluster_sync();
-        #pragma unroll
-        for (int r = 0; r < kRounds; ++r)
-            if ((warp * kRounds + r) * 32 + lane < count and key[r] < a.num_rows) atomicOr(a.touched + (key[r] >> 5), 1u << (key[r] & 31));
+        mark_touched(a, key[r]);
     }
     for (int pass = 0; pass < a.num_passes; ++pass) {
         const int shift = pass * a.digit_bits;
@@ -389,9 +424,6 @@ __global__ void __launch_bounds__(kEmbSortThreads) embedding_sort_count_kernel(c
     const int begin = int(min(first, int64_t(a.num_tokens))), end = int(min(first + a.keys_per_warp, int64_t(a.num_tokens)));
     for (int i = threadIdx.x; i < kWarps * bins; i += kEmbSortThreads) sort_smem[i] = 0;
     if (a.pass == 0 and blockIdx.x == 0 and threadIdx.x == 0) *a.num_crossing = 0;
-    if (a.pass == 0 and a.touched != nullptr)
-        for (int i = blockIdx.x * kEmbSortThreads + threadIdx.x; i < (a.num_rows + 31) / 32; i += gridDim.x * kEmbSortThreads)
-            a.touched[i] = 0;
     __syncthreads();
     sort_count(a, a.pass, sort_smem + warp * bins, begin, end, lane);
     __syncthreads();
@@ -454,7 +486,8 @@ EP_DEVICE void add_sum(float* out, float scale, const float (&acc)[kElems], cons
 // One warp per (chunk of sorted positions, slice of 32 * kElems * kPacks columns): the rows of a run are added in registers,
 // kAhead rows in flight. When the sums are added to a buffer, the rows that end in the group of kAhead are read ahead too:
 // a read at the end of each run would be a round trip to memory per id. Further warps write the zero rows of a dense gradient,
-// whose bytes are most of the work when the table is much larger than the batch.
+// whose bytes are most of the work when the table is much larger than the batch; a row each, so that they end together
+// (a range of rows per CTA, with the range's ids searched for instead of marked, took a third longer).
 template <typename In, typename Out, int kElems, int kPacks, bool kAccumulate>
 __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(const __grid_constant__ EmbGradArgs a) {
     using namespace emb_detail;
@@ -463,12 +496,11 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(const __grid_con
     cudaTriggerProgrammaticLaunchCompletion();                  // the join kernel may be set up meanwhile
     cudaGridDependencySynchronize();                            // the sort is done
     const unsigned slices = math::ceil_div(unsigned(a.hidden), 32u * kElems * kPacks);
-    const int64_t item = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
-    const int64_t sum_items = int64_t(a.num_chunks) * slices;
+    const int64_t item = int64_t(blockIdx.x) * 8 + threadIdx.x / 32, sum_items = int64_t(a.num_chunks) * slices;
     if (item >= sum_items) {
         // ---- rows without a token
         const int64_t row = item - sum_items;
-        if (a.touched == nullptr or row >= a.num_rows or ((a.touched[row >> 5] >> (row & 31)) & 1u)) return;
+        if (a.accumulate or row >= a.num_rows or ((a.touched[row >> 5] >> (row & 31)) & 1u)) return;
         const float nothing[kElems] = {};
         const Pack<Out, kElems> zero = pack<Out, kElems>(nothing);
         for (int c = lane * kElems; c < a.hidden; c += 32 * kElems)

@@ -33,10 +33,12 @@ struct EmbSortArgs {
     int *keys[2], *vals[2];   // [num_tokens]; many launches: pass p reads buffer (p + 1) % 2 (pass 0: `idx`) and writes p % 2;
                               // one launch: the result goes to buffer 0
     int* hist;                // form of many launches: [num_ctas][2^digit_bits] counts of this pass
-    uint32_t* touched;        // optional bitmap over the rows (bit set = the row receives a gradient), zeroed by pass 0
+    uint32_t* touched;        // optional bitmap over the rows (bit set = the row receives a gradient)
     int* num_crossing;        // set to 0 for the kernels that follow
 };
 
+constexpr int kEmbRankKeys = 8192;            // batches up to this size are ranked by counting
+constexpr int kEmbRankThreads = 1024;
 constexpr int kEmbSortThreads = 256;          // form of many launches: eight warps
 constexpr int kEmbClusterThreads = 1024;      // form of one launch: a cluster of up to eight CTAs ...
 constexpr int kEmbClusterMaxRounds = 8;       // ... with up to this many keys per thread
@@ -54,7 +56,7 @@ struct EmbGradArgs {
     float* partial;           // [num_chunks][2][hidden]: the piece of a run that began in an earlier chunk, the piece of one that goes on
     void* out;                // [num_rows, hidden], `out_stride` elements between rows
     int64_t out_stride;
-    int accumulate;           // fp32 `out`: add to its contents; otherwise overwrite
+    int accumulate;           // fp32 `out`: add to its contents; otherwise overwrite, rows without a token with zeros
     const uint32_t* touched;  // overwrite: rows without a set bit are written as zeros
     int *num_crossing, *crossing;   // list of the chunks in which a run begins that goes on in the next
 };

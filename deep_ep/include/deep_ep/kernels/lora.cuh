@@ -35,15 +35,17 @@ EP_DEVICE int adapter_of(const LoraRows& r, int row) {
     return static_cast<uint64_t>(id) < static_cast<uint64_t>(r.num_adapters) ? static_cast<int>(id) : -1;
 }
 
-// The adapters of a tile's 128 rows, four rows per lane: enumerated in ascending order by minimum search, which needs no
-// list, no sort and no other kernel. Every role that needs the order walks it on its own.
+// The adapters of a tile's rows (128, or 256 for a pair of CTAs): enumerated in ascending order by minimum search, which needs
+// no list, no sort and no other kernel.
+template <int kRows>
 struct TileAdapters {
-    int id[4];
-    bool inside[4];
+    static constexpr int kPer = kRows / 32;
+    int id[kPer];
+    bool inside[kPer];
 
     EP_DEVICE void load(const LoraRows& r, int m0, int lane) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kPer; ++i) {
             const int row = m0 + lane + 32 * i;
             inside[i] = row < r.num_rows;
             id[i] = adapter_of(r, row);
@@ -52,7 +54,7 @@ struct TileAdapters {
     EP_DEVICE int next(int last) const {
         unsigned best = kNone;
         #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kPer; ++i)
             if (id[i] > last) best = min(best, static_cast<unsigned>(id[i]));
         return static_cast<int>(__reduce_min_sync(0xffffffffu, best));
     }
@@ -60,7 +62,7 @@ struct TileAdapters {
     EP_DEVICE bool others_than(int e) const {
         bool other = false;
         #pragma unroll
-        for (int i = 0; i < 4; ++i) other = other or (inside[i] and id[i] != e);
+        for (int i = 0; i < kPer; ++i) other = other or (inside[i] and id[i] != e);
         return __any_sync(0xffffffffu, other);
     }
 };
@@ -106,6 +108,107 @@ EP_DEVICE int ld_cluster_int(uint32_t addr) {
     int v;
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
+}
+
+// Product of a row's t with what the writers have kept from the tensor cores at column n: infinities and NaN of the row's adapter,
+// by whole units of eight V elements
+__device__ __noinline__ float poisoned(const LoraGemmArgs& a, int row, int n) {
+    const int e = adapter_of(a.rows, row);
+    if (e < 0) return 0.0f;
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
+    const float* t = a.t + int64_t(row) * a.rows.rank;
+    float sum = 0.0f;
+    if (a.mn_major) {
+        for (int r = 0; r < a.rows.rank; ++r) {
+            const __nv_bfloat16* unit = v + int64_t(r) * a.n + (n & ~7);
+            if (has_non_finite(*reinterpret_cast<const uint4*>(unit))) sum += t[r] * __bfloat162float(unit[n & 7]);
+        }
+    } else {
+        for (int r = 0; r < a.rows.rank; r += 8) {
+            const __nv_bfloat16* unit = v + int64_t(n) * a.rows.rank + r;
+            if (has_non_finite(*reinterpret_cast<const uint4*>(unit)))
+                for (int j = 0; j < 8; ++j) sum += t[r + j] * __bfloat162float(unit[j]);
+        }
+    }
+    return sum;
+}
+
+// This row's t, 32 columns from 32 * c, as bf16 hi and lo
+EP_DEVICE void read_t(const LoraGemmArgs& a, int row, bool there, int c, uint4 (&hi)[4], uint4 (&lo)[4]) {
+    #pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        float v[8] = {};
+        if (there and 32 * c + 8 * u < a.rows.rank) load8(a.t + int64_t(row) * a.rows.rank + 32 * c + 8 * u, v);
+        split8(v, hi[u], lo[u]);
+    }
+}
+// A row's line of an A slot: hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8)
+EP_DEVICE void write_t(uint8_t* slot, int row, bool there, const uint4 (&hi)[4], const uint4 (&lo)[4]) {
+    uint8_t* line = slot + row * 128;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    #pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = there ? hi[u] : zero;
+        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = there ? lo[u] : zero;
+    }
+}
+// Takes infinities and NaN (whole units) out of the part of a V block that the products read: 32 columns of `columns` lines, or
+// (mn_major) 32 lines of each block of 64 columns. 128 threads; true where this thread found one.
+EP_DEVICE bool take_out_non_finite(uint8_t* block, int columns, bool mn_major, int thread) {
+    bool found = false;
+    const auto look = [&](uint8_t* at) {
+        uint4* unit = reinterpret_cast<uint4*>(at);
+        if (has_non_finite(*unit)) *unit = make_uint4(0, 0, 0, 0), found = true;
+    };
+    if (mn_major) {
+        for (int i = thread; i < columns / 64 * 32 * 8; i += 128) look(block + (i / 256) * 8192 + (i % 256) * 16);
+    } else {
+        for (int i = thread; i < columns * 4; i += 128) look(block + (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4));
+    }
+    return found;
+}
+
+// Epilogue of one warp: its 32 rows of an accumulator of `columns` columns, rounded to bf16 and stored by the TMA through a 4 KB
+// buffer (what lies beyond the matrix is cut off by the store). `fix`: add what the tensor cores did not get.
+EP_DEVICE void store_tile(const CUtensorMap* map_y, const LoraGemmArgs& a, uint32_t taddr, uint8_t* buffer, int row0, int n0, int columns, bool fix, int lane) {
+    uint8_t* line = buffer + lane * 128;
+    if (fix) cudaGridDependencySynchronize();
+    for (int c = 0; c < columns; c += 64) {
+        if (lane == 0) ptx::bulk_wait_read<0>();
+        __syncwarp();
+        if (not fix) {
+            uint32_t lo[32], hi[32];
+            tc::tmem_ld_32x32(taddr + c, lo);
+            tc::tmem_ld_32x32(taddr + c + 32, hi);
+            tc::wait_ld();
+            #pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                uint32_t w[4], w2[4];
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = ptx::float2_to_bf16x2(__uint_as_float(lo[8 * u + 2 * j]), __uint_as_float(lo[8 * u + 2 * j + 1]));
+                    w2[j] = ptx::float2_to_bf16x2(__uint_as_float(hi[8 * u + 2 * j]), __uint_as_float(hi[8 * u + 2 * j + 1]));
+                }
+                *reinterpret_cast<uint4*>(line + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(line + (((4 + u) ^ (lane & 7)) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+            }
+        } else {
+            for (int j = 0; j < 64; ++j) {
+                const uint32_t r = tc::tmem_ld_32x1(taddr + c + j);
+                tc::wait_ld();
+                float v = __uint_as_float(r);
+                if (row0 + lane < a.rows.num_rows and n0 + c + j < a.n) v += poisoned(a, row0 + lane, n0 + c + j);
+                __syncwarp();
+                *reinterpret_cast<__nv_bfloat16*>(line + (((j / 8) ^ (lane & 7)) << 4) + (j % 8) * 2) = __float2bfloat16_rn(v);
+            }
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 and row0 < a.rows.num_rows and n0 + c < a.n) {
+            tc::tma_store_2d(map_y, n0 + c, row0, buffer);
+            ptx::bulk_commit();
+        }
+    }
 }
 
 // A row of the accumulator (`columns` fp32, a multiple of 32) to shared memory at `to`, possibly of another CTA of the cluster.
@@ -155,6 +258,18 @@ EP_DEVICE bool wait(uint64_t* bar, uint32_t parity, volatile int* error_flag) {
         if (ptx::mbarrier_wait(bar, parity, 1 << 20, 100000000ull)) return true;
     }
     *error_flag = 1;
+    return false;
+}
+EP_DEVICE bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* error_flag) {
+    if (tc::mbarrier_try_wait_cluster(bar, parity)) return true;
+    const unsigned long long start = ptx::globaltimer_ns();
+    #pragma unroll 1
+    while (not *error_flag) {
+        #pragma unroll 1
+        for (int i = 0; i < 64; ++i)
+            if (tc::mbarrier_try_wait_cluster(bar, parity)) return true;
+        if (ptx::globaltimer_ns() - start > 10000000000ull) *error_flag = 1;
+    }
     return false;
 }
 EP_DEVICE bool wait_all_lanes(uint64_t* bar, uint32_t parity, volatile int* error_flag) {
@@ -219,7 +334,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     }
     if (warp == 0) {
         // this chunk's adapters
-        TileAdapters rows;
+        TileAdapters<kLoraTileRows> rows;
         rows.load(a.rows, m0, lane);
         int e = rows.next(-1);
         for (int i = 0; i < chunk * a.chunk and e != kNone; ++i) e = rows.next(e);
@@ -440,22 +555,15 @@ lora_shrink_rows_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16
 // Many tiles: persistent CTAs, two accumulators in tensor memory, so that the stores of one tile overlap the products of the
 // next. Few tiles (decode): a cluster shares the tile's contraction, so that all SMs pull on W; its CTAs send their parts
 // of a row to the CTA that owns the row, which adds them in rank order.
-constexpr int kLoraSplitBytes = 128 * 128 * 4;             // parts of the rows a CTA owns, BN = 128
+constexpr int kLoraGemmColumns = 128, kLoraGemmStages = 5;
+constexpr int kLoraGemmSmemBytes = kLoraGemmStages * (kLoraTileRows + kLoraGemmColumns) * kLoraBlockK * 2 + kLoraTileRows * kLoraGemmColumns * 4 + 1024;
 
-template <int BN>
-constexpr int lora_gemm_stages() { return BN == 256 ? 4 : 5; }
-template <int BN>
-constexpr int lora_gemm_smem_bytes() {
-    return lora_gemm_stages<BN>() * (kLoraTileRows + BN) * kLoraBlockK * 2 + (BN == 256 ? 4 * 4096 : kLoraSplitBytes) + 1024;
-}
-
-template <int BN>
 __global__ void __launch_bounds__(320, 1)
 lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_y, const __grid_constant__ LoraGemmArgs a) {
     using namespace lora_detail;
     extern __shared__ uint8_t smem_raw[];
-    constexpr int kStages = lora_gemm_stages<BN>(), kGroupM = 16;
+    constexpr int BN = kLoraGemmColumns, kStages = kLoraGemmStages, kGroupM = 16;
     constexpr uint32_t kABytes = kLoraTileRows * kLoraBlockK * 2, kBBytes = BN * kLoraBlockK * 2;
     constexpr int kPoisonSlots = 8;           // more tiles than the writers can be ahead of the epilogue
     __shared__ uint64_t full_bar[kStages], empty_bar[kStages], grant_bar[kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
@@ -515,29 +623,6 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     tc::fence_after_thread_sync();
     const uint32_t tmem = tmem_slot;
     if (split) tc::cluster_arrive();          // (waited for before the first access to another CTA's shared memory)
-
-    // product of this row's t with what the writers have kept from the tensor cores at column n: infinities and NaN of the row's
-    // adapter, by whole units of eight V elements
-    const auto poisoned = [&](int row, int n) {
-        const int e = adapter_of(a.rows, row);
-        if (e < 0) return 0.0f;
-        const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
-        const float* t = a.t + int64_t(row) * a.rows.rank;
-        float sum = 0.0f;
-        if (a.mn_major) {
-            for (int r = 0; r < a.rows.rank; ++r) {
-                const __nv_bfloat16* unit = v + int64_t(r) * a.n + (n & ~7);
-                if (has_non_finite(*reinterpret_cast<const uint4*>(unit))) sum += t[r] * __bfloat162float(unit[n & 7]);
-            }
-        } else {
-            for (int r = 0; r < a.rows.rank; r += 8) {
-                const __nv_bfloat16* unit = v + int64_t(n) * a.rows.rank + r;
-                if (has_non_finite(*reinterpret_cast<const uint4*>(unit)))
-                    for (int j = 0; j < 8; ++j) sum += t[r + j] * __bfloat162float(unit[j]);
-            }
-        }
-        return sum;
-    };
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -638,7 +723,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
             int m0, n0;
             origin(tile, m0, n0);
-            TileAdapters rows;
+            TileAdapters<kLoraTileRows> rows;
             rows.load(a.rows, m0, lane);
             const int mine = adapter_of(a.rows, m0 + row), slot = local & 1;
             if (warp == 6) {
@@ -652,54 +737,26 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
             }
             it += kb1 - kb0;
-            // this row's t, 32 columns as bf16 hi and lo: read before the ring has room for it, and once per tile when the rank
-            // is not larger (with many adapters per tile, a read per adapter would be a round trip to L2 each)
+            // read before the ring has room for it, and once per tile when the rank is not above 32 (with many adapters per tile, a
+            // read per adapter would be a round trip to L2 each)
             uint4 hi[4], lo[4];
-            const auto read = [&](int c) {
-                #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float v[8];
-                    const bool there = mine >= 0 and 32 * c + 8 * u < a.rows.rank;
-                    if (there) load8(a.t + int64_t(m0 + row) * a.rows.rank + 32 * c + 8 * u, v);
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = there ? v[j] : 0.0f;
-                    split8(v, hi[u], lo[u]);
-                }
-            };
-            if (rank_chunks == 1) read(0);
+            if (rank_chunks == 1) read_t(a, m0 + row, mine >= 0, 0, hi, lo);
             int turn = 0;
             for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
                 if (turn % cluster != rank) continue;
                 const bool shared_tile = rows.others_than(e);
                 for (int c = 0; c < rank_chunks and ok; ++c, ++it) {
                     const unsigned s = it % kStages, phase = (it / kStages) & 1;
-                    if (rank_chunks > 1 and mine == e) read(c);
+                    if (rank_chunks > 1 and mine == e) read_t(a, m0 + row, true, c, hi, lo);
                     ok = wait_all_lanes(&grant_bar[s], (granted >> s) & 1, &error_flag);
                     granted ^= 1u << s;
                     if (not ok) break;
-                    uint8_t* line = smem_a + s * kABytes + row * 128;
-                    const uint4 zero = make_uint4(0, 0, 0, 0);
-                    #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        // 16-byte unit u of row r sits at unit u ^ (r % 8) of its 128-byte line
-                        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = mine == e ? hi[u] : zero;
-                        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = mine == e ? lo[u] : zero;
-                    }
+                    write_t(smem_a + s * kABytes, row, mine == e, hi, lo);
                     if (shared_tile) {
                         // infinities and NaN of this adapter must not meet the zeros of other rows
                         ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
                         if (not ok) break;
-                        uint8_t* sb = smem_b + s * kBBytes;
-                        // the part of the block that the products read: 32 columns of BN lines, or 32 lines of each 64-column block
-                        const auto look = [&](uint8_t* at) {
-                            uint4* unit = reinterpret_cast<uint4*>(at);
-                            if (has_non_finite(*unit)) *unit = make_uint4(0, 0, 0, 0), poison[local % kPoisonSlots] = local + 1;
-                        };
-                        if (a.mn_major) {
-                            for (int i = row; i < BN / 64 * 32 * 8; i += 128) look(sb + (i / 256) * 8192 + (i % 256) * 16);
-                        } else {
-                            for (int i = row; i < BN * 4; i += 128) look(sb + (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4));
-                        }
+                        if (take_out_non_finite(smem_b + s * kBBytes, BN, a.mn_major, row)) poison[local % kPoisonSlots] = local + 1;
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
@@ -734,46 +791,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 tc::fence_before_thread_sync();
                 break;                        // one tile per cluster
             }
-            const bool fix = poison[local % kPoisonSlots] == local + 1;          // rare; the same for the whole warp
-            if (fix) cudaGridDependencySynchronize();
-            for (int c = 0; c < BN; c += 64) {
-                uint8_t* line = buffer + lane * 128;
-                if (lane == 0) ptx::bulk_wait_read<0>();
-                __syncwarp();
-                if (not fix) {
-                    uint32_t lo[32], hi[32];
-                    tc::tmem_ld_32x32(taddr + c, lo);
-                    tc::tmem_ld_32x32(taddr + c + 32, hi);
-                    tc::wait_ld();
-                    #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint32_t w[4], w2[4];
-                        #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            w[j] = ptx::float2_to_bf16x2(__uint_as_float(lo[8 * u + 2 * j]), __uint_as_float(lo[8 * u + 2 * j + 1]));
-                            w2[j] = ptx::float2_to_bf16x2(__uint_as_float(hi[8 * u + 2 * j]), __uint_as_float(hi[8 * u + 2 * j + 1]));
-                        }
-                        *reinterpret_cast<uint4*>(line + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (lane & 7)) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
-                    }
-                } else {
-                    for (int j = 0; j < 64; ++j) {
-                        const uint32_t r = tc::tmem_ld_32x1(taddr + c + j);
-                        tc::wait_ld();
-                        float v = __uint_as_float(r);
-                        if (m0 + row < a.rows.num_rows and n0 + c + j < a.n) v += poisoned(m0 + row, n0 + c + j);
-                        __syncwarp();
-                        *reinterpret_cast<__nv_bfloat16*>(line + (((j / 8) ^ (lane & 7)) << 4) + (j % 8) * 2) = __float2bfloat16_rn(v);
-                    }
-                }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                // rows and columns beyond the matrix are cut off by the store itself
-                if (lane == 0 and m0 + quarter * 32 < a.rows.num_rows and n0 + c < a.n) {
-                    tc::tma_store_2d(&map_y, n0 + c, m0 + quarter * 32, buffer);
-                    ptx::bulk_commit();
-                }
-            }
+            store_tile(&map_y, a, taddr, buffer, m0 + quarter * 32, n0, BN, poison[local % kPoisonSlots] == local + 1, lane);
             tc::fence_before_thread_sync();
             __syncwarp();
             if (lane == 0) ptx::mbarrier_arrive(&tmem_empty_bar[acc]);
@@ -799,7 +817,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             float v[8] = {};
             add_parts(v, smem_out, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
             if (fix)
-                for (int j = 0; j < 8; ++j) v[j] += poisoned(m0 + row, n0 + c + j);
+                for (int j = 0; j < 8; ++j) v[j] += poisoned(a, m0 + row, n0 + c + j);
             store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c, v);
         }
         tc::cluster_sync();                   // nobody leaves while others look at its flag
@@ -810,6 +828,242 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     if (warp == 1) {
         tc::fence_after_thread_sync();
         tc::tmem_dealloc(tmem, split ? BN : 2 * BN);
+    }
+    if (threadIdx.x == 0) report(error_flag != 0, a.rows.status);
+}
+
+// The same by pairs of CTAs (`cta_group::2`) for many tiles: 256 x 256 per pair, each CTA with its 128 rows of A, half of the 256
+// columns of B, and the accumulator of its rows. A CTA alone reads 12 KB of shared memory for the products of a K step of 16 and
+// takes in as much from the TMA: 192 bytes per clock, where shared memory has 128. A pair needs a third less per SM. Measured
+// with 8101 rows, K 7168, N 4096, rank 64: 351 us with 128 x 256 tiles by single CTAs.
+// The MMAs are issued by the even CTA; barriers that concern it count both CTAs. A V block lands on a barrier of its own CTA,
+// where the writers look at it; the even CTA learns from the writers of both that the block is complete.
+constexpr int kLoraPairStages = 6;
+constexpr int kLoraPairSmemBytes = kLoraPairStages * 2 * 128 * kLoraBlockK * 2 + 4 * 4096 + 1024;
+
+__global__ void __launch_bounds__(320, 1)
+lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ CUtensorMap map_y, const __grid_constant__ LoraGemmArgs a) {
+    using namespace lora_detail;
+    extern __shared__ uint8_t smem_raw[];
+    constexpr int kStages = kLoraPairStages, kGroupM = 8, kPoisonSlots = 8;
+    constexpr uint32_t kHalf = 128 * kLoraBlockK * 2;          // 128 rows of A, or 128 columns of B: 16 KB
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], v_bar[kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ uint64_t list_full_bar[2], list_empty_bar[2];
+    __shared__ int list[2][2 * kLoraTileRows], list_size[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int error_flag, poison[kPoisonSlots];
+
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
+    const int half = int(tc::cluster_ctarank());               // 0: even CTA, issues the MMAs
+    const bool leader = half == 0;
+    const int num_tiles = a.m_tiles * a.n_tiles, first_tile = int(blockIdx.x) / 2, tile_step = int(gridDim.x) / 2;
+    const int blocks = math::ceil_div(a.k, kLoraBlockK), rank_chunks = math::ceil_div(a.rows.rank, 32);
+    uint8_t* smem_a = align_1024(smem_raw);
+    uint8_t* smem_b = smem_a + kStages * kHalf;
+    uint8_t* smem_out = smem_b + kStages * kHalf;
+
+    // tile -> origin, see above
+    const auto origin = [&](int tile, int& m0, int& n0) {
+        const int group = tile / (kGroupM * a.n_tiles), first_m = group * kGroupM, gm = min(kGroupM, a.m_tiles - first_m);
+        const int local = tile - group * kGroupM * a.n_tiles;
+        m0 = (first_m + local % gm) * 2 * kLoraTileRows, n0 = local / gm * 256;
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s)
+            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&v_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 8);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 8);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], leader ? 2 : 1);
+        }
+        ptx::fence_mbarrier_init();
+        error_flag = 0;
+        for (int i = 0; i < kPoisonSlots; ++i) poison[i] = 0;
+    }
+    if (threadIdx.x == 64) tc::prefetch_tensormap(&map_x), tc::prefetch_tensormap(&map_w), tc::prefetch_tensormap(&map_v), tc::prefetch_tensormap(&map_y);
+    __syncthreads();
+    tc::cluster_sync();                       // both CTAs' barriers exist before anyone signals across the pair
+    if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 512);
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    tc::fence_after_thread_sync();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer (both CTAs)
+        Ring ring;
+        int issued = 0, local = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
+            int m0, n0;
+            origin(tile, m0, n0);
+            const int m_half = m0 + 128 * half, n_half = n0 + 128 * half;
+            for (int kb = 0; kb < blocks; ++kb) {
+                ok = wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag);
+                if (not ok) break;
+                if (elect_one()) {
+                    // the bytes of both CTAs are counted on the even CTA's barrier
+                    const uint32_t bar = tc::map_to_cta(&full_bar[ring.slot], 0);
+                    if (leader) ptx::mbarrier_arrive_expect_tx(&full_bar[ring.slot], 4 * kHalf);
+                    const int k0 = kb * kLoraBlockK;
+                    uint8_t* sb = smem_b + ring.slot * kHalf;
+                    tc::tma_load_2d_pair(smem_a + ring.slot * kHalf, &map_x, k0, m_half, bar);
+                    if (a.mn_major) {
+                        tc::tma_load_2d_pair(sb, &map_w, n_half, k0, bar);
+                        tc::tma_load_2d_pair(sb + 8192, &map_w, n_half + 64, k0, bar);
+                    } else {
+                        tc::tma_load_2d_pair(sb, &map_w, k0, n_half, bar);
+                    }
+                }
+                ++issued, ring.advance(kStages);
+            }
+            const int slot = local & 1;
+            ok = ok and wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
+            if (not ok) break;
+            const int size = list_size[slot];
+            for (int i = 0; i < size and ok; ++i) {
+                const int e = list[slot][i];
+                for (int c = 0; c < rank_chunks; ++c) {
+                    ok = wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag);
+                    if (not ok) break;
+                    if (elect_one()) {
+                        uint64_t* bar = &v_bar[ring.slot];
+                        ptx::mbarrier_arrive_expect_tx(bar, kHalf);
+                        uint8_t* sb = smem_b + ring.slot * kHalf;
+                        if (a.mn_major) {
+                            tc::tma_load_3d(sb, &map_v, n_half, 32 * c, e, bar);
+                            tc::tma_load_3d(sb + 8192, &map_v, n_half + 64, 32 * c, e, bar);
+                        } else {
+                            tc::tma_load_3d(sb, &map_v, 32 * c, n_half, e, bar);
+                        }
+                    }
+                    ++issued, ring.advance(kStages);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
+        }
+        // what this CTA asked for has landed, and been read by the MMAs, before it leaves (a bounded wait also when somebody gave up)
+        for (int i = max(0, issued - kStages); i < issued; ++i) ptx::mbarrier_wait(&empty_bar[i % kStages], (i / kStages) & 1);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer (even CTA only)
+        const uint32_t idesc = tc::make_idesc(tc::kFormatBF16, 256, 256, false, a.mn_major);
+        const uint32_t b_lead = a.mn_major ? 8192 : 16, b_k = (a.mn_major ? 2048 : 32) >> 4;
+        const uint64_t desc_a0 = tc::make_smem_desc(smem_a, 16, 1024), desc_b0 = tc::make_smem_desc(smem_b, b_lead, 1024);
+        Ring ring;
+        unsigned full_phase = 0, ext_phase = 0;       // per slot: a slot's blocks of x and of V complete on different barriers
+        int local = 0;
+        for (int tile = leader ? first_tile : num_tiles; tile < num_tiles; tile += tile_step, ++local) {
+            const int acc = local & 1, slot = local & 1;
+            const uint32_t d = tmem + acc * 256;
+            wait_cluster(&tmem_empty_bar[acc], ((local >> 1) & 1) ^ 1, &error_flag);
+            tc::fence_after_thread_sync();
+            for (int kb = 0; kb < blocks; ++kb, ring.advance(kStages)) {
+                wait(&full_bar[ring.slot], (full_phase >> ring.slot) & 1, &error_flag);
+                full_phase ^= 1u << ring.slot;
+                tc::fence_after_thread_sync();
+                if (elect_one()) {
+                    const uint64_t da = desc_a0 + uint64_t(ring.slot * (kHalf >> 4)), db = desc_b0 + uint64_t(ring.slot * (kHalf >> 4));
+                    #pragma unroll
+                    for (int k = 0; k < kLoraBlockK / 16; ++k) tc::mma_f16_pair(d, da + k * 2, db + k * b_k, idesc, kb > 0 or k > 0);
+                    tc::commit_pair(&empty_bar[ring.slot]);    // the stage is free in both CTAs once these MMAs have read it
+                }
+            }
+            const int size = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag) ? list_size[slot] : 0;
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
+            for (int i = 0; i < size * rank_chunks; ++i, ring.advance(kStages)) {
+                const int c = i % rank_chunks;
+                wait_cluster(&ext_bar[ring.slot], (ext_phase >> ring.slot) & 1, &error_flag);
+                ext_phase ^= 1u << ring.slot;
+                tc::fence_after_thread_sync();
+                if (elect_one()) {
+                    const uint64_t da = desc_a0 + uint64_t(ring.slot * (kHalf >> 4)), db = desc_b0 + uint64_t(ring.slot * (kHalf >> 4));
+                    for (int k = 0; k < 2 and 32 * c + 16 * k < a.rows.rank; ++k) {
+                        tc::mma_f16_pair(d, da + k * 2, db + k * b_k, idesc, true);             // hi
+                        tc::mma_f16_pair(d, da + 4 + k * 2, db + k * b_k, idesc, true);         // lo
+                    }
+                    tc::commit_pair(&empty_bar[ring.slot]);
+                }
+            }
+            if (elect_one()) tc::commit_pair(&tmem_full_bar[acc]);
+        }
+    } else if (warp >= 6) {
+        // ------------------------------------------------------------------ writers of the adapters' A operand (both CTAs, own rows)
+        cudaGridDependencySynchronize();      // t comes from the kernel before, which this one does not wait for until here
+        const int row = threadIdx.x - 192;
+        unsigned landed = 0;                  // per slot: parity of the next V block
+        int position = 0, local = 0;          // position in the ring
+        bool ok = true;
+        for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
+            int m0, n0;
+            origin(tile, m0, n0);
+            TileAdapters<2 * kLoraTileRows> rows;
+            rows.load(a.rows, m0, lane);
+            const int my_row = m0 + 128 * half + row, mine = adapter_of(a.rows, my_row), slot = local & 1;
+            if (warp == 6) {
+                // the adapters of the pair's 256 rows, for the producer and the MMA issuer
+                ok = wait_all_lanes(&list_empty_bar[slot], ((local >> 1) & 1) ^ 1, &error_flag);
+                int size = 0;
+                for (int e = rows.next(-1); e != kNone; e = rows.next(e), ++size)
+                    if (lane == 0) list[slot][size] = e;
+                if (lane == 0) list_size[slot] = size;
+                if (not ok) break;
+                if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
+            }
+            position = (position + blocks) % kStages;
+            uint4 hi[4], lo[4];
+            if (rank_chunks == 1) read_t(a, my_row, mine >= 0, 0, hi, lo);
+            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e)) {
+                const bool shared_tile = rows.others_than(e);
+                for (int c = 0; c < rank_chunks; ++c) {
+                    const int s = position;
+                    position = position + 1 == kStages ? 0 : position + 1;
+                    if (rank_chunks > 1 and mine == e) read_t(a, my_row, true, c, hi, lo);
+                    // the V block has landed, so the slot is this block's
+                    ok = wait_all_lanes(&v_bar[s], (landed >> s) & 1, &error_flag);
+                    landed ^= 1u << s;
+                    if (not ok) break;
+                    write_t(smem_a + s * kHalf, row, mine == e, hi, lo);
+                    // infinities and NaN of this adapter must not meet the zeros of other rows, in either CTA
+                    if (shared_tile and take_out_non_finite(smem_b + s * kHalf, 128, a.mn_major, row)) {
+                        for (int q = 0; q < 2; ++q)
+                            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(const_cast<const int*>(&poison[local % kPoisonSlots]), q)), "r"(local + 1) : "memory");
+                    }
+                    ptx::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tc::mbarrier_arrive_cluster(tc::map_to_cta(&ext_bar[s], 0));
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue (both CTAs, own rows)
+        const int quarter = warp & 3;
+        uint8_t* buffer = smem_out + quarter * 4096;
+        int local = 0;
+        for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++local) {
+            int m0, n0;
+            origin(tile, m0, n0);
+            const int acc = local & 1;
+            if (not __all_sync(0xffffffffu, wait_cluster(&tmem_full_bar[acc], (local >> 1) & 1, &error_flag))) break;
+            tc::fence_after_thread_sync();
+            store_tile(&map_y, a, tmem + acc * 256 + (uint32_t(quarter * 32) << 16), buffer, m0 + 128 * half + quarter * 32, n0, 256,
+                       poison[local % kPoisonSlots] == local + 1, lane);
+            tc::fence_before_thread_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbarrier_arrive_cluster(tc::map_to_cta(&tmem_empty_bar[acc], 0));
+        }
+        if (lane == 0) ptx::bulk_wait<0>();
+        __syncwarp();
+    }
+
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    tc::cluster_sync();                       // the pair's tensor memory is given back together
+    if (warp == 1) {
+        tc::fence_after_thread_sync();
+        tc::tmem_dealloc_pair(tmem, 512);
     }
     if (threadIdx.x == 0) report(error_flag != 0, a.rows.status);
 }
