@@ -13,7 +13,15 @@ using namespace kernels;
 
 namespace {
 
-constexpr int kFewTensors = 64;
+constexpr int kFewTensors = 64, kSomeTensors = 256;
+
+// The shortest table that holds `count` tensors: a launch copies all of it
+template <typename Launch>
+auto with_table(int count, Launch launch) {
+    if (count <= kFewTensors) return launch.template operator()<kFewTensors>();
+    if (count <= kSomeTensors) return launch.template operator()<kSomeTensors>();
+    return launch.template operator()<kGradMaxTensors>();
+}
 
 template <int kTensors>
 int fill_table(GradTable<kTensors>& table, const GradTensor* tensors, int count) {
@@ -63,8 +71,7 @@ int grad_square_sums(const std::vector<GradTensor>& tensors, double* partial, cu
     int sums = 0;
     for (size_t i = 0; i < tensors.size(); i += kGradMaxTensors) {
         const int count = static_cast<int>(std::min<size_t>(kGradMaxTensors, tensors.size() - i));
-        sums += count <= kFewTensors ? square_sum<kFewTensors>(tensors.data() + i, count, partial + sums, stream)
-                                     : square_sum<kGradMaxTensors>(tensors.data() + i, count, partial + sums, stream);
+        sums += with_table(count, [&]<int kTensors>() { return square_sum<kTensors>(tensors.data() + i, count, partial + sums, stream); });
     }
     return sums;
 }
@@ -74,8 +81,7 @@ void grad_norm_finish(const GradClipArgs& args, cudaStream_t stream) { launch_ea
 void grad_clip(const std::vector<GradTensor>& tensors, GradClipArgs args, cudaStream_t stream) {
     for (size_t i = 0; i < tensors.size(); i += kGradMaxTensors) {
         const int count = static_cast<int>(std::min<size_t>(kGradMaxTensors, tensors.size() - i));
-        if (count <= kFewTensors) clip<kFewTensors>(tensors.data() + i, count, args, stream);
-        else clip<kGradMaxTensors>(tensors.data() + i, count, args, stream);
+        with_table(count, [&]<int kTensors>() { clip<kTensors>(tensors.data() + i, count, args, stream); });
         args.norm = nullptr;
     }
 }

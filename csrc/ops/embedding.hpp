@@ -37,8 +37,9 @@ inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
 }
 
 // [*idx.shape, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
-inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale,
+inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx_in, double scale,
                                       const std::optional<torch::Tensor>& table_sf) {
+    const auto idx = idx_in.contiguous();
     check_rows(table), check_ids(idx, table);
     const auto type = embedding_type(table);
     EP_HOST_ASSERT_MSG((type == kernels::EmbType::kE4M3) == table_sf.has_value(), "an e4m3 table comes with its scales, another without");

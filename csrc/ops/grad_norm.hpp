@@ -3,6 +3,7 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -24,9 +25,23 @@ inline kernels::GradType gradient_type(const torch::Tensor& t) {
     }
 }
 
+// The tensors of a Python list or tuple, without a copy of each: a step's list may hold hundreds of them
+class TensorList {
+    pybind11::object sequence;
+
+public:
+    explicit TensorList(const pybind11::object& object) {
+        EP_HOST_ASSERT_MSG(PySequence_Check(object.ptr()), "a list or tuple of tensors");
+        sequence = pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(object.ptr(), "a list or tuple of tensors"));
+        for (size_t i = 0; i < size(); ++i) EP_HOST_ASSERT_MSG(THPVariable_Check(PySequence_Fast_GET_ITEM(sequence.ptr(), i)), "a list or tuple of tensors");
+    }
+    size_t size() const { return static_cast<size_t>(PySequence_Fast_GET_SIZE(sequence.ptr())); }
+    const torch::Tensor& operator[](size_t i) const { return THPVariable_Unpack(PySequence_Fast_GET_ITEM(sequence.ptr(), i)); }
+};
+
 // The tensors as flat memory. Written tensors may share no memory with each other or, other than element for element, with
 // a tensor that is read: two CTAs would then scale the same element.
-inline std::vector<launch::GradTensor> gradient_list(const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>* outs) {
+inline std::vector<launch::GradTensor> gradient_list(const TensorList& grads, const TensorList* outs) {
     struct Range {
         uintptr_t begin, end;
         bool written;
@@ -34,16 +49,18 @@ inline std::vector<launch::GradTensor> gradient_list(const std::vector<torch::Te
     std::vector<launch::GradTensor> list;
     std::vector<Range> ranges;
     list.reserve(grads.size());
+    EP_HOST_ASSERT_MSG(grads.size() > 0, "an empty list has no device");
     EP_HOST_ASSERT_MSG(outs == nullptr or outs->size() == grads.size(), "one output per gradient");
+    const auto device = grads[0].device();
     for (size_t i = 0; i < grads.size(); ++i) {
         const auto& g = grads[i];
-        EP_HOST_ASSERT_MSG(g.is_cuda() and g.device() == grads[0].device(), "gradients lie on one CUDA device");
+        EP_HOST_ASSERT_MSG(g.is_cuda() and g.device() == device, "gradients lie on one CUDA device");
         EP_HOST_ASSERT_MSG(g.is_non_overlapping_and_dense(), "gradients are dense (no gaps, no element twice)");
-        launch::GradTensor t = {g.data_ptr(), nullptr, g.numel(), gradient_type(g), gradient_type(g)};
+        launch::GradTensor t = {g.const_data_ptr(), nullptr, g.numel(), gradient_type(g), gradient_type(g)};
         const auto begin = reinterpret_cast<uintptr_t>(t.in);
         if (outs != nullptr) {
             const auto& o = (*outs)[i];
-            EP_HOST_ASSERT_MSG(o.device() == g.device() and o.sizes() == g.sizes() and o.is_non_overlapping_and_dense() and
+            EP_HOST_ASSERT_MSG(o.device() == device and o.sizes() == g.sizes() and o.is_non_overlapping_and_dense() and
                                (o.strides() == g.strides() or g.numel() <= 1), "an output has its gradient's shape, strides and device");
             t.out = o.data_ptr(), t.out_type = gradient_type(o);
             const auto out_begin = reinterpret_cast<uintptr_t>(t.out);
@@ -65,15 +82,19 @@ inline std::vector<launch::GradTensor> gradient_list(const std::vector<torch::Te
 }
 
 // fp64 sums of squares whose total is the squared norm; at least one element
-inline torch::Tensor grad_square_sums(const std::vector<torch::Tensor>& grads) {
-    EP_HOST_ASSERT_MSG(not grads.empty(), "an empty list has no device");
-    const auto list = gradient_list(grads, nullptr);
-    const c10::cuda::CUDAGuard guard(grads[0].device());
-    const auto options = grads[0].options().dtype(torch::kFloat64);
+inline torch::Tensor square_sums(const std::vector<launch::GradTensor>& list, c10::Device device) {
+    const c10::cuda::CUDAGuard guard(device);
+    const auto options = torch::TensorOptions().dtype(torch::kFloat64).device(device);
     if (list.empty()) return torch::zeros({1}, options);
     auto sums = torch::empty({launch::grad_norm_max_sums(static_cast<int>(list.size()))}, options);
     const int count = launch::grad_square_sums(list, sums.data_ptr<double>(), c10::cuda::getCurrentCUDAStream());
     return sums.narrow(0, 0, count);
+}
+
+inline torch::Tensor grad_square_sums(const pybind11::object& grads) {
+    const TensorList tensors(grads);
+    const auto list = gradient_list(tensors, nullptr);
+    return square_sums(list, tensors[0].device());
 }
 
 inline torch::Tensor grad_norm_finish(const torch::Tensor& sums) {
@@ -86,20 +107,22 @@ inline torch::Tensor grad_norm_finish(const torch::Tensor& sums) {
 }
 
 // the norm of one list
-inline torch::Tensor grad_norm(const std::vector<torch::Tensor>& grads) { return grad_norm_finish(grad_square_sums(grads)); }
+inline torch::Tensor grad_norm(const pybind11::object& grads) { return grad_norm_finish(grad_square_sums(grads)); }
 
 // outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), in place without `outs`; returns the norm
-inline torch::Tensor grad_clip(const std::vector<torch::Tensor>& grads, const std::optional<std::vector<torch::Tensor>>& outs,
-                               const std::optional<torch::Tensor>& sums, double max_norm) {
-    EP_HOST_ASSERT_MSG(not grads.empty(), "an empty list has no device");
-    const auto list = gradient_list(grads, outs.has_value() ? &*outs : &grads);
-    const c10::cuda::CUDAGuard guard(grads[0].device());
-    const auto total = sums.has_value() ? *sums : grad_square_sums(grads);
-    EP_HOST_ASSERT(total.device() == grads[0].device() and total.is_contiguous() and total.scalar_type() == torch::kFloat64);
+inline torch::Tensor grad_clip(const pybind11::object& grads, const pybind11::object& outs, const std::optional<torch::Tensor>& sums, double max_norm) {
+    const TensorList tensors(grads);
+    std::optional<TensorList> results;
+    if (not outs.is_none()) results.emplace(outs);
+    const auto list = gradient_list(tensors, results.has_value() ? &*results : &tensors);
+    const auto device = tensors[0].device();
+    const c10::cuda::CUDAGuard guard(device);
+    const auto total = sums.has_value() ? *sums : square_sums(list, device);
+    EP_HOST_ASSERT(total.device() == device and total.is_contiguous() and total.scalar_type() == torch::kFloat64);
     if (list.empty()) return grad_norm_finish(total);
     auto norm = torch::empty({}, total.options().dtype(torch::kFloat32));
     kernels::GradClipArgs args = {total.data_ptr<double>(), static_cast<int>(total.numel()), static_cast<float>(max_norm),
-                                  norm.data_ptr<float>(), not outs.has_value()};
+                                  norm.data_ptr<float>(), not results.has_value()};
     launch::grad_clip(list, args, c10::cuda::getCurrentCUDAStream());
     return norm;
 }

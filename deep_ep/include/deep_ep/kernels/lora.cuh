@@ -317,7 +317,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     cudaTriggerProgrammaticLaunchCompletion();
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = blockIdx.x % cluster;
-    const int chunk = (blockIdx.x / cluster) % a.num_chunks, tile = blockIdx.x / cluster / a.num_chunks;
+    // (first chunks first: the later ones of most tiles are empty)
+    const int tiles = math::ceil_div(a.rows.num_rows, kLoraTileRows), tile = int(blockIdx.x / cluster) % tiles, chunk = int(blockIdx.x / cluster) / tiles;
     const int m0 = tile * kLoraTileRows;
     // columns of the accumulator per adapter: the rank, padded (by zeros that the TMA fills in) to what the operand's layout has
     const int rp = math::align(a.rows.rank, a.mn_major ? 64 : 16);

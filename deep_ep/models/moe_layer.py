@@ -160,6 +160,20 @@ class MoELayer(nn.Module):
                                   self.config.expert_alignment, backend=self.config.expert_backend, row_scale=recv_w,
                                   route=route, backward_route=backward_route)
 
+    def clip_grad_norm_(self, max_norm: float) -> torch.Tensor:
+        """Clip the layer's gradients in place by their global norm and return the norm (fp32 scalar on the device).
+
+        Expert gradients (the fp32 `main_grad` of a weight that has one, else its `.grad`) differ from rank to rank, and their
+        squares are added over the layer's group; those of the router and the shared expert are the same on every rank once they
+        have been reduced, which comes before this call, and count once. Collective over the group when it has several ranks."""
+        from ..ops.grad_norm import clip_grad_norm_
+        def gradients(names):
+            found = [getattr(self, name, None) for name in names]
+            found = [getattr(p, 'main_grad', None) if getattr(p, 'main_grad', None) is not None else p.grad for p in found if p is not None]
+            return [g for g in found if g is not None]
+        return clip_grad_norm_(gradients(('w_gate_up', 'w_down')), max_norm, group=self.group if self.num_ranks > 1 else None,
+                               replicated=gradients(('gate', 'shared_gate_up', 'shared_down')))
+
     # ------------------------------------------------------------------------------------------ FP8 inference
     def quantize_weights(self) -> None:
         """Store the routed experts' weights as e4m3 with one fp32 scale per 128 x 128 block (used by `forward_fp8`)."""

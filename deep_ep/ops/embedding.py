@@ -21,7 +21,7 @@ _TABLE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 def _lookup(table: torch.Tensor, idx: torch.Tensor, scale: float, table_sf: Optional[torch.Tensor]) -> torch.Tensor:
     if table.is_cuda:
-        return _C.embedding_lookup(table, idx.contiguous(), scale, table_sf)
+        return _C.embedding_lookup(table, idx, scale, table_sf)
     flat = idx.reshape(-1)
     valid = (flat >= 0) & (flat < table.size(0))
     rows = table.new_zeros((flat.numel(), table.size(1)), dtype=torch.float32)
@@ -61,6 +61,8 @@ def embedding_lookup(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0,
     is bf16. `idx` is int64 or int32 of any shape. Products are taken in fp32 and rounded once. The gradient reaches `table`
     (not an e4m3 one) in its own type, or its fp32 `main_grad`.
     """
+    if table.is_cuda and not (table.requires_grad and torch.is_grad_enabled()):
+        return _C.embedding_lookup(table, idx, scale, table_sf)          # (which looks at every argument)
     assert table.dim() == 2 and idx.dtype in (torch.int64, torch.int32), 'table [rows, hidden], idx int64 or int32'
     assert idx.device == table.device, 'table and indices lie on one device'
     if table_sf is not None:

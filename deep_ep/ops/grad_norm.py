@@ -55,9 +55,9 @@ def grad_norm(grads: Sequence[torch.Tensor], group: Optional[dist.ProcessGroup] 
     Tensors are dense (contiguous, or a permutation of it). With `group` the squares of `grads` are added over its ranks,
     a collective call even for a rank whose list is empty (give it a tensor in `replicated`, or an empty tensor, so that the
     device is known); `replicated` is counted once. NaN or infinity in a gradient shows in the norm."""
+    if group is None and len(replicated) == 0 and not isinstance(grads, torch.Tensor) and len(grads) > 0 and grads[0].is_cuda:
+        return _C.grad_norm(grads)
     tensors, replicated, everything = _checked(grads, replicated)
-    if everything and everything[0].is_cuda and group is None and not replicated:
-        return _C.grad_norm(tensors)
     sums = _total(tensors, replicated, group)
     return _C.grad_norm_finish(sums) if sums.is_cuda else sums.sum().sqrt().float()
 
