@@ -6,6 +6,7 @@
 #include <deep_ep/kernels/embedding.cuh>
 
 #include "api.hpp"
+#include "early_launch.hpp"
 
 namespace deep_ep::launch {
 
@@ -25,9 +26,7 @@ void launch_lookup(EmbLookupArgs a, cudaStream_t stream) {
         piece.num_tokens = std::min(most, total - done);
         piece.idx = static_cast<const uint8_t*>(a.idx) + done * (a.idx64 ? 8 : 4);
         piece.out = static_cast<Out*>(a.out) + done * a.hidden;
-        const auto blocks = static_cast<unsigned>((piece.num_tokens * slices + 7) / 8);
-        embedding_lookup_kernel<In, Out, kElems, kUnroll><<<blocks, 256, 0, stream>>>(piece);
-        CUDA_CHECK(cudaGetLastError());
+        launch_kernel_as({(piece.num_tokens * slices + 7) / 8, 256}, embedding_lookup_kernel<In, Out, kElems, kUnroll>, stream, piece);
     }
 }
 
@@ -85,15 +84,7 @@ void sort_in_cluster(const EmbSortArgs& args, cudaStream_t stream) {
     int cluster = 1;
     while (cluster * kKeys < args.num_tokens) cluster *= 2;
     const int smem = 4 * kKeys * 4 + 3 * bins * 4 + (kEmbClusterThreads / 32) * bins * 2;
-    CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_cluster_kernel<kRounds>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(cluster), config.blockDim = dim3(kEmbClusterThreads);
-    config.dynamicSmemBytes = smem, config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    config.attrs = attr, config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, embedding_sort_cluster_kernel<kRounds>, args));
+    launch_kernel_as({cluster, kEmbClusterThreads, smem, cluster, args.touched == nullptr}, embedding_sort_cluster_kernel<kRounds>, stream, args);
 }
 
 }  // namespace
@@ -108,8 +99,8 @@ void embedding_sort(EmbSortArgs args, int* workspace, const int** ids, const int
     if (args.touched != nullptr) CUDA_CHECK(cudaMemsetAsync(args.touched, 0, (args.num_rows + 31ll) / 32 * 4, stream));
     if (n <= kEmbRankKeys) {
         args.keys[0] = workspace, args.vals[0] = workspace + n;
-        embedding_rank_kernel<<<math::ceil_div(n, 32), kEmbRankThreads, math::align(n, 32) * 4, stream>>>(args);
-        CUDA_CHECK(cudaGetLastError());
+        // (after a memset there is no kernel to begin beside)
+        launch_kernel_as({math::ceil_div(n, 32), kEmbRankThreads, math::align(n, 32) * 4, 1, args.touched == nullptr}, embedding_rank_kernel, stream, args);
         *ids = args.keys[0], *order = args.vals[0];
         return;
     }
@@ -150,23 +141,13 @@ int embedding_grad_chunk(int num_tokens, int hidden) {
 
 namespace {
 
-// A launch that may be set up while the kernel before it in the stream still runs; it waits for that one's results itself.
-void launch_early(void (*kernel)(EmbGradArgs), unsigned grid, cudaStream_t stream, const EmbGradArgs& args) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid), config.blockDim = dim3(256), config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attr, config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args));
-}
-
 template <typename In, typename Out, int kElems, int kPacks, bool kAccumulate>
 void launch_grad(const EmbGradArgs& a, cudaStream_t stream) {
     const int64_t slices = math::ceil_div(a.hidden, 32 * kElems * kPacks);
     const int64_t sums = int64_t(a.num_chunks) * slices, fills = a.accumulate ? 0 : a.num_rows;
     EP_HOST_ASSERT(sums < (int64_t(1) << 31));
-    launch_early(embedding_grad_kernel<In, Out, kElems, kPacks, kAccumulate>, static_cast<unsigned>((sums + fills + 7) / 8), stream, a);
-    if (a.num_chunks > 1) launch_early(embedding_grad_join_kernel<Out, kElems, kAccumulate>, 148 * 6, stream, a);
+    launch_kernel_as({(sums + fills + 7) / 8, 256}, embedding_grad_kernel<In, Out, kElems, kPacks, kAccumulate>, stream, a);
+    if (a.num_chunks > 1) launch_kernel_as({148 * 6, 256}, embedding_grad_join_kernel<Out, kElems, kAccumulate>, stream, a);
 }
 
 template <typename In, typename Out>

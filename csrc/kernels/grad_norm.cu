@@ -6,6 +6,7 @@
 #include <deep_ep/kernels/grad_norm.cuh>
 
 #include "api.hpp"
+#include "early_launch.hpp"
 
 namespace deep_ep::launch {
 
@@ -36,23 +37,11 @@ int fill_table(GradTable<kTensors>& table, const GradTensor* tensors, int count)
     return chunks;
 }
 
-// A launch that may begin while the one before it in the stream still runs: the kernel waits for it where it needs its results.
-template <typename... Params, typename... Args>
-void launch_early(void (*kernel)(Params...), int grid, cudaStream_t stream, const Args&... args) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid), config.blockDim = dim3(kGradThreads), config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attr, config.numAttrs = 1;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
-}
-
 template <int kTensors>
 int square_sum(const GradTensor* tensors, int count, double* partial, cudaStream_t stream) {
     GradTable<kTensors> table;
     const int grid = std::min(fill_table(table, tensors, count), kGradCtas);
-    grad_square_sum_kernel<kTensors><<<grid, kGradThreads, 0, stream>>>(table, GradNormArgs{partial});
-    CUDA_CHECK(cudaGetLastError());
+    launch_kernel_as({grid, kGradThreads}, grad_square_sum_kernel<kTensors>, stream, table, GradNormArgs{partial});
     return grid;
 }
 
@@ -60,7 +49,7 @@ template <int kTensors>
 void clip(const GradTensor* tensors, int count, const GradClipArgs& args, cudaStream_t stream) {
     GradTable<kTensors> table;
     const int grid = std::min(fill_table(table, tensors, count), kGradCtas);
-    launch_early(grad_clip_kernel<kTensors>, grid, stream, table, args);
+    launch_kernel_as({grid, kGradThreads}, grad_clip_kernel<kTensors>, stream, table, args);
 }
 
 }  // namespace
@@ -76,7 +65,7 @@ int grad_square_sums(const std::vector<GradTensor>& tensors, double* partial, cu
     return sums;
 }
 
-void grad_norm_finish(const GradClipArgs& args, cudaStream_t stream) { launch_early(grad_norm_finish_kernel, 1, stream, args); }
+void grad_norm_finish(const GradClipArgs& args, cudaStream_t stream) { launch_kernel_as({1, kGradThreads}, grad_norm_finish_kernel, stream, args); }
 
 void grad_clip(const std::vector<GradTensor>& tensors, GradClipArgs args, cudaStream_t stream) {
     for (size_t i = 0; i < tensors.size(); i += kGradMaxTensors) {

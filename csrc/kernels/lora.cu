@@ -5,6 +5,7 @@
 #include <deep_ep/kernels/lora.cuh>
 
 #include "api.hpp"
+#include "early_launch.hpp"
 #include "gemm_host.hpp"
 
 namespace deep_ep::launch {
@@ -30,30 +31,6 @@ int choose_cluster(int64_t units, int blocks, int least, int sms) {
     return cluster;
 }
 
-// `early`: may begin while the kernel before it in the stream still runs (it waits for that kernel's results itself).
-template <typename... Params, typename... Args>
-void launch_clusters(void (*kernel)(Params...), int64_t grid, int threads, int cluster, int64_t smem, bool early, cudaStream_t stream, const Args&... args) {
-    EP_HOST_ASSERT_MSG(grid < (int64_t(1) << 31), "too many tiles for one launch");
-    CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(grid)), config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = static_cast<size_t>(smem), config.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int count = 0;
-    if (cluster > 1) {
-        attr[count].id = cudaLaunchAttributeClusterDimension;
-        attr[count].val.clusterDim.x = cluster, attr[count].val.clusterDim.y = attr[count].val.clusterDim.z = 1;
-        ++count;
-    }
-    if (early) {
-        attr[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[count].val.programmaticStreamSerializationAllowed = 1;
-        ++count;
-    }
-    config.attrs = attr, config.numAttrs = count;
-    CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
-}
-
 constexpr int64_t kRingBytes = 192 * 1024;
 // Up to this many products of x A^T, the kernel without tensor cores is ahead: its time is that of reading rows * rank * k
 // elements of A from L2, the other's starts at what setting up a tile costs.
@@ -72,8 +49,7 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
         // (an SM divides its memory between cache and shared memory by the kernels on it: with the default, the next kernel's
         // CTAs, which need all of the latter, could not join before these have left)
         CUDA_CHECK(cudaFuncSetAttribute(lora_shrink_rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        lora_shrink_rows_kernel<<<rows * (rank / 4), 512, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), args);
-        CUDA_CHECK(cudaGetLastError());
+        launch_kernel_as({rows * int64_t(rank / 4), 512}, lora_shrink_rows_kernel, stream, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), args);
         return;
     }
     const int rp = math::align(rank, args.mn_major ? 64 : 16);
@@ -91,7 +67,7 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
     const CUtensorMap map_x = make_map_2d(x, rows, args.k, kLoraBlockK, kLoraTileRows);
     const CUtensorMap map_a = args.mn_major ? make_map_3d(a, args.rows.num_adapters, args.k, rank, 64, 64)
                                             : make_map_3d(a, args.rows.num_adapters, rank, args.k, kLoraBlockK, rp);
-    launch_clusters(lora_shrink_kernel, tiles * args.num_chunks * args.cluster, 192, args.cluster, smem, false, stream, map_x, map_a, args);
+    launch_kernel_as({tiles * args.num_chunks * args.cluster, 192, smem, args.cluster}, lora_shrink_kernel, stream, map_x, map_a, args);
 }
 
 namespace {
@@ -116,7 +92,7 @@ void launch_gemm(LoraGemmArgs args, const void* x, const void* w, int sms, cudaS
     args.cluster = choose_cluster(tiles, math::ceil_div(args.k, kLoraBlockK), 4, sms);
     const int64_t grid = args.cluster > 1 ? tiles * args.cluster : std::min<int64_t>(tiles, sms);
     const auto maps = gemm_maps(args, x, w);
-    launch_clusters(lora_gemm_kernel, grid, 320, args.cluster, kLoraGemmSmemBytes, true, stream, maps.x, maps.w, maps.v, maps.y, args);
+    launch_kernel_as({grid, 320, kLoraGemmSmemBytes, args.cluster}, lora_gemm_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
 }
 
 void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, cudaStream_t stream) {
@@ -124,7 +100,7 @@ void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, 
     const int64_t tiles = int64_t(args.m_tiles) * args.n_tiles;
     EP_HOST_ASSERT_MSG(tiles < (int64_t(1) << 30), "too many tiles for one launch");
     const auto maps = gemm_maps(args, x, w);
-    launch_clusters(lora_gemm_pair_kernel, 2 * std::min<int64_t>(tiles, sms / 2), 320, 2, kLoraPairSmemBytes, true, stream, maps.x, maps.w, maps.v, maps.y, args);
+    launch_kernel_as({2 * std::min<int64_t>(tiles, sms / 2), 320, kLoraPairSmemBytes, 2}, lora_gemm_pair_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
 }
 
 // Few rows: columns per tile and CTAs per cluster by an estimate of the time. W comes from memory at 6.5 TB/s however it is
@@ -156,7 +132,7 @@ bool launch_gemm_few(const LoraGemmArgs& g, const void* x, const void* w, int sm
     args.num_stages = static_cast<int>(std::min<int64_t>(32, budget / stage));
     const CUtensorMap map_x = make_map_2d(x, g.rows.num_rows, g.k, kLoraBlockK, args.x_box_rows);
     const CUtensorMap map_w = g.mn_major ? make_map_2d(w, g.k, g.n, 64, kLoraBlockK) : make_map_2d(w, g.n, g.k, kLoraBlockK, args.block_n);
-    launch_clusters(lora_gemm_few_kernel, tiles * args.cluster, 320, args.cluster, args.num_stages * stage + part_bytes + 1024, true, stream, map_x, map_w, args);
+    launch_kernel_as({tiles * args.cluster, 320, args.num_stages * stage + part_bytes + 1024, args.cluster}, lora_gemm_few_kernel, stream, map_x, map_w, args);
     return true;
 }
 
@@ -189,7 +165,7 @@ void lora_wgrad(LoraWgradArgs args, const void* x, cudaStream_t stream) {
     const int64_t part = int64_t(kLoraWgradColumns) * (math::align(args.rows.rank, 16) + 4) * 4;                      // overlays the ring
     const int64_t smem = std::max<int64_t>(int64_t(args.num_stages) * args.stage_bytes, part) + 1024;
     const CUtensorMap map_x = make_map_2d(x, args.rows.num_rows, args.m, 64, kLoraBlockK);
-    launch_clusters(lora_wgrad_kernel, int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 320, args.cluster, smem, false, stream, map_x, args);
+    launch_kernel_as({int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 320, smem, args.cluster, false}, lora_wgrad_kernel, stream, map_x, args);
 }
 
 }  // namespace deep_ep::launch

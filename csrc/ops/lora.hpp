@@ -32,11 +32,10 @@ inline kernels::LoraRows adapter_rows(const torch::Tensor& idx, const torch::Ten
     return {idx.data_ptr(), idx.scalar_type() == torch::kInt64, static_cast<int>(idx.size(0)), static_cast<int>(num_adapters), static_cast<int>(rank), nullptr};
 }
 
-// (t fp32 [rows, rank] = scaling[e] * x . A_e^T, presence uint8 [row tiles, adapters] or nothing). `transposed`: A is [adapters, k, rank].
-inline std::tuple<torch::Tensor, std::optional<torch::Tensor>> lora_shrink(const torch::Tensor& x_in, const torch::Tensor& a_in, const torch::Tensor& idx,
-                                                                           const torch::Tensor& scaling_in, bool transposed, bool with_presence) {
-    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
-    const auto x = operand(x_in, 2, x_in), a = operand(a_in, 3, x_in), scaling = operand(scaling_in, 1, x_in, torch::kFloat32);
+// t fp32 [rows, rank] = scaling[e] * x . A_e^T, and presence uint8 [row tiles, adapters] where it is wanted. `transposed`: A is
+// [adapters, k, rank]. Operands as `operand` leaves them.
+inline torch::Tensor lora_shrink(const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& idx, const torch::Tensor& scaling, bool transposed,
+                                 const std::optional<torch::Tensor>& presence) {
     const int64_t k = x.size(1), rank = transposed ? a.size(2) : a.size(1);
     EP_HOST_ASSERT_MSG((transposed ? a.size(1) : a.size(2)) == k and k >= 8 and k % 8 == 0, "contraction lengths agree and are multiples of 8");
     EP_HOST_ASSERT_MSG(scaling.size(0) == a.size(0), "one scaling per adapter");
@@ -44,24 +43,17 @@ inline std::tuple<torch::Tensor, std::optional<torch::Tensor>> lora_shrink(const
     args.rows = adapter_rows(idx, x, a.size(0), rank);
     args.k = static_cast<int>(k), args.mn_major = transposed, args.scaling = scaling.data_ptr<float>();
     auto t = torch::empty({x.size(0), rank}, x.options().dtype(torch::kFloat32));
-    args.t = t.data_ptr<float>();
-    std::optional<torch::Tensor> presence;
-    if (with_presence) {
-        presence = torch::empty({(x.size(0) + kernels::kLoraTileRows - 1) / kernels::kLoraTileRows, a.size(0)}, x.options().dtype(torch::kUInt8));
-        args.presence = presence->data_ptr<uint8_t>();
-    }
+    args.t = t.data_ptr<float>(), args.presence = presence.has_value() ? presence->data_ptr<uint8_t>() : nullptr;
     if (x.size(0) > 0) launch::lora_shrink(args, x.data_ptr(), a.data_ptr(), c10::cuda::getCurrentCUDAStream());
-    return {t, presence};
+    return t;
 }
 
-// y = x . W^T + t . V_e^T; `transposed`: W is [k, n] and V [adapters, rank, n] (the data gradient), else [n, k] and [adapters, n, rank]
-inline torch::Tensor lora_gemm(const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& t_in, const torch::Tensor& v_in,
-                               const torch::Tensor& idx, bool transposed) {
-    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
-    const auto x = operand(x_in, 2, x_in), w = operand(w_in, 2, x_in), t = operand(t_in, 2, x_in, torch::kFloat32), v = operand(v_in, 3, x_in);
+// y = x . W^T + t . V_e^T; `transposed`: W is [k, n] and V [adapters, rank, n] (the data gradient), else [n, k] and [adapters, n, rank].
+// Its kernel begins beside the one before it in the stream and waits for nothing but t: that one has to be `lora_shrink`'s,
+// with no other launch (a copy of an operand, say) in between.
+inline torch::Tensor lora_gemm_after_shrink(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& t, const torch::Tensor& v,
+                                            const torch::Tensor& idx, bool transposed) {
     const int64_t k = x.size(1), n = transposed ? w.size(1) : w.size(0), rank = t.size(1);
-    EP_HOST_ASSERT_MSG((transposed ? w.size(0) : w.size(1)) == k and k >= 8 and k % 8 == 0 and n >= 8 and n % 8 == 0, "dimensions agree and are multiples of 8");
-    EP_HOST_ASSERT_MSG(t.size(0) == x.size(0) and (transposed ? v.size(1) : v.size(2)) == rank and (transposed ? v.size(2) : v.size(1)) == n, "adapter shapes agree");
     kernels::LoraGemmArgs args = {};
     args.rows = adapter_rows(idx, x, v.size(0), rank);
     args.k = static_cast<int>(k), args.n = static_cast<int>(n), args.mn_major = transposed;
@@ -71,12 +63,37 @@ inline torch::Tensor lora_gemm(const torch::Tensor& x_in, const torch::Tensor& w
     return y;
 }
 
-// (y, t): both steps of the forward pass
-inline std::tuple<torch::Tensor, torch::Tensor> lora_forward(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& a, const torch::Tensor& b,
-                                                             const torch::Tensor& idx, const torch::Tensor& scaling) {
-    EP_HOST_ASSERT_MSG(a.dim() == 3 and b.dim() == 3 and a.size(0) == b.size(0), "as many A as B");
-    const auto t = std::get<0>(lora_shrink(x, a, idx, scaling, false, false));
-    return {lora_gemm(x, w, t, b, idx, false), t};
+inline void check_adapters(const torch::Tensor& w, const torch::Tensor& a, const torch::Tensor& b) {
+    const int64_t n = w.size(0), k = w.size(1);
+    EP_HOST_ASSERT_MSG(k >= 8 and k % 8 == 0 and n >= 8 and n % 8 == 0, "K and N are multiples of 8");
+    EP_HOST_ASSERT_MSG(a.size(0) == b.size(0) and a.size(2) == k and b.size(1) == n and b.size(2) == a.size(1),
+                       "w [N, K], a [adapters, rank, K], b [adapters, N, rank]");
+}
+
+// (y, t) of the forward pass
+inline std::tuple<torch::Tensor, torch::Tensor> lora_forward(const torch::Tensor& x_in, const torch::Tensor& w_in, const torch::Tensor& a_in,
+                                                             const torch::Tensor& b_in, const torch::Tensor& idx, const torch::Tensor& scaling_in) {
+    const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
+    const auto x = operand(x_in, 2, x_in), w = operand(w_in, 2, x_in), a = operand(a_in, 3, x_in), b = operand(b_in, 3, x_in);
+    const auto scaling = operand(scaling_in, 1, x_in, torch::kFloat32);
+    check_adapters(w, a, b);
+    const auto t = lora_shrink(x, a, idx, scaling, false, std::nullopt);
+    return {lora_gemm_after_shrink(x, w, t, b, idx, false), t};
+}
+
+// (dt, presence, dx or nothing) of the backward pass
+inline std::tuple<torch::Tensor, torch::Tensor, std::optional<torch::Tensor>> lora_backward(
+        const torch::Tensor& dy_in, const torch::Tensor& w_in, const torch::Tensor& a_in, const torch::Tensor& b_in, const torch::Tensor& idx,
+        const torch::Tensor& scaling_in, bool want_dx) {
+    const c10::cuda::OptionalCUDAGuard guard(dy_in.is_cuda() ? std::optional(dy_in.device()) : std::nullopt);
+    const auto dy = operand(dy_in, 2, dy_in), w = operand(w_in, 2, dy_in), a = operand(a_in, 3, dy_in), b = operand(b_in, 3, dy_in);
+    const auto scaling = operand(scaling_in, 1, dy_in, torch::kFloat32);
+    check_adapters(w, a, b);
+    auto presence = torch::empty({(dy.size(0) + kernels::kLoraTileRows - 1) / kernels::kLoraTileRows, b.size(0)}, dy.options().dtype(torch::kUInt8));
+    const auto dt = lora_shrink(dy, b, idx, scaling, true, presence);
+    std::optional<torch::Tensor> dx;
+    if (want_dx) dx = lora_gemm_after_shrink(dy, w, dt, a, idx, true);
+    return {dt, presence, dx};
 }
 
 // out[e] (+)= sum over the rows of adapter e of t[row]^T x[row]: [adapters, rank, m] (`rank_major`) or [adapters, m, rank]
@@ -106,10 +123,9 @@ inline void lora_wgrad(const torch::Tensor& x_in, const torch::Tensor& t_in, con
 
 inline void register_lora(pybind11::module_& m) {
     namespace py = pybind11;
-    m.def("lora_shrink", &lora_shrink, py::arg("x"), py::arg("a"), py::arg("idx"), py::arg("scaling"), py::arg("transposed") = false,
-          py::arg("with_presence") = false);
-    m.def("lora_gemm", &lora_gemm, py::arg("x"), py::arg("w"), py::arg("t"), py::arg("v"), py::arg("idx"), py::arg("transposed") = false);
     m.def("lora_forward", &lora_forward, py::arg("x"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling"));
+    m.def("lora_backward", &lora_backward, py::arg("dy"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling"),
+          py::arg("want_dx") = true);
     m.def("lora_wgrad", &lora_wgrad, py::arg("x"), py::arg("t"), py::arg("idx"), py::arg("presence"), py::arg("out"), py::arg("rank_major"),
           py::arg("accumulate") = false);
 }

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const __grid_cons
     const unsigned packs = unsigned(a.hidden) / kElems, slices = math::ceil_div(packs, 32u * kUnroll);
     const unsigned item = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const unsigned token = item / slices, slice = item - token * slices;
+    cudaGridDependencySynchronize();
     if (token >= a.num_tokens) return;
     const int64_t id = load_id(a.idx, a.idx64, token);
     const bool valid = static_cast<uint64_t>(id) < static_cast<uint64_t>(a.num_rows);
@@ -285,6 +286,7 @@ __global__ void __launch_bounds__(kEmbRankThreads) embedding_rank_kernel(const _
     __shared__ int counts[32];
     constexpr int kWarps = kEmbRankThreads / 32;
     const int lane = ptx::lane_id(), warp = threadIdx.x / 32, n = a.num_tokens, padded = math::align(n, 32);
+    cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();         // the kernel of the sums may be set up meanwhile
     if (blockIdx.x == 0 and threadIdx.x == 0) *a.num_crossing = 0;
     if (threadIdx.x < 32) counts[threadIdx.x] = 0;
@@ -334,6 +336,7 @@ __global__ void __launch_bounds__(kEmbClusterThreads, 1) embedding_sort_cluster_
     uint16_t* mine = counters + warp * bins;
     const int count = min(max(a.num_tokens - rank * kKeys, 0), kKeys);                          // this CTA's keys
 
+    cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();                  // the kernel of the sums may be set up meanwhile
     if (rank == 0 and threadIdx.x == 0) *a.num_crossing = 0;
     int key[kRounds], val[kRounds];

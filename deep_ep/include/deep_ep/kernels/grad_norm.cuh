@@ -206,6 +206,7 @@ EP_DEVICE float clip_factor(float norm, float max_norm) {
 template <int kTensors>
 __global__ void __launch_bounds__(kGradThreads, kGradCtasPerSm) grad_square_sum_kernel(const __grid_constant__ GradTable<kTensors> t, GradNormArgs a) {
     using namespace grad_detail;
+    cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
     const int chunks = t.first_chunk[t.num_tensors];
     double acc = 0.0;

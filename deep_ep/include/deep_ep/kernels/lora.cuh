@@ -314,7 +314,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     __shared__ int list[16], list_size;
     __shared__ volatile int error_flag;
 
-    cudaTriggerProgrammaticLaunchCompletion();
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = blockIdx.x % cluster;
     // (first chunks first: the later ones of most tiles are empty)
@@ -333,6 +332,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         error_flag = 0;
         tc::prefetch_tensormap(&map_x), tc::prefetch_tensormap(&map_a);
     }
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     if (warp == 0) {
         // this chunk's adapters
         TileAdapters<kLoraTileRows> rows;
@@ -482,6 +483,7 @@ lora_shrink_rows_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16
     using namespace lora_detail;
     constexpr int kColumns = 4, kThreads = 512;
     __shared__ float sums[kThreads / 32][kColumns];
+    cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
     const int groups = a.rows.rank / kColumns, row = blockIdx.x / groups, r0 = blockIdx.x % groups * kColumns;
     const int warp = threadIdx.x / 32, lane = ptx::lane_id();

@@ -50,9 +50,7 @@ class _LoraLinear(torch.autograd.Function):
         dx = dw = da = db = None
         want_x, want_w, want_a, want_b = ctx.needs_input_grad[:4]
         if want_x or want_a or want_b:
-            dt, presence = _C.lora_shrink(dy, lora_b, idx, scaling, transposed=True, with_presence=True)
-        if want_x:
-            dx = _C.lora_gemm(dy, w, dt, lora_a, idx, transposed=True)
+            dt, presence, dx = _C.lora_backward(dy, w, lora_a, lora_b, idx, scaling, want_x)
         if want_a:
             da = _weight_grad(x, dt, idx, presence, lora_a, True)
         if want_b:
