@@ -2,13 +2,13 @@
 //
 // Mathematics: norm = sqrt(sum of g^2 over all tensors), factor = min(1, max_norm / (norm + 1e-6)), g *= factor. Two sweeps
 // because the factor needs every element first; both are bound by HBM. The first reads everything once; the second reads
-// and writes everything, and when the factor is 1 in place it touches nothing. It walks the chunks from the end, so
+// and writes everything, and when the factor is 1 in place it touches nothing. It walks from the end to the beginning, so
 // that what the first sweep read last is still in L2 (126 MB).
 //
 // Sums: the squares of 64 bytes of elements are added in fp32 (at most ten roundings on the way of each), everything above
 // that in fp64, whose units would otherwise be the bound for 16-bit gradients. Squares that leave fp32's range (an element
 // beyond about 1e18, or all of them below 1e-14) are taken in fp64 instead, so neither huge nor tiny
-// gradients lose the norm. Each CTA takes a fixed set of chunks and its sum has a fixed slot: the same bits every time.
+// gradients lose the norm. Each CTA takes a fixed range of chunks and its sum has a fixed slot: the same bits every time.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -79,15 +79,17 @@ __device__ __noinline__ double sum_range(const T* p, int n) {
     double acc = 0.0;
     const int head = min(n, int((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / int(sizeof(T)));
     const int packs = (n - head) / Unpacked<T>::kCount, tail = head + packs * Unpacked<T>::kCount;
-    if (int(threadIdx.x) < head) acc += square(p[threadIdx.x]);
-    if (int(threadIdx.x) < n - tail) acc += square(p[tail + threadIdx.x]);
+    const int ends = head + n - tail, end = int(threadIdx.x) < head ? int(threadIdx.x) : tail + int(threadIdx.x) - head;     // what no pack holds
+    if (int(threadIdx.x) < ends) acc += square(p[end]);
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     constexpr int kAhead = 4;
-    int i = threadIdx.x;
-    for (; i + (kAhead - 1) * kGradThreads < packs; i += kAhead * kGradThreads) {
+    for (int i = threadIdx.x; i < packs; i += kAhead * kGradThreads) {
         uint4 e[kAhead];
         #pragma unroll
-        for (int u = 0; u < kAhead; ++u) e[u] = __ldg(body + i + u * kGradThreads);
+        for (int u = 0; u < kAhead; ++u) e[u] = __ldg(body + min(i + u * kGradThreads, packs - 1));     // (see scale_range)
+        #pragma unroll
+        for (int u = 1; u < kAhead; ++u)
+            if (i + u * kGradThreads >= packs) e[u] = make_uint4(0, 0, 0, 0);
         const float s = (square_sum<T>(e[0]) + square_sum<T>(e[1])) + (square_sum<T>(e[2]) + square_sum<T>(e[3]));
         if (s > 1e-28f and s < 1e36f) {
             acc += double(s);
@@ -96,77 +98,97 @@ __device__ __noinline__ double sum_range(const T* p, int n) {
             for (int u = 0; u < kAhead; ++u) acc += square_sum_exact<T>(u == 0 ? e[0] : u == 1 ? e[1] : u == 2 ? e[2] : e[3]);
         }
     }
-    for (; i < packs; i += kGradThreads) acc += square_sum_exact<T>(__ldg(body + i));
     return acc;
 }
 
-// Eight elements
-template <typename T>
-struct Eight {
-    static constexpr int kUnits = 8 * sizeof(T) / 16;
-    uint4 unit[kUnits];
-};
+// `kBytes` of a tensor
+template <int kBytes>
+using Unit = std::conditional_t<kBytes == 16, uint4, uint2>;
 
+// As many elements as 16 bytes of the wider type hold, so that both sides move in accesses without gaps between the lanes
 template <typename In, typename Out>
-EP_DEVICE Eight<Out> scaled(const Eight<In>& in, float factor) {
-    float v[8];
+constexpr int kScaled = 16 / int(sizeof(In) > sizeof(Out) ? sizeof(In) : sizeof(Out));
+
+template <typename T, int kCount>
+EP_DEVICE void to_floats(const Unit<kCount * int(sizeof(T))>& raw, float (&v)[kCount]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
     #pragma unroll
-    for (int u = 0; u < Eight<In>::kUnits; ++u) {
-        const Unpacked<In> e(in.unit[u]);
-        #pragma unroll
-        for (int j = 0; j < Unpacked<In>::kCount; ++j) v[u * Unpacked<In>::kCount + j] = e.v[j] * factor;
+    for (int i = 0; i < kCount; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else v[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu)));
     }
-    Eight<Out> out;
-    uint32_t w[4 * Eight<Out>::kUnits];
+}
+template <typename T, int kCount>
+EP_DEVICE Unit<kCount * int(sizeof(T))> from_floats(const float (&v)[kCount]) {
+    Unit<kCount * int(sizeof(T))> raw;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
     #pragma unroll
-    for (int j = 0; j < 4 * Eight<Out>::kUnits; ++j) {
-        if constexpr (sizeof(Out) == 4) {
-            w[j] = __float_as_uint(v[j]);
-        } else if constexpr (std::is_same_v<Out, __nv_bfloat16>) {
-            w[j] = ptx::float2_to_bf16x2(v[2 * j], v[2 * j + 1]);
+    for (int i = 0; i < kCount; i += sizeof(T) == 4 ? 1 : 2) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(v[i]);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            w[i / 2] = ptx::float2_to_bf16x2(v[i], v[i + 1]);
         } else {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+            w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
-    #pragma unroll
-    for (int u = 0; u < Eight<Out>::kUnits; ++u) out.unit[u] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-    return out;
+    return raw;
 }
 
 template <typename In, typename Out>
 __device__ __noinline__ void scale_range(const In* p, Out* q, int n, float factor) {
-    // first element from which both sides lie on 16-byte boundaries; none: element by element
-    int head = 0;
-    while (head < 8 and (((reinterpret_cast<uintptr_t>(p) + head * sizeof(In)) | (reinterpret_cast<uintptr_t>(q) + head * sizeof(Out))) & 15)) ++head;
-    if (head == 8) {
+    constexpr int kCount = kScaled<In, Out>, kInBytes = kCount * int(sizeof(In)), kOutBytes = kCount * int(sizeof(Out));
+    // First element from which both sides lie on the boundaries of their accesses, the written one on a sector of 32 bytes if
+    // there is such an element (tensors of a bucket begin anywhere); none: element by element.
+    const auto first = [&](int out_bytes, int most) {
+        int h = 0;
+        while (h < most and ((reinterpret_cast<uintptr_t>(p + h) % kInBytes) | (reinterpret_cast<uintptr_t>(q + h) % out_bytes))) ++h;
+        return h;
+    };
+    constexpr int kSector = 32 / int(sizeof(Out));
+    int head = first(32, kSector);
+    if (head == kSector) head = first(kOutBytes, kCount);
+    if (head == kCount and first(kOutBytes, kCount) == kCount) {
         for (int i = threadIdx.x; i < n; i += kGradThreads) q[i] = from_float<Out>(to_float(p[i]) * factor);
         return;
     }
     head = min(head, n);
-    const int eights = (n - head) / 8, tail = head + eights * 8;
-    if (int(threadIdx.x) < head) q[threadIdx.x] = from_float<Out>(to_float(p[threadIdx.x]) * factor);
-    if (int(threadIdx.x) < n - tail) q[tail + threadIdx.x] = from_float<Out>(to_float(p[tail + threadIdx.x]) * factor);
-    const uint4* src = reinterpret_cast<const uint4*>(p + head);
-    uint4* dst = reinterpret_cast<uint4*>(q + head);
-    constexpr int kAhead = 4 / Eight<In>::kUnits;             // 64 bytes a thread in flight
-    int i = threadIdx.x;
-    for (; i < eights; i += kAhead * kGradThreads) {
-        Eight<In> e[kAhead];
+    const int units = (n - head) / kCount, tail = head + units * kCount;
+    const auto* src = reinterpret_cast<const Unit<kInBytes>*>(p + head);
+    auto* dst = reinterpret_cast<Unit<kOutBytes>*>(q + head);
+    const auto scaled = [&](const Unit<kInBytes>& raw) {
+        float v[kCount];
+        to_floats<In, kCount>(raw, v);
         #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            #pragma unroll
-            for (int w = 0; w < Eight<In>::kUnits; ++w)
-                if (i + u * kGradThreads < eights) e[u].unit[w] = src[(i + u * kGradThreads) * Eight<In>::kUnits + w];
-        }
+        for (int j = 0; j < kCount; ++j) v[j] *= factor;
+        return from_floats<Out, kCount>(v);
+    };
+    // Eight loads, then eight stores, without conditions in between: with them the loads were not in flight together (in place,
+    // fp32: 4.4 TB/s against 6.4). What eight do not fill comes first (its loads repeat the last unit beyond the end, for
+    // nothing), then from the end to the beginning: what the sum has read last is still in L2.
+    constexpr int kAhead = 8, kStep = kAhead * kGradThreads;
+    const int whole = units / kStep * kStep;
+    if (whole < units) {
+        const int i = whole + int(threadIdx.x);
+        Unit<kInBytes> raw[kAhead];
         #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (i + u * kGradThreads >= eights) break;
-            const Eight<Out> o = scaled<In, Out>(e[u], factor);
-            #pragma unroll
-            for (int w = 0; w < Eight<Out>::kUnits; ++w) dst[(i + u * kGradThreads) * Eight<Out>::kUnits + w] = o.unit[w];
-        }
+        for (int u = 0; u < kAhead; ++u) raw[u] = src[min(i + u * kGradThreads, units - 1)];
+        #pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i + u * kGradThreads < units) dst[i + u * kGradThreads] = scaled(raw[u]);
     }
+    for (int i = whole - kStep + int(threadIdx.x); i >= 0; i -= kStep) {
+        Unit<kInBytes> raw[kAhead];
+        #pragma unroll
+        for (int u = 0; u < kAhead; ++u) raw[u] = src[i + u * kGradThreads];
+        #pragma unroll
+        for (int u = 0; u < kAhead; ++u) dst[i + u * kGradThreads] = scaled(raw[u]);
+    }
+    // what no unit holds
+    const int ends = head + n - tail, end = int(threadIdx.x) < head ? int(threadIdx.x) : tail + int(threadIdx.x) - head;
+    if (int(threadIdx.x) < ends) q[end] = from_float<Out>(to_float(p[end]) * factor);
 }
 
 // Sum over the CTA in a fixed order; valid in every thread
@@ -196,6 +218,9 @@ EP_DEVICE int tensor_of(const GradTable<kTensors>& t, int chunk) {
     return lo;
 }
 
+// first chunk of a CTA's share
+EP_DEVICE int share_begin(int chunks, unsigned cta, unsigned ctas) { return static_cast<int>(int64_t(chunks) * cta / ctas); }
+
 EP_DEVICE float clip_factor(float norm, float max_norm) {
     const float f = max_norm / (norm + 1e-6f);
     return f > 1.0f ? 1.0f : f;               // NaN stays NaN
@@ -210,15 +235,18 @@ __global__ void __launch_bounds__(kGradThreads, kGradCtasPerSm) grad_square_sum_
     cudaTriggerProgrammaticLaunchCompletion();
     const int chunks = t.first_chunk[t.num_tensors];
     double acc = 0.0;
-    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int i = tensor_of(t, chunk);
+    // a CTA takes consecutive chunks, as long pieces of as few tensors as they lie in
+    const int first = share_begin(chunks, blockIdx.x, gridDim.x), last = share_begin(chunks, blockIdx.x + 1, gridDim.x);
+    for (int chunk = first; chunk < last; ) {
+        const int i = tensor_of(t, chunk), until = min(last, t.first_chunk[i + 1]);
         const int64_t begin = int64_t(chunk - t.first_chunk[i]) * kGradChunk;
-        const int n = int(min(int64_t(kGradChunk), t.numel[i] - begin));
+        const int n = int(min(int64_t(until - chunk) * kGradChunk, t.numel[i] - begin));
         switch (static_cast<GradType>(t.in_type[i])) {
             case GradType::kBF16: acc += sum_range(static_cast<const __nv_bfloat16*>(t.in[i]) + begin, n); break;
             case GradType::kFP16: acc += sum_range(static_cast<const __half*>(t.in[i]) + begin, n); break;
             case GradType::kFP32: acc += sum_range(static_cast<const float*>(t.in[i]) + begin, n); break;
         }
+        chunk = until;
     }
     const double sum = block_sum(acc);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
@@ -247,11 +275,12 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_clip_kernel(const __grid
     const float factor = clip_factor(norm, a.max_norm);
     if (a.in_place and factor == 1.0f) return;
     const int chunks = t.first_chunk[t.num_tensors];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int chunk = chunks - 1 - c;
-        const int i = tensor_of(t, chunk);
+    const int first = share_begin(chunks, blockIdx.x, gridDim.x), last = share_begin(chunks, blockIdx.x + 1, gridDim.x);
+    for (int until = last; until > first; ) {
+        const int i = tensor_of(t, until - 1), chunk = max(first, t.first_chunk[i]);
         const int64_t begin = int64_t(chunk - t.first_chunk[i]) * kGradChunk;
-        const int n = int(min(int64_t(kGradChunk), t.numel[i] - begin));
+        const int n = int(min(int64_t(until - chunk) * kGradChunk, t.numel[i] - begin));
+        until = chunk;
         const auto to = [&](auto* in) {
             switch (static_cast<GradType>(t.out_type[i])) {
                 case GradType::kBF16: scale_range(in + begin, static_cast<__nv_bfloat16*>(t.out[i]) + begin, n, factor); break;

@@ -9,7 +9,7 @@ enum class GradType : int { kBF16 = 0, kFP16 = 1, kFP32 = 2 };
 
 constexpr int kGradThreads = 256;
 constexpr int kGradCtasPerSm = 6;             // 1536 threads with 64 bytes in flight each
-constexpr int kGradChunk = 16384;             // elements that one CTA takes at a time
+constexpr int kGradChunk = 16384;             // elements that are not divided among CTAs
 constexpr int kGradCtas = 148 * kGradCtasPerSm;
 constexpr int kGradMaxTensors = 1024;         // tensors of one launch: their table travels in the kernel's parameters
 
