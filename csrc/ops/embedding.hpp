@@ -7,6 +7,7 @@
 
 #include <limits>
 #include <optional>
+#include <utility>
 
 #include <deep_ep/common/exception.hpp>
 
@@ -74,6 +75,13 @@ inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, do
     EP_HOST_ASSERT_MSG(dy.scalar_type() == out.scalar_type() or out.scalar_type() == torch::kFloat32, "out is fp32 or of dy's type");
     EP_HOST_ASSERT_MSG(not accumulate or out.scalar_type() == torch::kFloat32, "only an fp32 gradient is accumulated into");
     EP_HOST_ASSERT_MSG(out.size(0) <= 1 or out.stride(0) >= out.size(1), "rows of out overlap");
+    const auto range = [](const torch::Tensor& t) {
+        const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+        return std::pair(begin, begin + (t.numel() == 0 ? 0 : ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size()));
+    };
+    const auto [dy_begin, dy_end] = range(dy);
+    const auto [out_begin, out_end] = range(out);
+    EP_HOST_ASSERT_MSG(out_end <= dy_begin or dy_end <= out_begin or out_begin == out_end or dy_begin == dy_end, "out shares memory with dy");
     constexpr int64_t kMost = std::numeric_limits<int>::max() / 2;
     EP_HOST_ASSERT_MSG(idx.numel() <= kMost and out.size(0) <= kMost and out.size(1) <= kMost, "sizes above 2^30");
     const auto in_type = embedding_type(dy), out_type = embedding_type(out);

@@ -143,12 +143,13 @@ __global__ void __launch_bounds__(256) embedding_lookup_kernel(const __grid_cons
     const In* row = reinterpret_cast<const In*>(a.table) + (valid ? id : 0) * a.table_stride;
     Pack<In, kElems> in[kUnroll];
     float sf[kUnroll];
-    #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const unsigned p = (slice * kUnroll + u) * 32 + lane;
-        sf[u] = 1.0f;
-        if (valid and p < packs) {
+    if (valid) {
+        // (no condition per load: lanes beyond the row's end repeat its last pack, for nothing)
+        #pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const unsigned p = min((slice * kUnroll + u) * 32 + lane, packs - 1);
             in[u] = load_pack<In, kElems>(row + int64_t(p) * kElems);
+            sf[u] = 1.0f;
             if constexpr (sizeof(In) == 1) sf[u] = __ldg(a.table_sf + id * a.sf_stride + p * kElems / 128);
         }
     }

@@ -55,7 +55,7 @@ def grad_norm(grads: Sequence[torch.Tensor], group: Optional[dist.ProcessGroup] 
     Tensors are dense (contiguous, or a permutation of it). With `group` the squares of `grads` are added over its ranks,
     a collective call even for a rank whose list is empty (give it a tensor in `replicated`, or an empty tensor, so that the
     device is known); `replicated` is counted once. NaN or infinity in a gradient shows in the norm."""
-    if group is None and len(replicated) == 0 and not isinstance(grads, torch.Tensor) and len(grads) > 0 and grads[0].is_cuda:
+    if group is None and isinstance(grads, (list, tuple)) and len(grads) > 0 and grads[0].is_cuda and not replicated:
         return _C.grad_norm(grads)
     tensors, replicated, everything = _checked(grads, replicated)
     sums = _total(tensors, replicated, group)

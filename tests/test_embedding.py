@@ -196,6 +196,23 @@ def test_gradient_of_nothing():
 
 
 @pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    import deep_ep
+    table, ids = torch.randn(8, 128, device='cuda'), torch.tensor([0, 1], device='cuda')
+    flat = torch.randn(1000, device='cuda')
+    for bad in (lambda: embedding_lookup(table, ids.float()), lambda: embedding_lookup(table[0], ids), lambda: embedding_lookup(table.double(), ids),
+                lambda: embedding_lookup(table, ids, table_sf=torch.ones(8, 1, device='cuda')), lambda: embedding_lookup(table.to(torch.float8_e4m3fn), ids),
+                lambda: embedding_lookup(table.to(torch.float8_e4m3fn), ids, table_sf=torch.ones(8, 2, device='cuda')),
+                lambda: embedding_lookup(table, ids.cpu()), lambda: embedding_lookup(table.t(), ids),
+                lambda: embedding_grad(torch.randn(3, 128, device='cuda'), ids, 8), lambda: embedding_grad(torch.randn(2, 128, device='cuda'), ids.cpu(), 8),
+                lambda: embedding_grad(flat[:20].view(2, 10), ids, 8, out=flat[10:90].view(8, 10)),
+                lambda: embedding_grad(flat[:20].view(2, 10), ids, 8, out=flat[100:].as_strided((8, 10), (5, 1))),
+                lambda: embedding_grad(flat[:20].view(2, 10), ids, 8, out=flat[100:180].view(10, 8).t())):
+        with pytest.raises((AssertionError, deep_ep.EPException)):
+            bad()
+
+
+@pytest.mark.gpu
 def test_non_finite_rows_stay_where_they_are():
     table = torch.randn(20, 256, device='cuda')
     table[3], table[4, 5] = float('nan'), float('inf')

@@ -81,6 +81,7 @@ def test_zero_norm_limit_empty_lists_and_scalars(device):
     assert float(grad_norm([])) == 0 and float(clip_grad_norm_([], 1.0)) == 0
     assert float(grad_norm([torch.empty(0, device=device)])) == 0
     g = torch.full((10,), 3.0, device=device)
+    assert abs(float(grad_norm(t for t in (g, g[:5]))) - math.sqrt(135)) < 1e-5 and abs(float(grad_norm(g)) - math.sqrt(90)) < 1e-5
     assert abs(float(clip_grad_norm_(g, 0.0)) - math.sqrt(90)) < 1e-5 and not g.any()
 
 
