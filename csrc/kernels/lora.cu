@@ -49,7 +49,7 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
         // (an SM divides its memory between cache and shared memory by the kernels on it: with the default, the next kernel's
         // CTAs, which need all of the latter, could not join before these have left)
         CUDA_CHECK(cudaFuncSetAttribute(lora_shrink_rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-        launch_kernel_as({rows * int64_t(rank / 4), 512}, lora_shrink_rows_kernel, stream, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), args);
+        launch_kernel_as({rows * int64_t(rank / 4), 256}, lora_shrink_rows_kernel, stream, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a), args);
         return;
     }
     const int rp = math::align(rank, args.mn_major ? 64 : 16);

@@ -476,12 +476,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 // The same for a few rows (decode): one CTA per (row, four rank columns), plain fp32 products. A tile of the kernel above would
 // be mostly empty, and its setup (tensor maps, tensor memory, a cluster) costs more than these products; the adapters are
 // read once per row, from L2. Its time is that of round trips to memory, those for its instructions among them: between two
-// calls a decode step streams more weights than L2 holds, so the code is cold. Hence many threads with a short loop each
-// instead of unrolled ones (which took 8.6 us for one row of 7168, of which 5 went to fetching instructions).
-__global__ void __launch_bounds__(512, 3)
+// calls a decode step streams more weights than L2 holds, so the code is cold. Hence a short loop instead of an unrolled one
+// (which took 8.6 us for one row of 7168, of which 5 went to fetching instructions). Small CTAs: three of them and one of the
+// kernel that reads W fit on an SM together, so that W is under way while these wait.
+__global__ void __launch_bounds__(256, 6)
 lora_shrink_rows_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a_all, const __grid_constant__ LoraShrinkArgs a) {
     using namespace lora_detail;
-    constexpr int kColumns = 4, kThreads = 512;
+    constexpr int kColumns = 4, kThreads = 256;
     __shared__ float sums[kThreads / 32][kColumns];
     cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
@@ -1080,7 +1081,9 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 //   warp 0      TMA producer     warp 1      MMA issuer
 //   warps 2-9   low-rank term; warps 2-5 then send the accumulator's rows to their owners, and all eight add and store
 // One tile per CTA. The wait for the kernel that computes t comes after W is under way.
-__global__ void __launch_bounds__(320, 1)
+// (launched with 320 threads; the bound keeps the registers at 88, beside which three CTAs of lora_shrink_rows_kernel fit in each
+// quarter of an SM: three warps of this kernel and six of that one)
+__global__ void __launch_bounds__(736, 1)
 lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ LoraGemmFewArgs a) {
     using namespace lora_detail;
     extern __shared__ uint8_t smem_raw[];
@@ -1162,64 +1165,79 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         row = rank * share + item / units, c = item % units * 8;
         return item < share * units and m0 + row < a.rows.num_rows and n0 + c < a.n;
     };
-    // low-rank terms of two items at once, in fp32
-    const auto low_rank = [&](int first, float (&v)[2][8]) {
-        const __nv_bfloat16* base[2];
-        const float* t[2];
-        bool there[2];
+    // low-rank term of an item in fp32, four 16-byte units of V at a time (few registers: see lora_shrink_rows_kernel)
+    const auto low_rank = [&](int item, float (&v)[8]) {
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            int row, c;
-            there[i] = place(first + 256 * i, row, c);
-            const int e = there[i] ? adapter_of(a.rows, m0 + row) : -1;
-            there[i] = e >= 0;
-            base[i] = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(max(e, 0)) * a.n * a.rows.rank + (a.mn_major ? n0 + c : int64_t(n0 + c) * a.rows.rank);
-            t[i] = a.t + int64_t(m0 + row) * a.rows.rank;
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        }
-        const int64_t pitch = a.mn_major ? a.n : a.rows.rank;
-        // four 16-byte units of V per item and step. mn_major: eight columns of the rank rows r .. r + 3; else eight rank columns of
-        // four of the columns
-        for (int step = 0; step < a.rows.rank / 4; ++step) {
-            const int r = a.mn_major ? step * 4 : step / 2 * 8, j0 = a.mn_major ? 0 : step % 2 * 4;
-            float f[2][8];
-            uint4 u[2][4];
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (not there[i]) continue;
-                if (a.mn_major) {
-                    const float4 g = *reinterpret_cast<const float4*>(t[i] + r);
-                    f[i][0] = g.x, f[i][1] = g.y, f[i][2] = g.z, f[i][3] = g.w;
-                } else {
-                    load8(t[i] + r, f[i]);
-                }
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        int row, c;
+        if (not place(item, row, c)) return;
+        const int e = adapter_of(a.rows, m0 + row);
+        if (e < 0) return;
+        const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
+        const float* t = a.t + int64_t(m0 + row) * a.rows.rank;
+        if (a.mn_major) {
+            // eight columns of the rank rows r .. r + 3
+            base += n0 + c;
+            #pragma unroll 1
+            for (int r = 0; r < a.rows.rank; r += 4) {
+                const float4 f4 = *reinterpret_cast<const float4*>(t + r);
+                const float f[4] = {f4.x, f4.y, f4.z, f4.w};
+                uint4 u[4];
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) u[i][j] = *reinterpret_cast<const uint4*>(base[i] + (a.mn_major ? (r + j) * pitch : (j0 + j) * pitch + r));
-            }
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (not there[i]) continue;
+                for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const uint4*>(base + int64_t(r + j) * a.n);
                 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t w[4] = {u[i][j].x, u[i][j].y, u[i][j].z, u[i][j].w};
-                    float sum = 0.0f;
+                    const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
                     #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const float2 g = ptx::bf16x2_to_float2(w[q]);
-                        if (a.mn_major) v[i][2 * q] = fmaf(f[i][j], g.x, v[i][2 * q]), v[i][2 * q + 1] = fmaf(f[i][j], g.y, v[i][2 * q + 1]);
-                        else sum = fmaf(f[i][2 * q], g.x, sum), sum = fmaf(f[i][2 * q + 1], g.y, sum);
+                        v[2 * q] = fmaf(f[j], g.x, v[2 * q]), v[2 * q + 1] = fmaf(f[j], g.y, v[2 * q + 1]);
                     }
-                    if (not a.mn_major) {
-                        if (j0 == 0) v[i][j] += sum; else v[i][4 + j] += sum;
+                }
+            }
+        } else {
+            // eight rank columns of four of the columns, twice
+            base += int64_t(n0 + c) * a.rows.rank;
+            #pragma unroll 1
+            for (int r = 0; r < a.rows.rank; r += 8) {
+                float f[8];
+                load8(t + r, f);
+                #pragma unroll
+                for (int j0 = 0; j0 < 8; j0 += 4) {
+                    uint4 u[4];
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const uint4*>(base + (j0 + j) * a.rows.rank + r);
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+                        #pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float2 g = ptx::bf16x2_to_float2(w[q]);
+                            v[j0 + j] = fmaf(f[2 * q], g.x, v[j0 + j]), v[j0 + j] = fmaf(f[2 * q + 1], g.y, v[j0 + j]);
+                        }
                     }
                 }
             }
         }
     };
     if (warp >= 2) {
+        // V does not depend on t: it moves into L2 while t is computed. (Read only when t was there, its round trips to memory, in
+        // competition with the stream of W, took 8 us for 96 rows of 64 adapters.)
+        #pragma unroll 1
+        for (int item = id; item < share * units; item += 256) {
+            int row, c;
+            if (not place(item, row, c)) continue;
+            const int e = adapter_of(a.rows, m0 + row);
+            if (e < 0) continue;
+            const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
+            if (not a.mn_major)
+                for (int i = 0; i < 8 * a.rows.rank; i += 64) ptx::prefetch_l2(base + int64_t(n0 + c) * a.rows.rank + i);
+            else if (c % 64 == 0)
+                for (int r = 0; r < a.rows.rank; ++r) ptx::prefetch_l2(base + int64_t(r) * a.n + n0 + c);
+        }
         cudaGridDependencySynchronize();      // t comes from the kernel before
-        low_rank(id, low);
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) low_rank(id + 256 * i, low[i]);
         __syncwarp();
     }
     if (warp >= 2 and warp < 6) {
@@ -1238,10 +1256,10 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     tc::cluster_sync();                       // all parts have arrived; nobody touches another CTA's shared memory after this
     if (warp >= 2) {
         for (int first = id; first < share * units; first += 512) {
-            if (first != id) low_rank(first, low);
             #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 int row, c;
+                if (first != id) low_rank(first + 256 * i, low[i]);
                 if (not place(first + 256 * i, row, c)) continue;
                 float v[8] = {};
                 add_parts(v, smem_part, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
