@@ -165,7 +165,10 @@ void lora_wgrad(LoraWgradArgs args, const void* x, cudaStream_t stream) {
     const int64_t part = int64_t(kLoraWgradColumns) * (math::align(args.rows.rank, 16) + 4) * 4;                      // overlays the ring
     const int64_t smem = std::max<int64_t>(int64_t(args.num_stages) * args.stage_bytes, part) + 1024;
     const CUtensorMap map_x = make_map_2d(x, args.rows.num_rows, args.m, 64, kLoraBlockK);
-    launch_kernel_as({int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 320, smem, args.cluster, false}, lora_wgrad_kernel, stream, map_x, args);
+    const LaunchShape shape = {int64_t(args.m_tiles) * args.rows.num_adapters * args.cluster, 320, smem, args.cluster, false};
+    if (args.rows.rank <= 32) launch_kernel_as(shape, lora_wgrad_kernel<2>, stream, map_x, args);
+    else if (args.rows.rank <= 64) launch_kernel_as(shape, lora_wgrad_kernel<4>, stream, map_x, args);
+    else launch_kernel_as(shape, lora_wgrad_kernel<kLoraMaxRank / 16>, stream, map_x, args);
 }
 
 }  // namespace deep_ep::launch

@@ -1289,6 +1289,8 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 constexpr int kLoraWgradColumns = 256;
 constexpr int kLoraMaxTileWords = 2048;       // bitmap of row tiles: 2048 * 32 tiles of 128 rows
 
+// kUnits: units of eight rank columns per writer thread (two threads share a row)
+template <int kUnits>
 __global__ void __launch_bounds__(320, 1)
 lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LoraWgradArgs a) {
     using namespace lora_detail;
@@ -1379,16 +1381,14 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     } else {
         // ------------------------------------------------------------------ writers of the B operand, then the epilogue
         const int id = (threadIdx.x - 64) & 127, group = (warp - 2) / 4, line = id & 63, side = id >> 6;
-        constexpr int kUnits = kLoraMaxRank / 8 / 2;            // units of eight rank columns, dealt out to two threads per row
         // a block's index is asked for in one step, its t in the next, and it is written in the one after that
         int first = -1, first_turn = 0, first32 = -1;           // block whose index has been asked for: first token, number, index as read
         int64_t first64 = -1;
-        int third = -1, third_turn = 0, turn = 0;               // block in registers as hi and lo
-        bool third_mine = false;
-        float next[kUnits][8];
-        uint4 hi[kUnits], lo[kUnits];
-        const auto write = [&]() {
-            const int s = third_turn % stages, phase = (third_turn / stages) & 1;
+        int second = -1, second_turn = 0, turn = 0;             // block whose t has been asked for
+        bool second_mine = false, odd = false;
+        float t_even[kUnits][8], t_odd[kUnits][8];              // of alternate blocks: a copy would wait for the read
+        const auto write = [&](const float (&values)[kUnits][8]) {
+            const int s = second_turn % stages, phase = (second_turn / stages) & 1;
             uint8_t* stage = smem + size_t(s) * a.stage_bytes;
             if (not wait_all_lanes(&empty_bar[s], phase ^ 1, &error_flag)) return false;
             const auto place = [&](int column) {                // 16-byte unit of this row's line in its block of 64 columns
@@ -1397,10 +1397,10 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int r = 8 * (2 * i + side);
-                if (r < a.rows.rank) *place(r) = hi[i], *place(half + r) = lo[i];
+                if (r < a.rows.rank) split8(values[i], *place(r), *place(half + r));
             }
             // rows of other requests in this block: zeros instead of whatever they hold (0 * inf would be NaN)
-            const bool foreign = not third_mine and third + line < a.rows.num_rows;
+            const bool foreign = not second_mine and second + line < a.rows.num_rows;
             if (__any_sync(0xffffffffu, foreign)) {
                 if (not wait_all_lanes(&full_bar[s], phase, &error_flag)) return false;
                 if (foreign)
@@ -1413,7 +1413,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             return true;
         };
         // one step of the pipeline: `token` enters (-1: none), what leaves it is written
-        const auto step = [&](int token, int token_turn) {
+        const auto advance = [&](int token, int token_turn, const float (&now)[kUnits][8], float (&next)[kUnits][8]) {
             // (compared with the adapter in the next step: a comparison here would wait for the read)
             int new32 = -1;
             int64_t new64 = -1;
@@ -1429,13 +1429,14 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 for (int j = 0; j < 8; ++j) next[i][j] = 0.0f;
                 if (mine and 8 * u < a.rows.rank) load8(a.t + int64_t(first + line) * a.rows.rank + 8 * u, next[i]);
             }
-            if (third >= 0 and not write()) return false;
-            third = first, third_mine = mine, third_turn = first_turn;
-            #pragma unroll
-            for (int i = 0; i < kUnits; ++i)
-                if (8 * (2 * i + side) < a.rows.rank) split8(next[i], hi[i], lo[i]);
+            if (second >= 0 and not write(now)) return false;
+            second = first, second_mine = mine, second_turn = first_turn;
             first = token, first32 = new32, first64 = new64, first_turn = token_turn;
             return true;
+        };
+        const auto step = [&](int token, int token_turn) {
+            odd = not odd;
+            return odd ? advance(token, token_turn, t_even, t_odd) : advance(token, token_turn, t_odd, t_even);
         };
         walk([&](int token) {
             const int this_turn = turn++;
