@@ -39,8 +39,9 @@ void choose_lookup(const EmbLookupArgs& a, cudaStream_t stream) {
                aligned(a.out, int64_t(a.hidden) * sizeof(Out), std::min(16, elems * int(sizeof(Out))));
     };
     if (fits(kWide)) {
-        // few rows: one access per lane and item, so that a row is spread over more SMs
-        const bool small = a.num_tokens * math::ceil_div(a.hidden / kWide, 32) < 148 * 64;
+        // few rows: one access per lane and item, so that a row is spread over more SMs. Measured with 7168 columns (one | four
+        // accesses, us): 16 tokens 1.55 | 1.79, 128 1.80 | 1.80, 256 2.31 | 2.07, 8192 47.5 | 37.2.
+        const bool small = a.num_tokens * math::ceil_div(a.hidden / kWide, 32) < 148 * 32;
         if (small) launch_lookup<In, Out, kWide, 1>(a, stream);
         else launch_lookup<In, Out, kWide, 4>(a, stream);
     } else if (kHalf > 1 and fits(kHalf)) {
@@ -131,10 +132,13 @@ void embedding_sort(EmbSortArgs args, int* workspace, const int** ids, const int
 
 // ---------------------------------------------------------------------------------------- gradient
 int embedding_grad_chunk(int num_tokens, int hidden) {
-    // 32 sorted positions per chunk; fewer while that leaves SMs without warps; more for long inputs, so that a run over all of
-    // them is joined from at most 2048 pieces
-    int chunk = 32;
-    while (chunk > 8 and int64_t(math::ceil_div(num_tokens, chunk)) * math::ceil_div(hidden, 128) < 148 * 16) chunk /= 2;
+    // Sorted positions per chunk: many make few runs that cross into the next chunk and have to be joined, few make enough items
+    // for all SMs. Measured (8 | 16 | 32 | 64 positions, us): 16384 tokens with frequent repeats, 7168 columns 240 | 213 | 201 | 193;
+    // 4096 without, 7168 columns 62 | 64 | 72 | 79; 5001 of 1003 columns 26 | 24 | 27 | 32; 500 of 7168 12.3 | 13.7 | 19.8 | 33.
+    // Long inputs take more, so that a run over all of them is joined from at most 2048 pieces.
+    int chunk = 64;
+    const auto items = [&] { return int64_t(math::ceil_div(num_tokens, chunk)) * math::ceil_div(hidden, 128); };
+    while ((chunk > 16 and items() < 148 * 64) or (chunk > 8 and items() < 148 * 16)) chunk /= 2;
     while (math::ceil_div(num_tokens, chunk) > 2048) chunk *= 2;
     return chunk;
 }

@@ -33,11 +33,21 @@ int choose_cluster(int64_t units, int blocks, int least, int sms) {
 
 constexpr int64_t kRingBytes = 192 * 1024;
 // Up to this many products of x A^T, the kernel without tensor cores is ahead: its time is that of reading rows * rank * k
-// elements of A from L2, the other's starts at what setting up a tile costs.
-constexpr int64_t kFewProducts = int64_t(1) << 24;
-// Up to this many elements of t, the low-rank term is computed beside the shared product's stream of W instead of on the
-// tensor cores.
-constexpr int64_t kFewTerms = 4096;
+// elements of A from L2, the other's starts at what setting up a tile costs. Measured (it | tensor cores, us): forward as a
+// whole, K 7168, N 4096: one row of rank 16 16.4 | 16.5, 16 rows of rank 64 20.8 | 24.0, 96 of rank 32 (2^24.4) 30.8 | 38.4, 64 of
+// rank 64 (2^24.8) 32.0 | 30.2. With the rank contiguous (backward) it reads A in pieces of eight bytes; alone, K 7168: 64 rows of
+// rank 8 (2^21.8) 6.8 | 9.6, 4 of rank 128 (2^21.8) 10.3 | 10.3, 16 of rank 64 (2^22.8) 17.1 | 9.6.
+constexpr int64_t kFewProducts = int64_t(1) << 25, kFewProductsRankContiguous = int64_t(1) << 22;
+
+// One row tile: the low-rank term is computed beside the shared product's stream of W while it has few elements of t, or few
+// for the blocks that the tensor cores would need (one per adapter that occurs). Measured with K 7168, N 4096 (beside the
+// stream | tensor cores, us): 8 adapters of rank 16: 64 rows 21.2 | 24.7, 128 rows 24.6 | 26.6; 64 adapters of rank 16: 128 rows
+// 27.3 | 44.6; 16 adapters of rank 32: 64 rows 28.7 | 28.5, 128 rows 37.1 | 33.5; 8 adapters of rank 128: 16 rows 30.8 | 31.2, 32 rows
+// 47.2 | 36.4.
+bool few_terms(const LoraRows& r) {
+    const int64_t terms = int64_t(r.num_rows) * r.rank, blocks = int64_t(std::min(r.num_adapters, r.num_rows)) * r.rank;
+    return r.num_rows <= kLoraTileRows and terms <= std::max<int64_t>(1536, 3 * blocks);
+}
 
 }  // namespace
 
@@ -45,7 +55,7 @@ void lora_shrink(LoraShrinkArgs args, const void* x, const void* a, cudaStream_t
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
     const int rows = args.rows.num_rows, rank = args.rows.rank;
-    if (rows <= kLoraTileRows and int64_t(rows) * rank * args.k <= kFewProducts) {
+    if (rows <= kLoraTileRows and int64_t(rows) * rank * args.k <= (args.mn_major ? kFewProductsRankContiguous : kFewProducts)) {
         // (an SM divides its memory between cache and shared memory by the kernels on it: with the default, the next kernel's
         // CTAs, which need all of the latter, could not join before these have left)
         CUDA_CHECK(cudaFuncSetAttribute(lora_shrink_rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
@@ -112,12 +122,11 @@ void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, 
 bool launch_gemm_few(const LoraGemmArgs& g, const void* x, const void* w, int sms, cudaStream_t stream) {
     LoraGemmFewArgs args = {};
     args.rows = g.rows, args.k = g.k, args.n = g.n, args.mn_major = g.mn_major, args.t = g.t, args.v = g.v, args.y = g.y;
-    args.m_tiles = math::ceil_div(g.rows.num_rows, kLoraTileRows);
-    args.x_box_rows = args.m_tiles > 1 ? kLoraTileRows : math::align(g.rows.num_rows, 8);
+    args.x_box_rows = math::align(g.rows.num_rows, 8);
     const int blocks = math::ceil_div(g.k, kLoraBlockK);
     double best = 0;
     for (int bn = 64; bn <= 128; bn *= 2) {
-        const int64_t tiles = int64_t(args.m_tiles) * math::ceil_div(g.n, bn);
+        const int64_t tiles = math::ceil_div(g.n, bn);
         if (tiles > sms) continue;
         const int block_bytes = (args.x_box_rows + bn) * kLoraBlockK * 2, sub = std::clamp(48 * 1024 / block_bytes, 1, 4);
         const int cluster = choose_cluster(tiles, math::ceil_div(blocks, sub), 2, sms);
@@ -126,7 +135,7 @@ bool launch_gemm_few(const LoraGemmArgs& g, const void* x, const void* w, int sm
         if (best == 0 or stream_us + tail_us < best) best = stream_us + tail_us, args.block_n = bn, args.cluster = cluster, args.stage_blocks = sub;
     }
     if (best == 0) return false;
-    const int64_t tiles = int64_t(args.m_tiles) * math::ceil_div(g.n, args.block_n);
+    const int64_t tiles = math::ceil_div(g.n, args.block_n);
     const int64_t part_bytes = int64_t(kLoraTileRows) * args.block_n * 4, budget = 225 * 1024 - 1024 - part_bytes;
     const int64_t stage = int64_t(args.stage_blocks) * (args.x_box_rows + args.block_n) * kLoraBlockK * 2;
     args.num_stages = static_cast<int>(std::min<int64_t>(32, budget / stage));
@@ -142,11 +151,13 @@ void lora_gemm(LoraGemmArgs args, const void* x, const void* w, cudaStream_t str
     ensure_context_once_per_thread();
     args.rows.status = failure_word_checked();
     const int sms = device_sms();
+    if (few_terms(args.rows) and launch_gemm_few(args, x, w, sms, stream)) return;
+    // A wave of 256 x 256 tiles by pairs of CTAs takes about 1.5 times as long as one of 128 x 128 tiles by single ones. Measured
+    // with K 4096, N 4096, rank 16 (pairs | single, us): 512 rows 37.9 | 31.0, 768 39.6 | 42.6, 1280 63.7 | 67.6, 8192 221 | 293.
     const int64_t rows = args.rows.num_rows;
-    if (rows * args.rows.rank <= kFewTerms and launch_gemm_few(args, x, w, sms, stream)) return;
-    // 256 x 256 tiles by pairs of CTAs as soon as every pair has one; smaller tiles keep more SMs busy before that
+    const int64_t tiles = math::ceil_div<int64_t>(rows, kLoraTileRows) * math::ceil_div(args.n, kLoraGemmColumns);
     const int64_t pair_tiles = math::ceil_div<int64_t>(rows, 2 * kLoraTileRows) * math::ceil_div(args.n, 256);
-    if (rows > kLoraTileRows and sms >= 2 and pair_tiles >= sms / 2) launch_gemm_pair(args, x, w, sms, stream);
+    if (sms >= 2 and 3 * math::ceil_div<int64_t>(pair_tiles, sms / 2) <= 2 * math::ceil_div<int64_t>(tiles, sms)) launch_gemm_pair(args, x, w, sms, stream);
     else launch_gemm(args, x, w, sms, stream);
 }
 

@@ -37,7 +37,7 @@ struct EmbSortArgs {
     int* num_crossing;        // set to 0 for the kernels that follow
 };
 
-constexpr int kEmbRankKeys = 8192;            // batches up to this size are ranked by counting
+constexpr int kEmbRankKeys = 8192;            // batches up to this size are ranked by counting (see embedding_rank_kernel)
 constexpr int kEmbRankThreads = 1024;
 constexpr int kEmbSortThreads = 256;          // form of many launches: eight warps
 constexpr int kEmbClusterThreads = 1024;      // form of one launch: a cluster of up to eight CTAs ...

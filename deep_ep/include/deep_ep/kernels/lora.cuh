@@ -839,7 +839,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 // The same by pairs of CTAs (`cta_group::2`) for many tiles: 256 x 256 per pair, each CTA with its 128 rows of A, half of the 256
 // columns of B, and the accumulator of its rows. A CTA alone reads 12 KB of shared memory for the products of a K step of 16 and
 // takes in as much from the TMA: 192 bytes per clock, where shared memory has 128. A pair needs a third less per SM. Measured
-// with 8101 rows, K 7168, N 4096, rank 64: 351 us with 128 x 256 tiles by single CTAs.
+// with K 4096, N 4096, rank 16: 121 / 221 us for 4096 / 8192 rows, 128 x 128 tiles by single CTAs 146 / 293 us.
 // The MMAs are issued by the even CTA; barriers that concern it count both CTAs. A V block lands on a barrier of its own CTA,
 // where the writers look at it; the even CTA learns from the writers of both that the block is complete.
 constexpr int kLoraPairStages = 6;
@@ -1073,7 +1073,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 }
 
 // ---------------------------------------------------------------------------------------- shared product + adapters, few rows
-// Decode: the time is that of reading W once. A cluster shares the contraction of (row tile, block_n columns of Y), so that
+// Decode, one row tile: the time is that of reading W once. A cluster shares the contraction of block_n columns of Y, so that
 // every SM pulls on W with all the shared memory it has in flight; rows of x that do not exist are not loaded (the products read
 // whatever lies behind them, into accumulator rows that are never stored). The low-rank term is too small for tensor-core
 // blocks of its own (a block per adapter costs about a microsecond, and every row may have another adapter): eight warps, idle
@@ -1095,7 +1095,7 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = ptx::lane_id();
     const int cluster = a.cluster, rank = cluster > 1 ? int(blockIdx.x) % cluster : 0, tile = int(blockIdx.x) / cluster;
     const int BN = a.block_n, stages = a.num_stages, sub = a.stage_blocks;       // a stage holds `sub` K blocks
-    const int m0 = tile % a.m_tiles * kLoraTileRows, n0 = tile / a.m_tiles * BN;
+    const int n0 = tile * BN;
     const int blocks = math::ceil_div(a.k, kLoraBlockK), per = math::align(math::ceil_div(blocks, cluster), sub);
     const int kb0 = min(rank * per, blocks), kb1 = min(kb0 + per, blocks), steps = math::ceil_div(kb1 - kb0, sub);
     const uint32_t x_bytes = a.x_box_rows * kLoraBlockK * 2, w_bytes = BN * kLoraBlockK * 2;       // of one K block
@@ -1108,7 +1108,7 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int i = 0; i < sub; ++i) {
             // (blocks behind the contraction's end read zeros; behind this CTA's share they are not multiplied)
             const int k0 = (kb0 + step * sub + i) * kLoraBlockK;
-            tc::tma_load_2d(smem_a + (s * sub + i) * x_bytes, &map_x, k0, m0, &full_bar[s]);
+            tc::tma_load_2d(smem_a + (s * sub + i) * x_bytes, &map_x, k0, 0, &full_bar[s]);
             uint8_t* sb = smem_b + (s * sub + i) * w_bytes;
             if (a.mn_major) for (int c = 0; c < BN / 64; ++c) tc::tma_load_2d(sb + c * 8192, &map_w, n0 + 64 * c, k0, &full_bar[s]);
             else tc::tma_load_2d(sb, &map_w, k0, n0, &full_bar[s]);
@@ -1163,7 +1163,7 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const int id = int(threadIdx.x) - 64;
     const auto place = [&](int item, int& row, int& c) {                         // false: not part of the result
         row = rank * share + item / units, c = item % units * 8;
-        return item < share * units and m0 + row < a.rows.num_rows and n0 + c < a.n;
+        return item < share * units and row < a.rows.num_rows and n0 + c < a.n;
     };
     // low-rank term of an item in fp32, four 16-byte units of V at a time (few registers: see lora_shrink_rows_kernel)
     const auto low_rank = [&](int item, float (&v)[8]) {
@@ -1171,10 +1171,10 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int j = 0; j < 8; ++j) v[j] = 0.0f;
         int row, c;
         if (not place(item, row, c)) return;
-        const int e = adapter_of(a.rows, m0 + row);
+        const int e = adapter_of(a.rows, row);
         if (e < 0) return;
         const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
-        const float* t = a.t + int64_t(m0 + row) * a.rows.rank;
+        const float* t = a.t + int64_t(row) * a.rows.rank;
         if (a.mn_major) {
             // eight columns of the rank rows r .. r + 3
             base += n0 + c;
@@ -1227,7 +1227,7 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int item = id; item < share * units; item += 256) {
             int row, c;
             if (not place(item, row, c)) continue;
-            const int e = adapter_of(a.rows, m0 + row);
+            const int e = adapter_of(a.rows, row);
             if (e < 0) continue;
             const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
             if (not a.mn_major)
@@ -1245,9 +1245,9 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         wait_all_lanes(&done_bar, 0, &error_flag);
         tc::fence_after_thread_sync();
         tc::cluster_wait();
-        if (m0 + quarter * 32 < a.rows.num_rows and quarter * 32 < a.x_box_rows)
+        if (quarter * 32 < a.rows.num_rows)
             send_part(tc::map_to_cta(smem_part + (rank * share + row % share) * (BN * 4), row / share), tmem + (uint32_t(quarter * 32) << 16), BN, row,
-                      m0 + row < a.rows.num_rows);
+                      row < a.rows.num_rows);
         tc::fence_before_thread_sync();
         __syncwarp();
     } else {
@@ -1265,7 +1265,7 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 add_parts(v, smem_part, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += low[i][j];
-                store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c, v);
+                store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(row) * a.n + n0 + c, v);
             }
         }
     }
@@ -1285,7 +1285,9 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 //   warp 0      TMA producer     warp 1      MMA issuer
 //   warps 2-9   writers of t, two groups that take the blocks in turn; warps 2-5 read the accumulator
 // A block of 64 tokens is little work for the tensor cores, so the writers set the pace: each asks for the index two blocks
-// ahead and for t one block ahead. (One group that read both when it needed them took 1.4 us per block.)
+// ahead and for t one block ahead, into registers of its own for every other block. Measured with 4099 rows of 4 adapters in runs,
+// 7168 columns: 22 / 25 / 69 us at rank 16 / 32 / 128 (one register set, copied from block to block: 28 / 32 / 66 us; one group that
+// read both when it needed them: 1.4 us per block). Rows in another order cost each adapter the row tiles in which it occurs.
 constexpr int kLoraWgradColumns = 256;
 constexpr int kLoraMaxTileWords = 2048;       // bitmap of row tiles: 2048 * 32 tiles of 128 rows
 

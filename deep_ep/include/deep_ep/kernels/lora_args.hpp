@@ -42,14 +42,13 @@ struct LoraGemmArgs {
     void* y;
 };
 
-// The same for few rows and a small rank
+// The same for one row tile and a small low-rank term
 struct LoraGemmFewArgs {
     LoraRows rows;
     int k, n, mn_major, cluster;
-    int m_tiles;
     int block_n;                          // columns of Y per tile: 64 or 128
     int stage_blocks, num_stages;         // K blocks per stage, stages
-    int x_box_rows;                       // rows of X that a load brings (a whole tile, or all rows there are)
+    int x_box_rows;                       // rows of X that a load brings: all, up to the next multiple of eight
     const float* t;
     const void* v;
     void* y;

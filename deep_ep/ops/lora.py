@@ -16,6 +16,7 @@ from .._C_loader import _C
 
 __all__ = ['lora_linear']
 
+
 def _reference(x, w, lora_a, lora_b, idx, scaling):
     """Plain form in fp32 (CPU): rows are picked by adapter, so one adapter's values never meet another's rows."""
     dtype = x.dtype
@@ -56,9 +57,8 @@ class _LoraLinear(torch.autograd.Function):
         if want_b:
             db = _weight_grad(dy, t, idx, presence, lora_b, False)
         if want_w:
-            from .dense import _one_group
             from .grouped_gemm import grouped_gemm_wgrad
-            one = _one_group(x.size(0), x.device)
+            one = torch.full((1,), x.size(0), dtype=torch.int32, device=x.device)       # one group, all rows
             dw = torch.empty((1, *w.shape), dtype=w.dtype, device=w.device)
             grouped_gemm_wgrad(dy, x.contiguous(), dw, one, one, accumulate=False)
             dw = dw[0]
@@ -75,7 +75,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     ranks with zero rows). Both products accumulate in fp32; the intermediate `x A^T` keeps 16 bits; `y` is rounded once.
 
     Gradients reach `x`, `lora_a` and `lora_b` (or their fp32 `main_grad`), and `w` if it wants one (K and N multiples of
-    128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to.
+    128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to. The adapters'
+    gradients read a row tile of 128 once per adapter that occurs in it, so long training batches are best ordered by adapter.
+    A backward pass may be captured in a CUDA graph when no eager autograd graph of the same leaves is alive.
     """
     if not isinstance(scaling, torch.Tensor):
         scaling = torch.full((lora_a.size(0),), float(scaling), dtype=torch.float32, device=x.device)

@@ -116,7 +116,8 @@ def test_refusals():
     (127, 1000, 520, 40, 3, 'runs'), (128, 512, 256, 128, 3, 'mixed'), (96, 2048, 1024, 16, 64, 'mixed'), (300, 1024, 392, 64, 200, 'mixed'),
     (257, 640, 384, 32, 2, 'none'), (1025, 512, 2048, 48, 4, 'runs'), (2500, 1096, 2056, 72, 3, 'runs'), (5000, 256, 4096, 8, 6, 'mixed'),
     (1, 256, 128, 8, 1, 'none'), (128, 1024, 512, 32, 7, 'mixed'), (129, 1024, 512, 32, 7, 'mixed'), (500, 2048, 200, 8, 3, 'mixed'),
-    (120, 4096, 1000, 64, 2, 'mixed'), (1, 128, 16384, 64, 2, 'same'), (64, 7168, 64, 128, 3, 'runs')])
+    (120, 4096, 1000, 64, 2, 'mixed'), (1, 128, 16384, 64, 2, 'same'), (64, 7168, 64, 128, 3, 'runs'), (700, 512, 4096, 16, 2, 'runs'),
+    (19500, 64, 120, 8, 3, 'runs')])
 def test_forward_and_gradients(rows, k, n, rank, adapters, order):
     args = make(rows, k, n, rank, adapters, 'cuda', order, seed=rows)
     results = run_all(args)
