@@ -67,9 +67,16 @@ inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::T
     return out;
 }
 
-// out[v] (+)= scale * sum of dy[t] over idx[t] == v; `out` fp32 or of dy's type, `accumulate` only for fp32
-inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, double scale, const torch::Tensor& out, bool accumulate) {
+// out[v] (+)= scale * sum of dy[t] over idx[t] == v; `out` fp32 or of dy's type (a new one of dy's type without), `accumulate`
+// only for fp32
+inline torch::Tensor embedding_grad(const torch::Tensor& dy_in, const torch::Tensor& idx_in, int64_t rows, double scale,
+                                    const std::optional<torch::Tensor>& out_in, bool accumulate) {
+    EP_HOST_ASSERT_MSG(dy_in.is_cuda() and dy_in.dim() == 2 and rows >= 0 and (out_in.has_value() or not accumulate), "dy is a CUDA matrix; accumulation needs `out`");
+    const auto dy = dy_in.size(1) > 1 and dy_in.stride(1) != 1 ? dy_in.contiguous() : dy_in;
+    const auto idx = idx_in.contiguous();
+    const auto out = out_in.has_value() ? *out_in : torch::empty({rows, dy.size(1)}, dy.options());
     check_rows(dy), check_rows(out), check_ids(idx, dy);
+    EP_HOST_ASSERT_MSG(out.size(0) == rows, "out is [num_rows, hidden]");
     EP_HOST_ASSERT_MSG(out.device() == dy.device(), "all tensors of a call lie on one device");
     EP_HOST_ASSERT_MSG(dy.size(0) == idx.numel() and dy.size(1) == out.size(1), "dy is [number of indices, hidden], out [rows, hidden]");
     EP_HOST_ASSERT_MSG(dy.scalar_type() == out.scalar_type() or out.scalar_type() == torch::kFloat32, "out is fp32 or of dy's type");
@@ -89,15 +96,15 @@ inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, do
     const c10::cuda::CUDAGuard guard(dy.device());
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
     const int num_tokens = static_cast<int>(idx.numel()), num_rows = static_cast<int>(out.size(0)), hidden = static_cast<int>(out.size(1));
-    if (num_rows == 0 or hidden == 0) return;
+    if (num_rows == 0 or hidden == 0) return out;
 
     kernels::EmbGradArgs g = {};
     g.dy = dy.data_ptr(), g.dy_stride = dy.stride(0);
     g.num_tokens = num_tokens, g.num_rows = num_rows, g.hidden = hidden, g.scale = static_cast<float>(scale);
     g.out = out.data_ptr(), g.out_stride = out.stride(0), g.accumulate = accumulate;
     if (num_tokens == 0) {
-        if (not accumulate) out.zero_();
-        return;
+        if (not accumulate) at::Tensor(out.detach()).zero_();
+        return out;
     }
     g.chunk = launch::embedding_grad_chunk(num_tokens, hidden), g.num_chunks = (num_tokens + g.chunk - 1) / g.chunk;
     // scratch of this call, from the caching allocator: freed in stream order, private to a graph that is being captured
@@ -113,12 +120,14 @@ inline void embedding_grad(const torch::Tensor& dy, const torch::Tensor& idx, do
     s.num_crossing = g.num_crossing = ints.data_ptr<int>() + sort_ints + bitmap_ints, g.crossing = g.num_crossing + 1;
     launch::embedding_sort(s, ints.data_ptr<int>(), &g.ids, &g.order, stream);
     launch::embedding_grad(g, in_type, out_type, stream);
+    return out;
 }
 
 inline void register_embedding(pybind11::module_& m) {
     namespace py = pybind11;
     m.def("embedding_lookup", &embedding_lookup, py::arg("table"), py::arg("idx"), py::arg("scale") = 1.0, py::arg("table_sf") = py::none());
-    m.def("embedding_grad", &embedding_grad, py::arg("dy"), py::arg("idx"), py::arg("scale"), py::arg("out"), py::arg("accumulate") = false);
+    m.def("embedding_grad", &embedding_grad, py::arg("dy"), py::arg("idx"), py::arg("num_rows"), py::arg("scale") = 1.0,
+          py::arg("out") = py::none(), py::arg("accumulate") = false);
 }
 
 }  // namespace deep_ep::ops

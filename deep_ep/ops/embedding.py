@@ -85,6 +85,8 @@ def embedding_grad(dy: torch.Tensor, idx: torch.Tensor, num_rows: int, scale: fl
     rows without a token become zero). With `accumulate` the sums are added to an fp32 `out` instead, and only the rows of
     tokens are touched. Sums are in fp32, in token order, scaled and rounded once.
     """
+    if dy.is_cuda:
+        return _C.embedding_grad(dy, idx, num_rows, scale, out, accumulate)          # (which looks at every argument)
     assert dy.dim() == 2 and dy.size(0) == idx.numel() and dy.dtype in _TABLE_TYPES, 'dy is [number of indices, hidden]'
     assert idx.dtype in (torch.int64, torch.int32) and idx.device == dy.device
     assert num_rows >= 0
@@ -94,12 +96,7 @@ def embedding_grad(dy: torch.Tensor, idx: torch.Tensor, num_rows: int, scale: fl
     assert out.shape == (num_rows, dy.size(1)) and out.device == dy.device, 'out is [num_rows, hidden]'
     assert out.dtype == torch.float32 or (out.dtype == dy.dtype and not accumulate), 'out is fp32, or of dy\'s type and overwritten'
     flat = idx.reshape(-1)
-    if not dy.is_cuda:
-        valid = (flat >= 0) & (flat < num_rows)
-        sums = torch.zeros((num_rows, dy.size(1)), dtype=torch.float32).index_add_(0, flat[valid].long(), dy[valid].float()) * scale
-        return out.add_(sums) if accumulate else out.copy_(sums)
-    if dy.size(1) > 1 and dy.stride(1) != 1 or dy.stride(0) < 0:
-        dy = dy.contiguous()
+    valid = (flat >= 0) & (flat < num_rows)
+    sums = torch.zeros((num_rows, dy.size(1)), dtype=torch.float32).index_add_(0, flat[valid].long(), dy[valid].float()) * scale
     with torch.no_grad():
-        _C.embedding_grad(dy, flat.contiguous(), float(scale), out, accumulate)
-    return out
+        return out.add_(sums) if accumulate else out.copy_(sums)
