@@ -1,0 +1,36 @@
+// What the native autograd nodes share. They are native because a pass over a small batch is a handful of launches of a few
+// microseconds each, to which a node in Python adds about forty.
+#pragma once
+
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/extension.h>
+
+#include <memory>
+#include <optional>
+
+#include <deep_ep/common/exception.hpp>
+
+namespace deep_ep::ops {
+
+// The fp32 buffer that a parameter's gradient is added to, if its Python object carries one
+inline std::optional<torch::Tensor> main_grad(const torch::Tensor& parameter) {
+    const pybind11::gil_scoped_acquire gil;
+    const auto object = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(parameter));
+    const pybind11::object buffer = pybind11::getattr(object, "main_grad", pybind11::none());
+    if (buffer.is_none()) return std::nullopt;
+    EP_HOST_ASSERT_MSG(THPVariable_Check(buffer.ptr()), "`main_grad` is a tensor");
+    return THPVariable_Unpack(buffer.ptr());
+}
+
+// Gradients that were asked for with a graph of their own: an error where somebody differentiates them
+inline void refuse_second_derivatives(torch::autograd::variable_list& grads, const char* message) {
+    for (auto& g : grads) {
+        if (not g.defined()) continue;
+        auto leaf = g.detach();
+        leaf.set_requires_grad(true);
+        g = (*std::make_shared<torch::autograd::DelayedError>(message, 1))({leaf})[0];
+    }
+}
+
+}  // namespace deep_ep::ops

@@ -12,6 +12,7 @@
 #include <deep_ep/common/exception.hpp>
 
 #include "../kernels/api.hpp"
+#include "autograd.hpp"
 
 namespace deep_ep::ops {
 
@@ -38,8 +39,8 @@ inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
 }
 
 // [*idx.shape, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
-inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx_in, double scale,
-                                      const std::optional<torch::Tensor>& table_sf) {
+inline torch::Tensor lookup_rows(const torch::Tensor& table, const torch::Tensor& idx_in, double scale,
+                                 const std::optional<torch::Tensor>& table_sf) {
     const auto idx = idx_in.contiguous();
     check_rows(table), check_ids(idx, table);
     const auto type = embedding_type(table);
@@ -121,6 +122,37 @@ inline torch::Tensor embedding_grad(const torch::Tensor& dy_in, const torch::Ten
     launch::embedding_sort(s, ints.data_ptr<int>(), &g.ids, &g.order, stream);
     launch::embedding_grad(g, in_type, out_type, stream);
     return out;
+}
+
+class EmbeddingLookup : public torch::autograd::Function<EmbeddingLookup> {
+public:
+    static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& table, const torch::Tensor& idx, double scale) {
+        ctx->save_for_backward({idx});
+        ctx->saved_data["table"] = table;        // the parameter itself, for its `main_grad`; its values may change before the backward pass
+        ctx->saved_data["scale"] = scale;
+        return lookup_rows(table, idx, scale, std::nullopt);
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+        const bool again = at::GradMode::is_enabled();           // the gradient is to be differentiated in turn: refused where that happens
+        torch::autograd::variable_list out(3);
+        {
+            const at::NoGradGuard no_grad;
+            const auto table = ctx->saved_data["table"].toTensor();
+            const auto idx = ctx->get_saved_variables()[0].reshape({-1}), dy = grads[0].reshape({idx.numel(), table.size(1)});
+            const double scale = ctx->saved_data["scale"].toDouble();
+            const auto buffer = main_grad(table);
+            const auto dtable = embedding_grad(dy, idx, table.size(0), scale, buffer, buffer.has_value());
+            if (not buffer.has_value()) out[0] = dtable;
+        }
+        if (again) refuse_second_derivatives(out, "embedding_lookup is differentiable once");
+        return out;
+    }
+};
+
+inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale, const std::optional<torch::Tensor>& table_sf) {
+    if (not at::GradMode::is_enabled() or not table.requires_grad() or table_sf.has_value()) return lookup_rows(table, idx, scale, table_sf);
+    return EmbeddingLookup::apply(table, idx, scale);
 }
 
 inline void register_embedding(pybind11::module_& m) {

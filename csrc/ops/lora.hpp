@@ -12,6 +12,7 @@
 #include <deep_ep/common/exception.hpp>
 
 #include "../kernels/api.hpp"
+#include "autograd.hpp"
 
 namespace deep_ep::ops {
 
@@ -121,13 +122,77 @@ inline void lora_wgrad(const torch::Tensor& x_in, const torch::Tensor& t_in, con
     launch::lora_wgrad(args, x.data_ptr(), c10::cuda::getCurrentCUDAStream());
 }
 
+// Gradient of a [N, K] weight: dy^T x, in the weight's type
+inline torch::Tensor dense_weight_grad(const torch::Tensor& dy, const torch::Tensor& x, const torch::Tensor& w, bool pairs) {
+    auto dw = torch::empty_like(w, w.options(), torch::MemoryFormat::Contiguous);
+    if (x.size(0) == 0) return dw.zero_();
+    const auto rows = torch::full({1}, x.size(0), x.options().dtype(torch::kInt32));          // one group, all rows
+    kernels::GroupedGemmArgs args = {};
+    args.mode = kernels::kModeWgrad, args.epilogue = kernels::kEpilogueStore, args.num_groups = 1, args.out_bf16 = true;
+    args.psum = args.count = rows.data_ptr<int>();
+    args.m = static_cast<int>(dy.size(1)), args.n = static_cast<int>(x.size(1)), args.d = dw.data_ptr();
+    launch::grouped_gemm(args, dy.data_ptr(), dy.size(0), dy.size(1), x.data_ptr(), x.size(0), x.size(1), 0, c10::cuda::getCurrentCUDAStream(), pairs);
+    return dw;
+}
+
+class LoraLinear : public torch::autograd::Function<LoraLinear> {
+public:
+    static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& a,
+                                 const torch::Tensor& b, const torch::Tensor& idx, const torch::Tensor& scaling, bool pairs) {
+        auto [y, t] = lora_forward(x, w, a, b, idx, scaling);
+        ctx->save_for_backward({x, w, a, b, idx, scaling, t});
+        ctx->saved_data["pairs"] = pairs;
+        return y;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+        const bool again = at::GradMode::is_enabled();           // the gradients are to be differentiated in turn: refused where that happens
+        torch::autograd::variable_list out(7);
+        {
+            const at::NoGradGuard no_grad;
+            const auto saved = ctx->get_saved_variables();
+            const auto &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &idx = saved[4], &scaling = saved[5], &t = saved[6];
+            const c10::cuda::CUDAGuard guard(x.device());
+            const auto dy = operand(grads[0].to(torch::kBFloat16), 2, x);
+            const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_a = ctx->needs_input_grad(2), want_b = ctx->needs_input_grad(3);
+            // gradient of A or B; added to the parameter's buffer where it has one
+            const auto adapter_grad = [&](const torch::Tensor& rows, const torch::Tensor& low, const torch::Tensor& presence, const torch::Tensor& parameter, bool rank_major) {
+                const auto buffer = main_grad(parameter);
+                const auto result = buffer.has_value() ? *buffer : torch::empty_like(parameter, parameter.options(), torch::MemoryFormat::Contiguous);
+                lora_wgrad(rows, low, idx, presence, result, rank_major, buffer.has_value());
+                return buffer.has_value() ? torch::Tensor() : result;
+            };
+            if (want_x or want_a or want_b) {
+                const auto [dt, presence, dx] = lora_backward(dy, w, a, b, idx, scaling, want_x);
+                if (want_x) out[0] = *dx;
+                if (want_a) out[2] = adapter_grad(x, dt, presence, a, true);
+                if (want_b) out[3] = adapter_grad(dy, t, presence, b, false);
+            }
+            if (want_w) out[1] = dense_weight_grad(dy, operand(x, 2, x), w, ctx->saved_data["pairs"].toBool());
+        }
+        if (again) refuse_second_derivatives(out, "lora_linear is differentiable once");
+        return out;
+    }
+};
+
+// y of the operator; `scalings` (fp32 [adapters]) goes before `scaling`
+inline torch::Tensor lora_linear(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& idx_in,
+                                 double scaling, const std::optional<torch::Tensor>& scalings, bool pairs) {
+    EP_HOST_ASSERT_MSG(x.is_cuda() and a.dim() == 3 and idx_in.dim() == 1, "x is a CUDA matrix, a [adapters, rank, K], adapter indices [rows]");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto idx = idx_in.contiguous();
+    const auto s = scalings.has_value() ? *scalings : torch::full({a.size(0)}, scaling, x.options().dtype(torch::kFloat32).requires_grad(false));
+    EP_HOST_ASSERT_MSG(not s.requires_grad(), "scaling receives no gradient");
+    if (not at::GradMode::is_enabled() or not (x.requires_grad() or w.requires_grad() or a.requires_grad() or b.requires_grad()))
+        return std::get<0>(lora_forward(x, w, a, b, idx, s));
+    EP_HOST_ASSERT_MSG(not w.requires_grad() or (w.dim() == 2 and w.size(0) % 128 == 0 and w.size(1) % 128 == 0), "the gradient of w needs K and N to be multiples of 128");
+    return LoraLinear::apply(x, w, a, b, idx, s, pairs);
+}
+
 inline void register_lora(pybind11::module_& m) {
     namespace py = pybind11;
-    m.def("lora_forward", &lora_forward, py::arg("x"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling"));
-    m.def("lora_backward", &lora_backward, py::arg("dy"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling"),
-          py::arg("want_dx") = true);
-    m.def("lora_wgrad", &lora_wgrad, py::arg("x"), py::arg("t"), py::arg("idx"), py::arg("presence"), py::arg("out"), py::arg("rank_major"),
-          py::arg("accumulate") = false);
+    m.def("lora_linear", &lora_linear, py::arg("x"), py::arg("w"), py::arg("a"), py::arg("b"), py::arg("idx"), py::arg("scaling") = 1.0,
+          py::arg("scalings") = py::none(), py::arg("gemm_pairs") = true);
 }
 
 }  // namespace deep_ep::ops

@@ -20,8 +20,6 @@ _TABLE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _lookup(table: torch.Tensor, idx: torch.Tensor, scale: float, table_sf: Optional[torch.Tensor]) -> torch.Tensor:
-    if table.is_cuda:
-        return _C.embedding_lookup(table, idx, scale, table_sf)
     flat = idx.reshape(-1)
     valid = (flat >= 0) & (flat < table.size(0))
     rows = table.new_zeros((flat.numel(), table.size(1)), dtype=torch.float32)
@@ -32,7 +30,7 @@ def _lookup(table: torch.Tensor, idx: torch.Tensor, scale: float, table_sf: Opti
     return out.view(*idx.shape, table.size(1))
 
 
-class _Lookup(torch.autograd.Function):
+class _Lookup(torch.autograd.Function):          # CPU; the native call has its own
     @staticmethod
     def forward(ctx, table, idx, scale):
         ctx.save_for_backward(idx)
@@ -44,7 +42,7 @@ class _Lookup(torch.autograd.Function):
     def backward(ctx, dy):
         idx, = ctx.saved_tensors
         table = ctx.table
-        dy = dy.reshape(-1, table.size(1))
+        dy = dy.reshape(idx.numel(), table.size(1))
         main_grad = getattr(table, 'main_grad', None)
         if main_grad is not None:
             embedding_grad(dy, idx, table.size(0), ctx.scale, out=main_grad, accumulate=True)
@@ -62,8 +60,8 @@ def embedding_lookup(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0,
     (not an e4m3 one) in its own type, or its fp32 `main_grad`; a backward pass may be captured in a CUDA graph when no eager
     autograd graph of the same table is alive.
     """
-    if table.is_cuda and not (table.requires_grad and torch.is_grad_enabled()):
-        return _C.embedding_lookup(table, idx, scale, table_sf)          # (which looks at every argument)
+    if table.is_cuda:
+        return _C.embedding_lookup(table, idx, scale, table_sf)          # (which looks at every argument, and is the autograd node)
     assert table.dim() == 2 and idx.dtype in (torch.int64, torch.int32), 'table [rows, hidden], idx int64 or int32'
     assert idx.device == table.device, 'table and indices lie on one device'
     if table_sf is not None:

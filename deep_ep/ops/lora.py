@@ -13,6 +13,7 @@ from typing import Optional, Union
 import torch
 
 from .._C_loader import _C
+from .grouped_gemm import MODE_WGRAD, _pairs
 
 __all__ = ['lora_linear']
 
@@ -26,43 +27,6 @@ def _reference(x, w, lora_a, lora_b, idx, scaling):
         rows = torch.nonzero(idx == e).flatten()          # (an adapter without rows gets a gradient of zeros, as on the GPU)
         y = y.index_add(0, rows, scaling[e] * ((x[rows] @ lora_a[e].t()) @ lora_b[e].t()))
     return y.to(dtype)
-
-
-def _weight_grad(x, t, idx, presence, parameter, rank_major):
-    """Gradient of A (`rank_major`) or B; added to the parameter's fp32 `main_grad` where it has one."""
-    main_grad = getattr(parameter, 'main_grad', None)
-    out = torch.empty_like(parameter, memory_format=torch.contiguous_format) if main_grad is None else main_grad
-    _C.lora_wgrad(x, t, idx, presence, out, rank_major, main_grad is not None)
-    return out if main_grad is None else None
-
-
-class _LoraLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, lora_a, lora_b, idx, scaling):
-        y, t = _C.lora_forward(x, w, lora_a, lora_b, idx, scaling)
-        ctx.save_for_backward(x, w, lora_a, lora_b, idx, scaling, t)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w, lora_a, lora_b, idx, scaling, t = ctx.saved_tensors
-        dy = dy.to(torch.bfloat16).contiguous()
-        dx = dw = da = db = None
-        want_x, want_w, want_a, want_b = ctx.needs_input_grad[:4]
-        if want_x or want_a or want_b:
-            dt, presence, dx = _C.lora_backward(dy, w, lora_a, lora_b, idx, scaling, want_x)
-        if want_a:
-            da = _weight_grad(x, dt, idx, presence, lora_a, True)
-        if want_b:
-            db = _weight_grad(dy, t, idx, presence, lora_b, False)
-        if want_w:
-            from .grouped_gemm import grouped_gemm_wgrad
-            one = torch.full((1,), x.size(0), dtype=torch.int32, device=x.device)       # one group, all rows
-            dw = torch.empty((1, *w.shape), dtype=w.dtype, device=w.device)
-            grouped_gemm_wgrad(dy, x.contiguous(), dw, one, one, accumulate=False)
-            dw = dw[0]
-        return dx, dw, da, db, None, None
 
 
 def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_idx: torch.Tensor,
@@ -79,17 +43,14 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     gradients read a row tile of 128 once per adapter that occurs in it, so long training batches are best ordered by adapter.
     A backward pass may be captured in a CUDA graph when no eager autograd graph of the same leaves is alive.
     """
+    if x.is_cuda:
+        # (the native call looks at every argument, and is the autograd node where a gradient is wanted)
+        if isinstance(scaling, torch.Tensor):
+            return _C.lora_linear(x, w, lora_a, lora_b, adapter_idx, 1.0, scaling, _pairs(MODE_WGRAD))
+        return _C.lora_linear(x, w, lora_a, lora_b, adapter_idx, scaling, None, _pairs(MODE_WGRAD))
     if not isinstance(scaling, torch.Tensor):
         scaling = torch.full((lora_a.size(0),), float(scaling), dtype=torch.float32, device=x.device)
     assert not scaling.requires_grad, 'scaling receives no gradient'
-    if x.is_cuda:
-        if adapter_idx.dim() == 1 and adapter_idx.size(0) > 1 and adapter_idx.stride(0) != 1:
-            adapter_idx = adapter_idx.contiguous()
-        if not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or lora_a.requires_grad or lora_b.requires_grad)):
-            return _C.lora_forward(x, w, lora_a, lora_b, adapter_idx, scaling)[0]       # (which looks at every argument)
-        if w.requires_grad:
-            assert w.size(0) % 128 == 0 and w.size(1) % 128 == 0, 'the gradient of w needs K and N to be multiples of 128'
-        return _LoraLinear.apply(x, w, lora_a, lora_b, adapter_idx, scaling)
     assert x.dim() == 2 and w.dim() == 2 and lora_a.dim() == 3 and lora_b.dim() == 3, 'x [rows, K], w [N, K], lora_a [E, rank, K], lora_b [E, N, rank]'
     rows, k = x.shape
     n, adapters, rank = w.size(0), lora_a.size(0), lora_a.size(1)

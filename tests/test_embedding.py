@@ -277,3 +277,23 @@ def test_autograd_main_grad_other_stream_and_graph():
     static_ids.copy_(flat), static_dy.copy_(dy.view(-1, 320))
     graph.replay()
     assert torch.equal(grad, expected)
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_changed_empty_or_computed_table():
+    ids = torch.tensor([[1, 3], [1, -1]], device='cuda')
+    table = torch.randn(5, 32, device='cuda').requires_grad_()
+    out = embedding_lookup(table, ids, 2.0)
+    with torch.no_grad():
+        table.zero_()                               # the gradient does not depend on the values
+    out.sum().backward()
+    expected = torch.zeros(5, 32, device='cuda')
+    expected[1], expected[3] = 4.0, 2.0
+    assert torch.equal(table.grad, expected)
+    assert (torch.autograd.grad(embedding_lookup(table, ids[:0]).sum(), table)[0] == 0).all()
+    # a table that is itself computed, and second derivatives
+    grad, = torch.autograd.grad(embedding_lookup(table * 3, ids, 2.0).sum(), table)
+    assert torch.equal(grad, 3 * expected)
+    kept, = torch.autograd.grad(embedding_lookup(table, ids, 2.0).sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        kept.sum().backward()

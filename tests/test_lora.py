@@ -244,3 +244,15 @@ def test_refusals_on_the_gpu():
                 lambda: lora_linear(x, w, a[0], b, idx, s), lambda: lora_linear(x, w.cpu(), a, b, idx, s)):
         with refused:
             bad()
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused_where_they_are_taken():
+    x, w, a, b, dy, idx, s = make(9, 64, 64, 8, 2, 'cuda')
+    a.requires_grad_()
+    y = lora_linear(x, w, a, b, idx, s)
+    plain, = torch.autograd.grad(y, a, dy, retain_graph=True)
+    kept, = torch.autograd.grad(y, a, dy, create_graph=True)
+    assert torch.equal(plain, kept)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        kept.sum().backward()
