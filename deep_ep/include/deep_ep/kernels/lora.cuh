@@ -1081,7 +1081,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 //   warp 0      TMA producer     warp 1      MMA issuer
 //   warps 2-9   low-rank term; warps 2-5 then send the accumulator's rows to their owners, and all eight add and store
 // One tile per CTA. The wait for the kernel that computes t comes after W is under way.
-// (launched with 320 threads; the bound keeps the registers at 88, beside which three CTAs of lora_shrink_rows_kernel fit in each
+// (launched with 320 threads; the bound keeps the registers at 88 or less, beside which three CTAs of lora_shrink_rows_kernel fit in each
 // quarter of an SM: three warps of this kernel and six of that one)
 __global__ void __launch_bounds__(736, 1)
 lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ LoraGemmFewArgs a) {

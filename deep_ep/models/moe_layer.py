@@ -171,7 +171,9 @@ class MoELayer(nn.Module):
             found = [getattr(self, name, None) for name in names]
             found = [getattr(p, 'main_grad', None) if getattr(p, 'main_grad', None) is not None else p.grad for p in found if p is not None]
             return [g for g in found if g is not None]
-        return clip_grad_norm_(gradients(('w_gate_up', 'w_down')), max_norm, group=self.group if self.num_ranks > 1 else None,
+        # (an empty tensor keeps the collective on the layer's device when no expert has a gradient yet)
+        experts = gradients(('w_gate_up', 'w_down')) or [torch.empty(0, device=self.w_gate_up.device)]
+        return clip_grad_norm_(experts, max_norm, group=self.group if self.num_ranks > 1 else None,
                                replicated=gradients(('gate', 'shared_gate_up', 'shared_down')))
 
     # ------------------------------------------------------------------------------------------ FP8 inference

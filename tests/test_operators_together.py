@@ -25,6 +25,7 @@ def _step_worker(rank, world, device):
     a = (torch.randn(adapters, rank_r, hidden, device=device) * hidden ** -0.5).to(torch.bfloat16).requires_grad_()
     b = (torch.randn(adapters, hidden, rank_r, device=device) * 0.3).to(torch.bfloat16).requires_grad_()
     layer = MoELayer(dist.group.WORLD, cfg, device=torch.device(device))
+    assert float(layer.clip_grad_norm_(1.0)) == 0.0                  # no gradients yet
     torch.manual_seed(10 + rank)
     ids = torch.randint(-1, vocab, (tokens,), device=device)
     idx = torch.randint(-1, adapters, (tokens,), device=device)
