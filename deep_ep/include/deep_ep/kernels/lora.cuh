@@ -58,12 +58,12 @@ struct TileAdapters {
             if (id[i] > last) best = min(best, static_cast<unsigned>(id[i]));
         return static_cast<int>(__reduce_min_sync(0xffffffffu, best));
     }
-    // some row of the batch in this tile has another adapter (or none) than `e`
-    EP_DEVICE bool others_than(int e) const {
-        bool other = false;
+    // some row of the batch in this tile has no adapter
+    EP_DEVICE bool some_without() const {
+        bool without = false;
         #pragma unroll
-        for (int i = 0; i < kPer; ++i) other = other or (inside[i] and id[i] != e);
-        return __any_sync(0xffffffffu, other);
+        for (int i = 0; i < kPer; ++i) without = without or (inside[i] and id[i] < 0);
+        return __any_sync(0xffffffffu, without);
     }
 };
 
@@ -133,38 +133,43 @@ __device__ __noinline__ float poisoned(const LoraGemmArgs& a, int row, int n) {
     return sum;
 }
 
-// This row's t, 32 columns from 32 * c, as bf16 hi and lo
-EP_DEVICE void read_t(const LoraGemmArgs& a, int row, bool there, int c, uint4 (&hi)[4], uint4 (&lo)[4]) {
+// This row's t, 32 columns from 32 * c (zeros behind the rank). Asked for a block ahead of its use: a read of a K block's own would be
+// a round trip to L2 per block.
+EP_DEVICE void read_t(const LoraGemmArgs& a, int row, bool there, int c, float (&t)[4][8]) {
     #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        float v[8] = {};
-        if (there and 32 * c + 8 * u < a.rows.rank) load8(a.t + int64_t(row) * a.rows.rank + 32 * c + 8 * u, v);
-        split8(v, hi[u], lo[u]);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) t[u][j] = 0.0f;
+        if (there and 32 * c + 8 * u < a.rows.rank) load8(a.t + int64_t(row) * a.rows.rank + 32 * c + 8 * u, t[u]);
     }
 }
-// A row's line of an A slot: hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8)
-EP_DEVICE void write_t(uint8_t* slot, int row, bool there, const uint4 (&hi)[4], const uint4 (&lo)[4]) {
+// A row's line of an A slot: bf16 hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8)
+EP_DEVICE void write_t(uint8_t* slot, int row, bool there, const float (&t)[4][8]) {
     uint8_t* line = slot + row * 128;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
     #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = there ? hi[u] : zero;
-        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = there ? lo[u] : zero;
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = make_uint4(0, 0, 0, 0);
+        if (there) split8(t[u], hi, lo);
+        *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = hi;
+        *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = lo;
     }
 }
-// Takes infinities and NaN (whole units) out of the part of a V block that the products read: 32 columns of `columns` lines, or
-// (mn_major) 32 lines of each block of 64 columns. 128 threads; true where this thread found one.
-EP_DEVICE bool take_out_non_finite(uint8_t* block, int columns, bool mn_major, int thread) {
-    bool found = false;
-    const auto look = [&](uint8_t* at) {
-        uint4* unit = reinterpret_cast<uint4*>(at);
-        if (has_non_finite(*unit)) *unit = make_uint4(0, 0, 0, 0), found = true;
-    };
-    if (mn_major) {
-        for (int i = thread; i < columns / 64 * 32 * 8; i += 128) look(block + (i / 256) * 8192 + (i % 256) * 16);
-    } else {
-        for (int i = thread; i < columns * 4; i += 128) look(block + (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4));
+// Takes infinities and NaN (whole units) out of the part of a V block of 128 columns that the products read: 32 columns of 128
+// lines, or (mn_major) 32 lines of each of two blocks of 64 columns. 128 threads; true where this thread found one.
+EP_DEVICE bool take_out_non_finite(uint8_t* block, bool mn_major, int thread) {
+    constexpr int kUnits = 4;                 // per thread, read before any of them is looked at
+    uint4* at[kUnits];
+    uint4 unit[kUnits];
+    #pragma unroll
+    for (int q = 0; q < kUnits; ++q) {
+        const int i = thread + q * 128;
+        at[q] = reinterpret_cast<uint4*>(block + (mn_major ? (i / 256) * 8192 + (i % 256) * 16 : (i / 4) * 128 + (((i % 4) ^ ((i / 4) & 7)) << 4)));
+        unit[q] = *at[q];
     }
+    bool found = false;
+    #pragma unroll
+    for (int q = 0; q < kUnits; ++q)
+        if (has_non_finite(unit[q])) *at[q] = make_uint4(0, 0, 0, 0), found = true;
     return found;
 }
 
@@ -614,7 +619,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&grant_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 4);
         for (int i = 0; i < 2; ++i) {
             ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 4);
-            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], 2);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], 6);
         }
         ptx::fence_mbarrier_init();
         error_flag = 0;
@@ -741,32 +746,34 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
             }
             it += kb1 - kb0;
-            // read before the ring has room for it, and once per tile when the rank is not above 32 (with many adapters per tile, a
-            // read per adapter would be a round trip to L2 each)
-            uint4 hi[4], lo[4];
-            if (rank_chunks == 1) read_t(a, m0 + row, mine >= 0, 0, hi, lo);
-            int turn = 0;
-            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e), ++turn) {
-                if (turn % cluster != rank) continue;
-                const bool shared_tile = rows.others_than(e);
-                for (int c = 0; c < rank_chunks and ok; ++c, ++it) {
+            float t[4][8];                    // chunk 0 is read before the ring has room for it
+            read_t(a, m0 + row, mine >= 0, 0, t);
+            ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
+            if (not ok) break;
+            const int size = list_size[slot];
+            // infinities and NaN of an adapter must not meet the zeros of other rows
+            const bool shared_tile = size > 1 or rows.some_without();
+            for (int i = rank; i < size and ok; i += cluster) {
+                const int e = list[slot][i];
+                for (int c = 0; c < rank_chunks; ++c, ++it) {
                     const unsigned s = it % kStages, phase = (it / kStages) & 1;
-                    if (rank_chunks > 1 and mine == e) read_t(a, m0 + row, true, c, hi, lo);
                     ok = wait_all_lanes(&grant_bar[s], (granted >> s) & 1, &error_flag);
                     granted ^= 1u << s;
                     if (not ok) break;
-                    write_t(smem_a + s * kABytes, row, mine == e, hi, lo);
+                    write_t(smem_a + s * kABytes, row, mine == e, t);
+                    if (mine == e and c + 1 < rank_chunks) read_t(a, m0 + row, true, c + 1, t);
                     if (shared_tile) {
-                        // infinities and NaN of this adapter must not meet the zeros of other rows
                         ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
                         if (not ok) break;
-                        if (take_out_non_finite(smem_b + s * kBBytes, BN, a.mn_major, row)) poison[local % kPoisonSlots] = local + 1;
+                        if (take_out_non_finite(smem_b + s * kBBytes, a.mn_major, row)) poison[local % kPoisonSlots] = local + 1;
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
                 }
             }
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
         }
     }
 
@@ -879,7 +886,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&v_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 8);
         for (int i = 0; i < 2; ++i) {
             ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 8);
-            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], leader ? 2 : 1);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], leader ? 6 : 5);
         }
         ptx::fence_mbarrier_init();
         error_flag = 0;
@@ -1017,21 +1024,25 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
             }
             position = (position + blocks) % kStages;
-            uint4 hi[4], lo[4];
-            if (rank_chunks == 1) read_t(a, my_row, mine >= 0, 0, hi, lo);
-            for (int e = rows.next(-1); e != kNone and ok; e = rows.next(e)) {
-                const bool shared_tile = rows.others_than(e);
+            float t[4][8];                    // chunk 0 is read before the ring has room for it
+            read_t(a, my_row, mine >= 0, 0, t);
+            ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
+            if (not ok) break;
+            const int size = list_size[slot];
+            // infinities and NaN of an adapter must not meet the zeros of other rows, in either CTA
+            const bool shared_tile = size > 1 or rows.some_without();
+            for (int i = 0; i < size and ok; ++i) {
+                const int e = list[slot][i];
                 for (int c = 0; c < rank_chunks; ++c) {
                     const int s = position;
                     position = position + 1 == kStages ? 0 : position + 1;
-                    if (rank_chunks > 1 and mine == e) read_t(a, my_row, true, c, hi, lo);
                     // the V block has landed, so the slot is this block's
                     ok = wait_all_lanes(&v_bar[s], (landed >> s) & 1, &error_flag);
                     landed ^= 1u << s;
                     if (not ok) break;
-                    write_t(smem_a + s * kHalf, row, mine == e, hi, lo);
-                    // infinities and NaN of this adapter must not meet the zeros of other rows, in either CTA
-                    if (shared_tile and take_out_non_finite(smem_b + s * kHalf, 128, a.mn_major, row)) {
+                    write_t(smem_a + s * kHalf, row, mine == e, t);
+                    if (mine == e and c + 1 < rank_chunks) read_t(a, my_row, true, c + 1, t);
+                    if (shared_tile and take_out_non_finite(smem_b + s * kHalf, a.mn_major, row)) {
                         for (int q = 0; q < 2; ++q)
                             asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(const_cast<const int*>(&poison[local % kPoisonSlots]), q)), "r"(local + 1) : "memory");
                     }
@@ -1040,6 +1051,8 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     if (lane == 0) tc::mbarrier_arrive_cluster(tc::map_to_cta(&ext_bar[s], 0));
                 }
             }
+            __syncwarp();
+            if (lane == 0) ptx::mbarrier_arrive(&list_empty_bar[slot]);
         }
     } else {
         // ------------------------------------------------------------------ epilogue (both CTAs, own rows)
