@@ -102,7 +102,7 @@ void launch_gemm(LoraGemmArgs args, const void* x, const void* w, int sms, cudaS
     args.cluster = choose_cluster(tiles, math::ceil_div(args.k, kLoraBlockK), 4, sms);
     const int64_t grid = args.cluster > 1 ? tiles * args.cluster : std::min<int64_t>(tiles, sms);
     const auto maps = gemm_maps(args, x, w);
-    launch_kernel_as({grid, 320, kLoraGemmSmemBytes, args.cluster}, lora_gemm_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
+    launch_kernel_as({grid, kLoraGemmThreads, kLoraGemmSmemBytes, args.cluster}, lora_gemm_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
 }
 
 void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, cudaStream_t stream) {
@@ -110,7 +110,7 @@ void launch_gemm_pair(LoraGemmArgs args, const void* x, const void* w, int sms, 
     const int64_t tiles = int64_t(args.m_tiles) * args.n_tiles;
     EP_HOST_ASSERT_MSG(tiles < (int64_t(1) << 30), "too many tiles for one launch");
     const auto maps = gemm_maps(args, x, w);
-    launch_kernel_as({2 * std::min<int64_t>(tiles, sms / 2), 320, kLoraPairSmemBytes, 2}, lora_gemm_pair_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
+    launch_kernel_as({2 * std::min<int64_t>(tiles, sms / 2), kLoraGemmThreads, kLoraPairSmemBytes, 2}, lora_gemm_pair_kernel, stream, maps.x, maps.w, maps.v, maps.y, args);
 }
 
 // Few rows: columns per tile and CTAs per cluster by an estimate of the time. W comes from memory at 6.5 TB/s however it is

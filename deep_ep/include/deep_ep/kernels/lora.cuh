@@ -560,14 +560,15 @@ lora_shrink_rows_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16
 //   warp 0      TMA producer: K blocks of x and W, then the V blocks of the tile's adapters
 //   warp 1      MMA issuer
 //   warps 2-5   epilogue
-//   warps 6-9   writers: the A operand of the adapters' K blocks (t as bf16 hi | lo, zeros in the rows of others)
+//   warps 6-13  writers: the A operand of the adapters' K blocks (t as bf16 hi | lo, zeros in the rows of others), two groups that
+//               take the blocks in turn: one block takes a group about as long as three take the tensor cores
 // Many tiles: persistent CTAs, two accumulators in tensor memory, so that the stores of one tile overlap the products of the
 // next. Few tiles (decode): a cluster shares the tile's contraction, so that all SMs pull on W; its CTAs send their parts
 // of a row to the CTA that owns the row, which adds them in rank order.
-constexpr int kLoraGemmColumns = 128, kLoraGemmStages = 5;
+constexpr int kLoraGemmColumns = 128, kLoraGemmStages = 5, kLoraGemmThreads = 448;
 constexpr int kLoraGemmSmemBytes = kLoraGemmStages * (kLoraTileRows + kLoraGemmColumns) * kLoraBlockK * 2 + kLoraTileRows * kLoraGemmColumns * 4 + 1024;
 
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(kLoraGemmThreads, 1)
 lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_y, const __grid_constant__ LoraGemmArgs a) {
     using namespace lora_detail;
@@ -575,7 +576,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     constexpr int BN = kLoraGemmColumns, kStages = kLoraGemmStages, kGroupM = 16;
     constexpr uint32_t kABytes = kLoraTileRows * kLoraBlockK * 2, kBBytes = BN * kLoraBlockK * 2;
     constexpr int kPoisonSlots = 8;           // more tiles than the writers can be ahead of the epilogue
-    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], grant_bar[kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], grant_bar[2][kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
     __shared__ uint64_t list_full_bar[2], list_empty_bar[2];
     __shared__ int list[2][kLoraTileRows], list_size[2];       // the adapters of a tile
     __shared__ uint32_t tmem_slot;
@@ -616,10 +617,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s)
-            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&grant_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 4);
+            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&grant_bar[0][s], 1), ptx::mbarrier_init(&grant_bar[1][s], 1), ptx::mbarrier_init(&ext_bar[s], 4);
         for (int i = 0; i < 2; ++i) {
             ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 4);
-            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], 6);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], 10);
         }
         ptx::fence_mbarrier_init();
         error_flag = 0;
@@ -637,6 +638,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         // ------------------------------------------------------------------ TMA producer
         Ring ring;
         int issued = 0, local = 0;
+        unsigned ext = 0;                     // adapters' blocks so far
         bool ok = true;
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
             int m0, n0;
@@ -658,7 +660,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     if (not ok) break;
                     if (elect_one()) {
                         uint64_t* bar = &full_bar[ring.slot];
-                        ptx::mbarrier_arrive(&grant_bar[ring.slot]);    // the writers may fill the A slot
+                        ptx::mbarrier_arrive(&grant_bar[ext & 1][ring.slot]);    // the writers may fill the A slot
                         ptx::mbarrier_arrive_expect_tx(bar, kBBytes);
                         uint8_t* sb = smem_b + ring.slot * kBBytes;
                         if (a.mn_major) {
@@ -669,7 +671,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                             for (int j = 0; j < BN / 128; ++j) tc::tma_load_3d(sb + j * 16384, &map_v, 32 * c, n0 + 128 * j, e, bar);
                         }
                     }
-                    ++issued, ring.advance(kStages);
+                    ++issued, ++ext, ring.advance(kStages);
                 }
             }
             __syncwarp();
@@ -723,10 +725,12 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     } else if (warp >= 6) {
         // ------------------------------------------------------------------ writers of the adapters' A operand
         cudaGridDependencySynchronize();      // t comes from the kernel before, which this one does not wait for until here
-        const int row = threadIdx.x - 192;
+        const int row = (threadIdx.x - 192) & 127;
+        const unsigned group = (warp - 6) / 4;
         // These warps do not follow the ring through the K blocks of x, so they cannot tell from a slot's own barriers (which
-        // show a phase's parity only) whether it is free for THIS block: the producer, which can, grants it.
-        unsigned it = 0, granted = 0;
+        // show a phase's parity only) whether it is free for THIS block: the producer, which can, grants it (on barriers of the
+        // group's own, of which it thus misses no phase).
+        unsigned it = 0, ext = 0, granted = 0;
         int local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
@@ -746,8 +750,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                 if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
             }
             it += kb1 - kb0;
-            float t[4][8];                    // chunk 0 is read before the ring has room for it
-            read_t(a, m0 + row, mine >= 0, 0, t);
+            // this group's first chunk of the row's t (exact when the chunks are even in number) is read before the ring has room for it
+            int held = rank_chunks % 2 == 0 and (ext & 1) != group ? 1 : 0;
+            float t[4][8];
+            read_t(a, m0 + row, mine >= 0, held, t);
             ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
             if (not ok) break;
             const int size = list_size[slot];
@@ -755,13 +761,15 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             const bool shared_tile = size > 1 or rows.some_without();
             for (int i = rank; i < size and ok; i += cluster) {
                 const int e = list[slot][i];
-                for (int c = 0; c < rank_chunks; ++c, ++it) {
+                for (int c = 0; c < rank_chunks; ++c, ++it, ++ext) {
+                    if ((ext & 1) != group) continue;
                     const unsigned s = it % kStages, phase = (it / kStages) & 1;
-                    ok = wait_all_lanes(&grant_bar[s], (granted >> s) & 1, &error_flag);
+                    if (mine == e and held != c) read_t(a, m0 + row, true, c, t);
+                    ok = wait_all_lanes(&grant_bar[group][s], (granted >> s) & 1, &error_flag);
                     granted ^= 1u << s;
                     if (not ok) break;
                     write_t(smem_a + s * kABytes, row, mine == e, t);
-                    if (mine == e and c + 1 < rank_chunks) read_t(a, m0 + row, true, c + 1, t);
+                    if (mine == e and c + 2 < rank_chunks) held = c + 2, read_t(a, m0 + row, true, held, t);
                     if (shared_tile) {
                         ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
                         if (not ok) break;
@@ -822,7 +830,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         bool fix = false;
         for (int q = 0; q < cluster; ++q) fix = fix or ld_cluster_int(tc::map_to_cta(const_cast<const int*>(&poison[0]), q)) != 0;
         if (fix) cudaGridDependencySynchronize();
-        for (int item = threadIdx.x; item < share * (BN / 8); item += 320) {
+        for (int item = threadIdx.x; item < share * (BN / 8); item += kLoraGemmThreads) {
             const int row = rank * share + item / (BN / 8), c = item % (BN / 8) * 8;
             if (m0 + row >= a.rows.num_rows or n0 + c >= a.n) continue;
             float v[8] = {};
@@ -852,14 +860,14 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 constexpr int kLoraPairStages = 6;
 constexpr int kLoraPairSmemBytes = kLoraPairStages * 2 * 128 * kLoraBlockK * 2 + 4 * 4096 + 1024;
 
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(kLoraGemmThreads, 1)
 lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ CUtensorMap map_y, const __grid_constant__ LoraGemmArgs a) {
     using namespace lora_detail;
     extern __shared__ uint8_t smem_raw[];
     constexpr int kStages = kLoraPairStages, kGroupM = 8, kPoisonSlots = 8;
     constexpr uint32_t kHalf = 128 * kLoraBlockK * 2;          // 128 rows of A, or 128 columns of B: 16 KB
-    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], v_bar[kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], v_bar[2][kStages], ext_bar[kStages], tmem_full_bar[2], tmem_empty_bar[2];
     __shared__ uint64_t list_full_bar[2], list_empty_bar[2];
     __shared__ int list[2][2 * kLoraTileRows], list_size[2];
     __shared__ uint32_t tmem_slot;
@@ -883,10 +891,10 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s)
-            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&v_bar[s], 1), ptx::mbarrier_init(&ext_bar[s], 8);
+            ptx::mbarrier_init(&full_bar[s], 1), ptx::mbarrier_init(&empty_bar[s], 1), ptx::mbarrier_init(&v_bar[0][s], 1), ptx::mbarrier_init(&v_bar[1][s], 1), ptx::mbarrier_init(&ext_bar[s], 8);
         for (int i = 0; i < 2; ++i) {
             ptx::mbarrier_init(&tmem_full_bar[i], 1), ptx::mbarrier_init(&tmem_empty_bar[i], 8);
-            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], leader ? 6 : 5);
+            ptx::mbarrier_init(&list_full_bar[i], 1), ptx::mbarrier_init(&list_empty_bar[i], leader ? 10 : 9);
         }
         ptx::fence_mbarrier_init();
         error_flag = 0;
@@ -905,6 +913,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         // ------------------------------------------------------------------ TMA producer (both CTAs)
         Ring ring;
         int issued = 0, local = 0;
+        unsigned ext = 0;                     // adapters' blocks so far
         bool ok = true;
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
             int m0, n0;
@@ -939,7 +948,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     ok = wait_all_lanes(&empty_bar[ring.slot], ring.phase ^ 1, &error_flag);
                     if (not ok) break;
                     if (elect_one()) {
-                        uint64_t* bar = &v_bar[ring.slot];
+                        uint64_t* bar = &v_bar[ext & 1][ring.slot];
                         ptx::mbarrier_arrive_expect_tx(bar, kHalf);
                         uint8_t* sb = smem_b + ring.slot * kHalf;
                         if (a.mn_major) {
@@ -949,7 +958,7 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                             tc::tma_load_3d(sb, &map_v, 32 * c, n_half, e, bar);
                         }
                     }
-                    ++issued, ring.advance(kStages);
+                    ++issued, ++ext, ring.advance(kStages);
                 }
             }
             __syncwarp();
@@ -1003,8 +1012,9 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     } else if (warp >= 6) {
         // ------------------------------------------------------------------ writers of the adapters' A operand (both CTAs, own rows)
         cudaGridDependencySynchronize();      // t comes from the kernel before, which this one does not wait for until here
-        const int row = threadIdx.x - 192;
-        unsigned landed = 0;                  // per slot: parity of the next V block
+        const int row = (threadIdx.x - 192) & 127;
+        const unsigned group = (warp - 6) / 4;
+        unsigned landed = 0, ext = 0;         // per slot: parity of this group's next V block; blocks so far
         int position = 0, local = 0;          // position in the ring
         bool ok = true;
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
@@ -1024,8 +1034,10 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                 if (lane == 0) ptx::mbarrier_arrive(&list_full_bar[slot]);
             }
             position = (position + blocks) % kStages;
-            float t[4][8];                    // chunk 0 is read before the ring has room for it
-            read_t(a, my_row, mine >= 0, 0, t);
+            // this group's first chunk of the row's t (exact when the chunks are even in number) is read before the ring has room for it
+            int held = rank_chunks % 2 == 0 and (ext & 1) != group ? 1 : 0;
+            float t[4][8];
+            read_t(a, my_row, mine >= 0, held, t);
             ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
             if (not ok) break;
             const int size = list_size[slot];
@@ -1033,20 +1045,22 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             const bool shared_tile = size > 1 or rows.some_without();
             for (int i = 0; i < size and ok; ++i) {
                 const int e = list[slot][i];
-                for (int c = 0; c < rank_chunks; ++c) {
+                for (int c = 0; c < rank_chunks; ++c, ++ext) {
                     const int s = position;
                     position = position + 1 == kStages ? 0 : position + 1;
+                    if ((ext & 1) != group) continue;
+                    if (mine == e and held != c) read_t(a, my_row, true, c, t);
                     // the V block has landed, so the slot is this block's
-                    ok = wait_all_lanes(&v_bar[s], (landed >> s) & 1, &error_flag);
+                    ok = wait_all_lanes(&v_bar[group][s], (landed >> s) & 1, &error_flag);
                     landed ^= 1u << s;
                     if (not ok) break;
                     write_t(smem_a + s * kHalf, row, mine == e, t);
-                    if (mine == e and c + 1 < rank_chunks) read_t(a, my_row, true, c + 1, t);
+                    if (mine == e and c + 2 < rank_chunks) held = c + 2, read_t(a, my_row, true, held, t);
                     if (shared_tile and take_out_non_finite(smem_b + s * kHalf, a.mn_major, row)) {
                         for (int q = 0; q < 2; ++q)
                             asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(const_cast<const int*>(&poison[local % kPoisonSlots]), q)), "r"(local + 1) : "memory");
                     }
-                    ptx::fence_proxy_async();
+                    ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) tc::mbarrier_arrive_cluster(tc::map_to_cta(&ext_bar[s], 0));
                 }
