@@ -34,19 +34,18 @@ int choose_cluster(int64_t units, int blocks, int least, int sms) {
 constexpr int64_t kRingBytes = 192 * 1024;
 // Up to this many products of x A^T, the kernel without tensor cores is ahead: its time is that of reading rows * rank * k
 // elements of A from L2, the other's starts at what setting up a tile costs. Measured (it | tensor cores, us): forward as a
-// whole, K 7168, N 4096: one row of rank 16 16.4 | 16.5, 16 rows of rank 64 20.8 | 24.0, 96 of rank 32 (2^24.4) 30.8 | 38.4, 64 of
-// rank 64 (2^24.8) 32.0 | 30.2. With the rank contiguous (backward) it reads A in pieces of eight bytes; alone, K 7168: 64 rows of
-// rank 8 (2^21.8) 6.8 | 9.6, 4 of rank 128 (2^21.8) 10.3 | 10.3, 16 of rank 64 (2^22.8) 17.1 | 9.6.
-constexpr int64_t kFewProducts = int64_t(1) << 25, kFewProductsRankContiguous = int64_t(1) << 22;
+// whole, K 7168, N 4096, 8 adapters: 16 rows of rank 16 17.4 | 24.0, 96 of rank 32 (2^24.4) 27.4 | 27.9, 64 of rank 64 (2^24.8)
+// 30.2 | 28.7, 128 of rank 64 (2^25.8) 36.4 | 30.2. With the rank contiguous (backward) it reads A in pieces of eight bytes; alone,
+// K 7168: 64 rows of rank 8 (2^21.8) 6.8 | 9.6, 4 of rank 128 (2^21.8) 10.3 | 10.3, 16 of rank 64 (2^22.8) 17.1 | 9.6.
+constexpr int64_t kFewProducts = int64_t(3) << 23, kFewProductsRankContiguous = int64_t(1) << 22;
 
-// One row tile: the low-rank term is computed beside the shared product's stream of W while it has few elements of t, or few
-// for the blocks that the tensor cores would need (one per adapter that occurs). Measured with K 7168, N 4096 (beside the
-// stream | tensor cores, us): 8 adapters of rank 16: 64 rows 21.2 | 24.7, 128 rows 24.6 | 26.6; 64 adapters of rank 16: 128 rows
-// 27.3 | 44.6; 16 adapters of rank 32: 64 rows 28.7 | 28.5, 128 rows 37.1 | 33.5; 8 adapters of rank 128: 16 rows 30.8 | 31.2, 32 rows
-// 47.2 | 36.4.
+// One row tile: the low-rank term is computed beside the shared product's stream of W while it has few elements of t, more of
+// them when each reads little of V. Measured with K 7168, N 4096 (beside the stream | tensor cores, us): 8 adapters of rank 16:
+// 64 rows 21.4 | 24.0, 128 rows 24.8 | 26.0; 64 adapters of rank 16: 128 rows 28.4 | 33.3; 8 of rank 32: 32 rows 20.8 | 24.0, 64 rows
+// 27.4 | 25.3; 64 of rank 32: 32 rows 24.7 | 27.2, 64 rows 36.3 | 31.0; 8 of rank 64: 16 rows 21.9 | 23.9, 32 rows 30.2 | 26.1.
 bool few_terms(const LoraRows& r) {
-    const int64_t terms = int64_t(r.num_rows) * r.rank, blocks = int64_t(std::min(r.num_adapters, r.num_rows)) * r.rank;
-    return r.num_rows <= kLoraTileRows and terms <= std::max<int64_t>(1536, 3 * blocks);
+    const int64_t terms = int64_t(r.num_rows) * r.rank;
+    return r.num_rows <= kLoraTileRows and (terms <= 1024 or terms * r.rank <= 32768);
 }
 
 }  // namespace
@@ -153,7 +152,7 @@ void lora_gemm(LoraGemmArgs args, const void* x, const void* w, cudaStream_t str
     const int sms = device_sms();
     if (few_terms(args.rows) and launch_gemm_few(args, x, w, sms, stream)) return;
     // A wave of 256 x 256 tiles by pairs of CTAs takes about 1.5 times as long as one of 128 x 128 tiles by single ones. Measured
-    // with K 4096, N 4096, rank 16 (pairs | single, us): 512 rows 37.9 | 31.0, 768 39.6 | 42.6, 1280 63.7 | 67.6, 8192 221 | 293.
+    // with K 4096, N 4096, rank 16 (pairs | single, us): 512 rows 37.8 | 31.5, 768 38.0 | 41.0, 1280 60.5 | 64.4, 8192 209 | 300.
     const int64_t rows = args.rows.num_rows;
     const int64_t tiles = math::ceil_div<int64_t>(rows, kLoraTileRows) * math::ceil_div(args.n, kLoraGemmColumns);
     const int64_t pair_tiles = math::ceil_div<int64_t>(rows, 2 * kLoraTileRows) * math::ceil_div(args.n, 256);
