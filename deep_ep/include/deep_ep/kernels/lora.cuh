@@ -14,9 +14,11 @@
 // t enters the tensor cores as two bf16 numbers (its rounding and the rest), which keeps 16 of its bits: the low-rank
 // product is as exact as its bf16 operands allow, at twice a cost that is a few percent of the shared product.
 //
-// Zeros do not hide infinities or NaN (0 * inf = NaN). lora_gemm therefore looks for them in the adapter's block whenever a
-// tile holds other rows too, takes them out of the tensor cores' operand, and adds their products to the owner's rows
-// separately; lora_wgrad overwrites the rows of other requests with zeros. One request cannot poison another.
+// Neither zeros nor a sum of two parts hide infinities or NaN (0 * inf = NaN, and so is hi * inf + lo * inf where lo is zero or of
+// the other sign). lora_gemm therefore takes them out of both operands of an adapter's block and adds their products, in fp32, to the
+// owner's rows; lora_wgrad overwrites the rows of other requests with zeros, and where the sum of hi's products is not finite that is
+// the result. One request cannot poison another, and its own results are infinite or NaN where the formulas say so, whoever
+// shares its tile.
 #pragma once
 
 #include "../device/sync.cuh"
@@ -41,15 +43,10 @@ template <int kRows>
 struct TileAdapters {
     static constexpr int kPer = kRows / 32;
     int id[kPer];
-    bool inside[kPer];
 
     EP_DEVICE void load(const LoraRows& r, int m0, int lane) {
         #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int row = m0 + lane + 32 * i;
-            inside[i] = row < r.num_rows;
-            id[i] = adapter_of(r, row);
-        }
+        for (int i = 0; i < kPer; ++i) id[i] = adapter_of(r, m0 + lane + 32 * i);
     }
     EP_DEVICE int next(int last) const {
         unsigned best = kNone;
@@ -57,13 +54,6 @@ struct TileAdapters {
         for (int i = 0; i < kPer; ++i)
             if (id[i] > last) best = min(best, static_cast<unsigned>(id[i]));
         return static_cast<int>(__reduce_min_sync(0xffffffffu, best));
-    }
-    // some row of the batch in this tile has no adapter
-    EP_DEVICE bool some_without() const {
-        bool without = false;
-        #pragma unroll
-        for (int i = 0; i < kPer; ++i) without = without or (inside[i] and id[i] < 0);
-        return __any_sync(0xffffffffu, without);
     }
 };
 
@@ -75,19 +65,28 @@ EP_DEVICE bool has_non_finite(const uint4& u) {
     return bad;
 }
 
-// v = hi + lo with both bf16 (an infinite or NaN v has no rest)
-EP_DEVICE void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+// v can be written as hi + lo with both bf16: not if it is infinite, NaN, or rounds to infinity
+EP_DEVICE bool splits(float v) { return isfinite(__bfloat162float(__float2bfloat16_rn(v))); }
+// v = hi + lo. What cannot be split has no lo, and with kTakeOut no hi either; true where there is such a value.
+template <bool kTakeOut>
+EP_DEVICE bool split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = ptx::float2_to_bf16x2(a, b);
     const float2 h = ptx::bf16x2_to_float2(hi);
     const float ra = a - h.x, rb = b - h.y;
-    lo = ptx::float2_to_bf16x2(isfinite(ra) ? ra : 0.0f, isfinite(rb) ? rb : 0.0f);
+    const bool fa = isfinite(ra), fb = isfinite(rb);           // exactly where `splits` is true
+    lo = ptx::float2_to_bf16x2(fa ? ra : 0.0f, fb ? rb : 0.0f);
+    if (kTakeOut) hi &= (fa ? 0x0000ffffu : 0u) | (fb ? 0xffff0000u : 0u);
+    return not (fa and fb);
 }
 // eight values -> one 16-byte unit each of hi and lo
-EP_DEVICE void split8(const float (&v)[8], uint4& hi, uint4& lo) {
+template <bool kTakeOut>
+EP_DEVICE bool split8(const float (&v)[8], uint4& hi, uint4& lo) {
     uint32_t h[4], l[4];
+    bool found = false;
     #pragma unroll
-    for (int i = 0; i < 4; ++i) split2(v[2 * i], v[2 * i + 1], h[i], l[i]);
+    for (int i = 0; i < 4; ++i) found |= split2<kTakeOut>(v[2 * i], v[2 * i + 1], h[i], l[i]);
     hi = make_uint4(h[0], h[1], h[2], h[3]), lo = make_uint4(l[0], l[1], l[2], l[3]);
+    return found;
 }
 EP_DEVICE void load8(const float* p, float (&v)[8]) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
@@ -110,8 +109,8 @@ EP_DEVICE int ld_cluster_int(uint32_t addr) {
     return v;
 }
 
-// Product of a row's t with what the writers have kept from the tensor cores at column n: infinities and NaN of the row's adapter,
-// by whole units of eight V elements
+// Products of a row's t and its adapter's V at column n that the writers have kept from the tensor cores: those of t that cannot be
+// split, and of units of eight V elements with an infinity or NaN
 __device__ __noinline__ float poisoned(const LoraGemmArgs& a, int row, int n) {
     const int e = adapter_of(a.rows, row);
     if (e < 0) return 0.0f;
@@ -121,13 +120,14 @@ __device__ __noinline__ float poisoned(const LoraGemmArgs& a, int row, int n) {
     if (a.mn_major) {
         for (int r = 0; r < a.rows.rank; ++r) {
             const __nv_bfloat16* unit = v + int64_t(r) * a.n + (n & ~7);
-            if (has_non_finite(*reinterpret_cast<const uint4*>(unit))) sum += t[r] * __bfloat162float(unit[n & 7]);
+            if (not splits(t[r]) or has_non_finite(*reinterpret_cast<const uint4*>(unit))) sum += t[r] * __bfloat162float(unit[n & 7]);
         }
     } else {
         for (int r = 0; r < a.rows.rank; r += 8) {
             const __nv_bfloat16* unit = v + int64_t(n) * a.rows.rank + r;
-            if (has_non_finite(*reinterpret_cast<const uint4*>(unit)))
-                for (int j = 0; j < 8; ++j) sum += t[r + j] * __bfloat162float(unit[j]);
+            const bool whole = has_non_finite(*reinterpret_cast<const uint4*>(unit));
+            for (int j = 0; j < 8; ++j)
+                if (whole or not splits(t[r + j])) sum += t[r + j] * __bfloat162float(unit[j]);
         }
     }
     return sum;
@@ -143,16 +143,19 @@ EP_DEVICE void read_t(const LoraGemmArgs& a, int row, bool there, int c, float (
         if (there and 32 * c + 8 * u < a.rows.rank) load8(a.t + int64_t(row) * a.rows.rank + 32 * c + 8 * u, t[u]);
     }
 }
-// A row's line of an A slot: bf16 hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8)
-EP_DEVICE void write_t(uint8_t* slot, int row, bool there, const float (&t)[4][8]) {
+// A row's line of an A slot: bf16 hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8).
+// True where the row has a t that cannot be split, which is written as zero.
+EP_DEVICE bool write_t(uint8_t* slot, int row, bool there, const float (&t)[4][8]) {
     uint8_t* line = slot + row * 128;
+    bool found = false;
     #pragma unroll
     for (int u = 0; u < 4; ++u) {
         uint4 hi = make_uint4(0, 0, 0, 0), lo = make_uint4(0, 0, 0, 0);
-        if (there) split8(t[u], hi, lo);
+        if (there) found |= split8<true>(t[u], hi, lo);
         *reinterpret_cast<uint4*>(line + ((u ^ (row & 7)) << 4)) = hi;
         *reinterpret_cast<uint4*>(line + (((4 + u) ^ (row & 7)) << 4)) = lo;
     }
+    return found;
 }
 // Takes infinities and NaN (whole units) out of the part of a V block of 128 columns that the products read: 32 columns of 128
 // lines, or (mn_major) 32 lines of each of two blocks of 64 columns. 128 threads; true where this thread found one.
@@ -737,11 +740,11 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
             int m0, n0;
             origin(tile, m0, n0);
-            TileAdapters<kLoraTileRows> rows;
-            rows.load(a.rows, m0, lane);
             const int mine = adapter_of(a.rows, m0 + row), slot = local & 1;
             if (warp == 6) {
                 // the tile's adapters for the producer and the MMA issuer
+                TileAdapters<kLoraTileRows> rows;
+                rows.load(a.rows, m0, lane);
                 ok = wait_all_lanes(&list_empty_bar[slot], ((local >> 1) & 1) ^ 1, &error_flag);
                 int size = 0;
                 for (int e = rows.next(-1); e != kNone; e = rows.next(e), ++size)
@@ -758,8 +761,6 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
             if (not ok) break;
             const int size = list_size[slot];
-            // infinities and NaN of an adapter must not meet the zeros of other rows
-            const bool shared_tile = size > 1 or rows.some_without();
             for (int i = rank; i < size and ok; i += cluster) {
                 const int e = list[slot][i];
                 for (int c = 0; c < rank_chunks; ++c, ++it, ++ext) {
@@ -769,13 +770,12 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
                     ok = wait_all_lanes(&grant_bar[group][s], (granted >> s) & 1, &error_flag);
                     granted ^= 1u << s;
                     if (not ok) break;
-                    write_t(smem_a + s * kABytes, row, mine == e, t);
+                    bool found = write_t(smem_a + s * kABytes, row, mine == e, t);
                     if (mine == e and c + 2 < rank_chunks) held = c + 2, read_t(a, m0 + row, true, held, t);
-                    if (shared_tile) {
-                        ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
-                        if (not ok) break;
-                        if (take_out_non_finite(smem_b + s * kBBytes, a.mn_major, row)) poison[local % kPoisonSlots] = local + 1;
-                    }
+                    ok = wait_all_lanes(&full_bar[s], phase, &error_flag);
+                    if (not ok) break;
+                    found |= take_out_non_finite(smem_b + s * kBBytes, a.mn_major, row);
+                    if (found) poison[local % kPoisonSlots] = local + 1;
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) ptx::mbarrier_arrive(&ext_bar[s]);
@@ -1021,11 +1021,11 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
         for (int tile = first_tile; tile < num_tiles and ok; tile += tile_step, ++local) {
             int m0, n0;
             origin(tile, m0, n0);
-            TileAdapters<2 * kLoraTileRows> rows;
-            rows.load(a.rows, m0, lane);
             const int my_row = m0 + 128 * half + row, mine = adapter_of(a.rows, my_row), slot = local & 1;
             if (warp == 6) {
                 // the adapters of the pair's 256 rows, for the producer and the MMA issuer
+                TileAdapters<2 * kLoraTileRows> rows;
+                rows.load(a.rows, m0, lane);
                 ok = wait_all_lanes(&list_empty_bar[slot], ((local >> 1) & 1) ^ 1, &error_flag);
                 int size = 0;
                 for (int e = rows.next(-1); e != kNone; e = rows.next(e), ++size)
@@ -1042,8 +1042,6 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             ok = wait_all_lanes(&list_full_bar[slot], (local >> 1) & 1, &error_flag);
             if (not ok) break;
             const int size = list_size[slot];
-            // infinities and NaN of an adapter must not meet the zeros of other rows, in either CTA
-            const bool shared_tile = size > 1 or rows.some_without();
             for (int i = 0; i < size and ok; ++i) {
                 const int e = list[slot][i];
                 for (int c = 0; c < rank_chunks; ++c, ++ext) {
@@ -1055,9 +1053,10 @@ lora_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     ok = wait_all_lanes(&v_bar[group][s], (landed >> s) & 1, &error_flag);
                     landed ^= 1u << s;
                     if (not ok) break;
-                    write_t(smem_a + s * kHalf, row, mine == e, t);
+                    // a row's t concerns this CTA's accumulator, a column of V both
+                    if (write_t(smem_a + s * kHalf, row, mine == e, t)) poison[local % kPoisonSlots] = local + 1;
                     if (mine == e and c + 2 < rank_chunks) held = c + 2, read_t(a, my_row, true, held, t);
-                    if (shared_tile and take_out_non_finite(smem_b + s * kHalf, a.mn_major, row)) {
+                    if (take_out_non_finite(smem_b + s * kHalf, a.mn_major, row)) {
                         for (int q = 0; q < 2; ++q)
                             asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(tc::map_to_cta(const_cast<const int*>(&poison[local % kPoisonSlots]), q)), "r"(local + 1) : "memory");
                     }
@@ -1427,7 +1426,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
                 const int r = 8 * (2 * i + side);
-                if (r < a.rows.rank) split8(values[i], *place(r), *place(half + r));
+                if (r < a.rows.rank) split8<false>(values[i], *place(r), *place(half + r));
             }
             // rows of other requests in this block: zeros instead of whatever they hold (0 * inf would be NaN)
             const bool foreign = not second_mine and second + line < a.rows.num_rows;
@@ -1479,6 +1478,11 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             tc::fence_after_thread_sync();
             const int quarter = warp & 3;
             float* part = reinterpret_cast<float*>(smem);
+            // an infinity or NaN of X shows in hi's products as in those of t itself, lo's products with it have another sign or are NaN
+            const auto sum = [](uint32_t hi, uint32_t lo) {
+                const float h = __uint_as_float(hi);
+                return isfinite(h) ? h + __uint_as_float(lo) : h;
+            };
             for (int m = 0; m < 2; ++m) {
                 float* out = part + (m * 128 + quarter * 32 + lane) * pitch;
                 for (int c = 0; c < a.rows.rank; c += 16) {
@@ -1490,9 +1494,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (count > 0)
-                            v = make_float4(__uint_as_float(r[i]) + __uint_as_float(q[i]), __uint_as_float(r[i + 1]) + __uint_as_float(q[i + 1]),
-                                            __uint_as_float(r[i + 2]) + __uint_as_float(q[i + 2]), __uint_as_float(r[i + 3]) + __uint_as_float(q[i + 3]));
+                        if (count > 0) v = make_float4(sum(r[i], q[i]), sum(r[i + 1], q[i + 1]), sum(r[i + 2], q[i + 2]), sum(r[i + 3], q[i + 3]));
                         *reinterpret_cast<float4*>(out + c + i) = v;
                     }
                 }
