@@ -18,10 +18,36 @@ from .grouped_gemm import MODE_WGRAD, _pairs
 __all__ = ['lora_linear']
 
 
+class _Widened(torch.autograd.Function):
+    """`t.float()` of an adapter matrix. Its gradient is added to the matrix's `main_grad`, if it has one by then, as on the GPU."""
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(t):
+        return t.float()
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.parameter, = inputs
+
+    @staticmethod
+    def backward(ctx, grad):
+        main_grad = getattr(ctx.parameter, 'main_grad', None)
+        if main_grad is None:
+            return grad.to(ctx.parameter.dtype)
+        with torch.no_grad():
+            main_grad.add_(grad)
+
+    @staticmethod
+    def jvp(ctx, tangent):
+        return tangent.float()
+
+
 def _reference(x, w, lora_a, lora_b, idx, scaling):
     """Plain form in fp32 (CPU): rows are picked by adapter, so one adapter's values never meet another's rows."""
     dtype = x.dtype
-    x, w, lora_a, lora_b = x.float(), w.float(), lora_a.float(), lora_b.float()      # once: their gradients are summed in fp32 too
+    # once: their gradients are summed in fp32 too
+    x, w, lora_a, lora_b = x.float(), w.float(), _Widened.apply(lora_a), _Widened.apply(lora_b)
     y = x @ w.t()
     for e in range(lora_a.size(0)):
         rows = torch.nonzero(idx == e).flatten()          # (an adapter without rows gets a gradient of zeros, as on the GPU)
@@ -39,9 +65,10 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     ranks with zero rows). Both products accumulate in fp32; the intermediate `x A^T` keeps 16 bits; `y` is rounded once.
 
     Gradients reach `x`, `lora_a` and `lora_b` (or their fp32 `main_grad`), and `w` if it wants one (K and N multiples of
-    128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to, whose results are
-    infinite or NaN as the formulas say. The adapters' gradients read a row tile of 128 once per adapter that occurs in it, so long training batches are best ordered by adapter.
-    A backward pass may be captured in a CUDA graph when no eager autograd graph of the same leaves is alive.
+    128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to, whose
+    results are infinite or NaN as the formulas say. The adapters' gradients read a row tile of 128 once per adapter that occurs
+    in it, so long training batches are best ordered by adapter. A backward pass may be captured in a CUDA graph when no eager
+    autograd graph of the same leaves is alive.
     """
     if x.is_cuda:
         # (the native call looks at every argument, and is the autograd node where a gradient is wanted)

@@ -1,0 +1,47 @@
+"""Weight gradients that go to a parameter's fp32 `main_grad` buffer, on the CPU as on the GPU."""
+import pytest
+import torch
+
+from deep_ep.ops.lora import lora_linear
+from test_lora import U, check, make, reference
+
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+
+
+def test_adapters_on_the_cpu():
+    x, w, a, b, dy, idx, s = make(37, 48, 24, 6, 3, 'cpu')
+    leaves = [t.clone().requires_grad_() for t in (w, a, b)]
+    for t in leaves[1:]:
+        t.main_grad = torch.zeros_like(t, dtype=torch.float32)
+    for _ in range(2):
+        lora_linear(x, *leaves, idx, s).backward(dy)
+    assert leaves[1].grad is None and leaves[2].grad is None and leaves[0].grad is not None
+    refs, bounds = reference(x, w, a, b, dy, idx, s)
+    check(leaves[1].main_grad, 2 * refs[2], 2 * bounds[2], 2 * U)
+    check(leaves[2].main_grad, 2 * refs[3], 2 * bounds[3], 2 * U)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_one_adapter_matrix_with_a_buffer(device):
+    """A with a buffer, B without: each where it belongs, and the same bits as without any."""
+    x, w, a, b, dy, idx, s = make(50, 64, 32, 8, 3, device)
+    plain = [t.clone().requires_grad_() for t in (x, a, b)]
+    y = lora_linear(plain[0], w, plain[1], plain[2], idx, s)
+    y.backward(dy)
+    mixed = [t.clone().requires_grad_() for t in (x, a, b)]
+    mixed[1].main_grad = torch.zeros_like(a, dtype=torch.float32)
+    z = lora_linear(mixed[0], w, mixed[1], mixed[2], idx, s)
+    z.backward(dy)
+    assert torch.equal(y, z) and torch.equal(plain[0].grad, mixed[0].grad) and torch.equal(plain[2].grad, mixed[2].grad)
+    assert mixed[1].grad is None and torch.equal(mixed[1].main_grad.to(torch.bfloat16), plain[1].grad)
+
+
+def test_cpu_adapters_without_a_buffer_can_be_differentiated_twice_and_forward():
+    x, w, a, b, dy, idx, s = make(9, 16, 8, 8, 2, 'cpu')
+    leaves = [t.clone().requires_grad_() for t in (a, b)]
+    y = lora_linear(x, w, *leaves, idx, s)
+    da, = torch.autograd.grad(y, leaves[0], dy, create_graph=True)
+    assert torch.autograd.grad(da.float().square().sum(), leaves[1])[0].any()
+    with torch.autograd.forward_ad.dual_level():
+        y = lora_linear(x, w, torch.autograd.forward_ad.make_dual(a, torch.ones_like(a)), b, idx, s)
+        assert torch.autograd.forward_ad.unpack_dual(y).tangent.any()
