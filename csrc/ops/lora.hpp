@@ -141,6 +141,8 @@ public:
                                  const torch::Tensor& b, const torch::Tensor& idx, const torch::Tensor& scaling, bool pairs) {
         auto [y, t] = lora_forward(x, w, a, b, idx, scaling);
         ctx->save_for_backward({x, w, a, b, idx, scaling, t});
+        // the parameters themselves, for their `main_grad`: what a hook on saved tensors (checkpointing) gives back is another tensor
+        ctx->saved_data["a"] = a, ctx->saved_data["b"] = b;
         ctx->saved_data["pairs"] = pairs;
         return y;
     }
@@ -156,7 +158,8 @@ public:
             const auto dy = operand(grads[0].to(torch::kBFloat16), 2, x);
             const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_a = ctx->needs_input_grad(2), want_b = ctx->needs_input_grad(3);
             // gradient of A or B; added to the parameter's buffer where it has one
-            const auto adapter_grad = [&](const torch::Tensor& rows, const torch::Tensor& low, const torch::Tensor& presence, const torch::Tensor& parameter, bool rank_major) {
+            const auto adapter_grad = [&](const torch::Tensor& rows, const torch::Tensor& low, const torch::Tensor& presence, const char* name, bool rank_major) {
+                const auto parameter = ctx->saved_data[name].toTensor();
                 const auto buffer = main_grad(parameter);
                 const auto result = buffer.has_value() ? *buffer : torch::empty_like(parameter, parameter.options(), torch::MemoryFormat::Contiguous);
                 lora_wgrad(rows, low, idx, presence, result, rank_major, buffer.has_value());
@@ -165,8 +168,8 @@ public:
             if (want_x or want_a or want_b) {
                 const auto [dt, presence, dx] = lora_backward(dy, w, a, b, idx, scaling, want_x);
                 if (want_x) out[0] = *dx;
-                if (want_a) out[2] = adapter_grad(x, dt, presence, a, true);
-                if (want_b) out[3] = adapter_grad(dy, t, presence, b, false);
+                if (want_a) out[2] = adapter_grad(x, dt, presence, "a", true);
+                if (want_b) out[3] = adapter_grad(dy, t, presence, "b", false);
             }
             if (want_w) out[1] = dense_weight_grad(dy, operand(x, 2, x), w, ctx->saved_data["pairs"].toBool());
         }

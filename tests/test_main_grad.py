@@ -1,7 +1,10 @@
-"""Weight gradients that go to a parameter's fp32 `main_grad` buffer, on the CPU as on the GPU."""
+"""Weight gradients that go to a parameter's fp32 `main_grad` buffer: on the CPU as on the GPU, also when the forward pass is
+checkpointed or its saved tensors are stored elsewhere (a hook hands the backward pass other tensors than the parameters then)."""
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
+from deep_ep.ops.embedding import embedding_lookup
 from deep_ep.ops.lora import lora_linear
 from test_lora import U, check, make, reference
 
@@ -45,3 +48,44 @@ def test_cpu_adapters_without_a_buffer_can_be_differentiated_twice_and_forward()
     with torch.autograd.forward_ad.dual_level():
         y = lora_linear(x, w, torch.autograd.forward_ad.make_dual(a, torch.ones_like(a)), b, idx, s)
         assert torch.autograd.forward_ad.unpack_dual(y).tangent.any()
+
+
+# ------------------------------------------------------------------------------------------------ hooks on saved tensors
+def embedding_case(device):
+    table = torch.randn(50, 16, device=device).to(torch.bfloat16)
+    ids, dy = torch.randint(0, 50, (40,), device=device), torch.randn(40, 16, device=device).to(torch.bfloat16)
+    return [table], lambda p: embedding_lookup(p[0], ids, 2.0), dy
+
+
+def adapter_case(device):
+    x, w, a, b, dy, idx, s = make(150, 64, 128, 16, 3, device)
+    return [a, b], lambda p: lora_linear(x, w, p[0], p[1], idx, s), dy
+
+
+CASES = [(embedding_case, ()), (adapter_case, ())]
+
+
+@pytest.mark.parametrize('how', ['checkpoint', 'hooks'])
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('case,args', CASES)
+def test_under_saved_tensor_hooks(device, case, args, how):
+    torch.manual_seed(0)
+    values, forward, dy = case(device, *args)
+
+    def run(wrapped):
+        leaves = [v.clone().requires_grad_() for v in values]
+        for t in leaves:
+            t.main_grad = torch.zeros_like(t, dtype=torch.float32)
+        if not wrapped:
+            y = forward(leaves)
+        elif how == 'checkpoint':
+            y = checkpoint(lambda *p: forward(p), *leaves, use_reentrant=False)
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t):
+                y = forward(leaves)
+        y.backward(dy)
+        assert all(t.grad is None for t in leaves)
+        return [t.main_grad for t in leaves]
+
+    for plain, hooked in zip(run(False), run(True)):
+        assert plain.any() and torch.equal(plain, hooked)
