@@ -133,7 +133,7 @@ class GroupedSwiGLUFFNFp8(torch.autograd.Function):
         y = fp8_gemm(act_q, act_sf, w2_q, w2_sf, psum, count, alignment, route=route)
         ctx.save_for_backward(x, w_gate_up, w_down, row_scale, psum, count, h, act)
         ctx.transposed = (w1t_q, w1t_sf, w2t_q, w2t_sf)
-        ctx.alignment, ctx.backward_route = alignment, backward_route
+        ctx.weights, ctx.alignment, ctx.backward_route = (w_gate_up, w_down), alignment, backward_route
         return y
 
     @staticmethod
@@ -145,7 +145,7 @@ class GroupedSwiGLUFFNFp8(torch.autograd.Function):
         dy = dy.contiguous()
         dy_q, dy_sf = row_quant(dy)
         dact = fp8_gemm(dy_q, dy_sf, w2t_q, w2t_sf, psum, count, ctx.alignment)
-        dw_down = _wgrad(dy, act, w_down, psum, count, wgrad_alignment) if ctx.needs_input_grad[2] else None
+        dw_down = _wgrad(dy, act, ctx.weights[1], psum, count, wgrad_alignment) if ctx.needs_input_grad[2] else None
         d_row_scale = row_scale_grad(dact, act, row_scale) if row_scale is not None and ctx.needs_input_grad[3] else None
         dh = _swiglu_backward(h, dact, row_scale)
         dx = None
@@ -156,7 +156,7 @@ class GroupedSwiGLUFFNFp8(torch.autograd.Function):
                 barrier()
             dh_q, dh_sf = row_quant(dh)
             dx = fp8_gemm(dh_q, dh_sf, w1t_q, w1t_sf, psum, count, ctx.alignment, route=table)
-        dw_gate_up = _wgrad(dh, x, w_gate_up, psum, count, wgrad_alignment) if ctx.needs_input_grad[1] else None
+        dw_gate_up = _wgrad(dh, x, ctx.weights[0], psum, count, wgrad_alignment) if ctx.needs_input_grad[1] else None
         return dx, dw_gate_up, dw_down, d_row_scale, None, None, None, None, None, None
 
 

@@ -62,7 +62,8 @@ def grouped_gemm_dgrad(dy: torch.Tensor, w: torch.Tensor, psum: torch.Tensor, co
 
 
 def _wgrad(dy, x, w, psum, count, alignment):
-    """Weight gradient of one grouped linear layer, honouring a persistent fp32 `main_grad` buffer on the parameter."""
+    """Weight gradient of one grouped linear layer, honouring a persistent fp32 `main_grad` buffer on the parameter `w`: the
+    parameter itself, since a hook on saved tensors (checkpointing) gives the backward pass another tensor."""
     main_grad = getattr(w, 'main_grad', None)
     if alignment % 64 == 0:
         # fp32 accumulation happens in tensor memory; without a persistent fp32 buffer the result is rounded once and
@@ -100,7 +101,7 @@ class GroupedSwiGLUFFN(torch.autograd.Function):
         # with `route`, rows that are their token's only one leave this GEMM for the owner's combine landing slot
         y = grouped_gemm_forward(act, w_down, psum, count, alignment=alignment, route=route)
         ctx.save_for_backward(x, w_gate_up, w_down, row_scale, psum, count, h, act)
-        ctx.alignment = alignment
+        ctx.weights, ctx.alignment = (w_gate_up, w_down), alignment
         # `backward_route = (table, barrier)`: the data-gradient GEMM of the first layer feeds the combine that is the
         # backward of dispatch, so it can deliver single-row tokens the same way; `barrier()` is called right before it
         ctx.backward_route = backward_route
@@ -111,7 +112,7 @@ class GroupedSwiGLUFFN(torch.autograd.Function):
         x, w_gate_up, w_down, row_scale, psum, count, h, act = ctx.saved_tensors
         dy = dy.contiguous()
         dact = grouped_gemm_dgrad(dy, w_down, psum, count, alignment=ctx.alignment)
-        dw_down = _wgrad(dy, act, w_down, psum, count, ctx.alignment) if ctx.needs_input_grad[2] else None
+        dw_down = _wgrad(dy, act, ctx.weights[1], psum, count, ctx.alignment) if ctx.needs_input_grad[2] else None
         d_row_scale = row_scale_grad(dact, act, row_scale) if row_scale is not None and ctx.needs_input_grad[3] else None
         dh = _C.swiglu_backward(h, dact, row_scale)
         dx = None
@@ -121,7 +122,7 @@ class GroupedSwiGLUFFN(torch.autograd.Function):
                 table, barrier = ctx.backward_route
                 barrier()
             dx = grouped_gemm_dgrad(dh, w_gate_up, psum, count, alignment=ctx.alignment, route=table)
-        dw_gate_up = _wgrad(dh, x, w_gate_up, psum, count, ctx.alignment) if ctx.needs_input_grad[1] else None
+        dw_gate_up = _wgrad(dh, x, ctx.weights[0], psum, count, ctx.alignment) if ctx.needs_input_grad[1] else None
         return dx, dw_gate_up, dw_down, d_row_scale, None, None, None, None, None
 
 
@@ -156,7 +157,7 @@ class GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, psum, count, alignment):
         ctx.save_for_backward(x, w, psum, count)
-        ctx.alignment = alignment
+        ctx.weight, ctx.alignment = w, alignment
         # the alignment reaches the kernels so that the padding rows of every expert's region are written as zeros: the
         # tensor-core weight-gradient GEMM reads whole 64-row blocks, padding included
         return grouped_gemm_forward(x, w, psum, count, alignment=alignment)
@@ -166,7 +167,7 @@ class GroupedLinear(torch.autograd.Function):
         x, w, psum, count = ctx.saved_tensors
         dy = dy.contiguous()
         dx = grouped_gemm_dgrad(dy, w, psum, count, alignment=ctx.alignment) if ctx.needs_input_grad[0] else None
-        dw = _wgrad(_zero_padding_rows(dy, psum, count, ctx.alignment), x, w, psum, count, ctx.alignment) \
+        dw = _wgrad(_zero_padding_rows(dy, psum, count, ctx.alignment), x, ctx.weight, psum, count, ctx.alignment) \
             if ctx.needs_input_grad[1] else None
         return dx, dw, None, None, None
 

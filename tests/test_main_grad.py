@@ -6,6 +6,7 @@ from torch.utils.checkpoint import checkpoint
 
 from deep_ep.ops.embedding import embedding_lookup
 from deep_ep.ops.lora import lora_linear
+from test_grouped_gemm_gpu import make_layout
 from test_lora import U, check, make, reference
 
 DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
@@ -62,12 +63,35 @@ def adapter_case(device):
     return [a, b], lambda p: lora_linear(x, w, p[0], p[1], idx, s), dy
 
 
-CASES = [(embedding_case, ()), (adapter_case, ())]
+def grouped_linear_case(device):
+    from deep_ep.ops.grouped_gemm import GroupedLinear
+    psum, count, rows, _ = make_layout([100, 0, 37], 128, torch.device(device))
+    x, w = torch.randn(rows, 256, device=device).to(torch.bfloat16), (torch.randn(3, 128, 256, device=device) * 0.06).to(torch.bfloat16)
+    dy = torch.randn(rows, 128, device=device).to(torch.bfloat16)
+    return [w], lambda p: GroupedLinear.apply(x, p[0], psum, count, 128), dy
+
+
+def ffn_case(device, fp8):
+    from deep_ep.ops.fp8_training import Fp8WeightCache, grouped_swiglu_ffn_fp8_training
+    from deep_ep.ops.grouped_gemm import grouped_swiglu_ffn
+    psum, count, rows, starts = make_layout([100, 0, 37], 128, torch.device(device))
+    x, dy = (torch.zeros(rows, 512, dtype=torch.bfloat16, device=device) for _ in range(2))
+    for start, c in zip(starts, [100, 0, 37]):
+        x[start:start + c], dy[start:start + c] = torch.randn(c, 512).to(device), torch.randn(c, 512).to(device)
+    w1, w2 = ((torch.randn(*shape) * 0.05).to(torch.bfloat16).to(device) for shape in ((3, 1024, 512), (3, 512, 512)))
+    cache = Fp8WeightCache()
+    if fp8:
+        return [w1, w2], lambda p: grouped_swiglu_ffn_fp8_training(x, *p, psum, count, 128, cache), dy
+    return [w1, w2], lambda p: grouped_swiglu_ffn(x, *p, psum, count, None, 128), dy
+
+
+CASES = [('cpu', embedding_case, ()), ('cpu', adapter_case, ()), ('cpu', ffn_case, (True,))] + [
+    pytest.param('cuda', *c, marks=pytest.mark.gpu) for c in ((embedding_case, ()), (adapter_case, ()), (grouped_linear_case, ()),
+                                                              (ffn_case, (False,)), (ffn_case, (True,)))]
 
 
 @pytest.mark.parametrize('how', ['checkpoint', 'hooks'])
-@pytest.mark.parametrize('device', DEVICES)
-@pytest.mark.parametrize('case,args', CASES)
+@pytest.mark.parametrize('device,case,args', CASES)
 def test_under_saved_tensor_hooks(device, case, args, how):
     torch.manual_seed(0)
     values, forward, dy = case(device, *args)
