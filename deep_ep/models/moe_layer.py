@@ -163,13 +163,14 @@ class MoELayer(nn.Module):
     def clip_grad_norm_(self, max_norm: float) -> torch.Tensor:
         """Clip the layer's gradients in place by their global norm and return the norm (fp32 scalar on the device).
 
-        Expert gradients (the fp32 `main_grad` of a weight that has one, else its `.grad`) differ from rank to rank, and their
-        squares are added over the layer's group; those of the router and the shared expert are the same on every rank once they
-        have been reduced, which comes before this call, and count once. Collective over the group when it has several ranks."""
+        Expert gradients differ from rank to rank, and their squares are added over the layer's group; those of the router and the
+        shared expert are the same on every rank once they have been reduced, which comes before this call, and count once.
+        A parameter's gradient is its `.grad`; without one it is the fp32 `main_grad` (where the grouped expert kernels leave it, as
+        may a training loop that empties `.grad` into such buffers). Collective over the group when it has several ranks."""
         from ..ops.grad_norm import clip_grad_norm_
         def gradients(names):
             found = [getattr(self, name, None) for name in names]
-            found = [getattr(p, 'main_grad', None) if getattr(p, 'main_grad', None) is not None else p.grad for p in found if p is not None]
+            found = [p.grad if p.grad is not None else getattr(p, 'main_grad', None) for p in found if p is not None]
             return [g for g in found if g is not None]
         # (an empty tensor keeps the collective on the layer's device when no expert has a gradient yet)
         experts = gradients(('w_gate_up', 'w_down')) or [torch.empty(0, device=self.w_gate_up.device)]

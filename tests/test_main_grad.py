@@ -1,11 +1,16 @@
 """Weight gradients that go to a parameter's fp32 `main_grad` buffer: on the CPU as on the GPU, also when the forward pass is
-checkpointed or its saved tensors are stored elsewhere (a hook hands the backward pass other tensors than the parameters then)."""
+checkpointed or its saved tensors are stored elsewhere (a hook hands the backward pass other tensors than the parameters then),
+and clipping of a layer whose parameters carry such buffers."""
+import math
+
 import pytest
 import torch
+import torch.distributed as dist
 from torch.utils.checkpoint import checkpoint
 
 from deep_ep.ops.embedding import embedding_lookup
 from deep_ep.ops.lora import lora_linear
+from dist_utils import run_distributed
 from test_grouped_gemm_gpu import make_layout
 from test_lora import U, check, make, reference
 
@@ -113,3 +118,70 @@ def test_under_saved_tensor_hooks(device, case, args, how):
 
     for plain, hooked in zip(run(False), run(True)):
         assert plain.any() and torch.equal(plain, hooked)
+
+
+# ------------------------------------------------------------------------------------------------ the layer's clipping
+def _clip_worker(rank, world, device):
+    from deep_ep.models.moe_layer import MoEConfig, MoELayer
+    torch.manual_seed(3)
+    cfg = MoEConfig(hidden=128, intermediate=128, num_experts=8 if device == 'cpu' else 128, num_topk=2, num_shared_experts=1,
+                    num_max_tokens_per_rank=64, expert_alignment=16 if device == 'cpu' else 128,
+                    expert_backend='torch' if device == 'cpu' else 'grouped')
+    layer = MoELayer(dist.group.WORLD, cfg, device=torch.device(device))
+    experts, others = [layer.w_gate_up, layer.w_down], [layer.gate, layer.shared_gate_up, layer.shared_down]
+
+    def step(stale):
+        """Gradients of one step, every parameter with a buffer; those that no kernel adds to hold `stale`."""
+        for p in experts + others:
+            p.grad, p.main_grad = None, torch.full_like(p, 0.0 if p is layer.w_gate_up or p is layer.w_down else stale, dtype=torch.float32)
+        torch.manual_seed(10 + rank)
+        layer(torch.randn(64, 128, device=device).to(torch.bfloat16)).float().square().mean().backward()
+
+    def norm_of(sharded, replicated):
+        squares = torch.stack([g.double().square().sum() for g in sharded]).sum()
+        if world > 1:
+            dist.all_reduce(squares)
+        return math.sqrt(float(squares) + sum(float(g.double().square().sum()) for g in replicated))
+
+    def clipped(grads, call, ref):
+        before = [g.clone() for g in grads]
+        assert abs(float(call()) - ref) <= 1e-6 * ref
+        for g, o in zip(grads, before):
+            assert o.any() and torch.allclose(g.double(), o.double() * (ref / 2 / (ref + 1e-6)), rtol=torch.finfo(g.dtype).eps + 1e-6, atol=1e-30)
+
+    step(1e3)
+    for p in others:
+        assert p.grad is not None
+        if world > 1:
+            mean = p.grad.float()
+            dist.all_reduce(mean)
+            p.grad.copy_(mean / world)
+    # the kernels add the experts' gradients to their buffers, plain torch operations leave them in `.grad`
+    held = [p.grad if device == 'cpu' else p.main_grad for p in experts]
+    assert all((p.grad is None) == (device != 'cpu') for p in experts)
+    plain = [p.grad for p in others]
+    ref = norm_of(held, plain)
+    clipped(held + plain, lambda: layer.clip_grad_norm_(ref / 2), ref)
+    assert all((p.main_grad == 1e3).all() for p in others)
+    # a training loop that moves every gradient into its buffer
+    step(0.0)
+    for p in experts + others:
+        if p.grad is not None:
+            p.main_grad.add_(p.grad)
+            p.grad = None
+    if world > 1:
+        for p in others:
+            dist.all_reduce(p.main_grad)
+    ref = norm_of([p.main_grad for p in experts], [p.main_grad for p in others])
+    clipped([p.main_grad for p in experts + others], lambda: layer.clip_grad_norm_(ref / 2), ref)
+    layer.destroy()
+
+
+@pytest.mark.parametrize('world', [1, 2])
+def test_layer_clipping_with_buffers_on_cpu_ranks(world, master_port):
+    run_distributed(_clip_worker, world, master_port, 'gloo', args=('cpu',), timeout_s=180)
+
+
+@pytest.mark.gpu
+def test_layer_clipping_with_buffers_on_the_gpu(master_port):
+    run_distributed(_clip_worker, 1, master_port, 'nccl', args=('cuda',), timeout_s=180)
