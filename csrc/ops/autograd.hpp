@@ -33,4 +33,9 @@ inline void refuse_second_derivatives(torch::autograd::variable_list& grads, con
     }
 }
 
+// The kernels carry no tangents; a tensor that has one is refused rather than answered without its derivative
+inline void refuse_tangent(const torch::Tensor& t) {
+    EP_HOST_ASSERT_MSG(not t._fw_grad(0).defined(), "no forward-mode differentiation on the GPU");
+}
+
 }  // namespace deep_ep::ops

@@ -77,6 +77,7 @@ inline torch::Tensor embedding_grad(const torch::Tensor& dy_in, const torch::Ten
     const auto idx = idx_in.contiguous();
     const auto out = out_in.has_value() ? *out_in : torch::empty({rows, dy.size(1)}, dy.options());
     check_rows(dy), check_rows(out), check_ids(idx, dy);
+    refuse_tangent(dy_in), refuse_tangent(out);
     EP_HOST_ASSERT_MSG(out.size(0) == rows, "out is [num_rows, hidden]");
     EP_HOST_ASSERT_MSG(out.device() == dy.device(), "all tensors of a call lie on one device");
     EP_HOST_ASSERT_MSG(dy.size(0) == idx.numel() and dy.size(1) == out.size(1), "dy is [number of indices, hidden], out [rows, hidden]");
@@ -151,6 +152,7 @@ public:
 };
 
 inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale, const std::optional<torch::Tensor>& table_sf) {
+    refuse_tangent(table);
     if (not at::GradMode::is_enabled() or not table.requires_grad() or table_sf.has_value()) return lookup_rows(table, idx, scale, table_sf);
     return EmbeddingLookup::apply(table, idx, scale);
 }

@@ -13,6 +13,7 @@
 #include <deep_ep/common/exception.hpp>
 
 #include "../kernels/api.hpp"
+#include "autograd.hpp"
 
 namespace deep_ep::ops {
 
@@ -62,6 +63,7 @@ inline std::vector<launch::GradTensor> gradient_list(const TensorList& grads, co
             const auto& o = (*outs)[i];
             EP_HOST_ASSERT_MSG(o.device() == device and o.sizes() == g.sizes() and o.is_non_overlapping_and_dense() and
                                (o.strides() == g.strides() or g.numel() <= 1), "an output has its gradient's shape, strides and device");
+            refuse_tangent(g), refuse_tangent(o);
             t.out = o.data_ptr(), t.out_type = gradient_type(o);
             const auto out_begin = reinterpret_cast<uintptr_t>(t.out);
             if (t.numel > 0) {

@@ -186,6 +186,7 @@ inline torch::Tensor lora_linear(const torch::Tensor& x, const torch::Tensor& w,
     const auto idx = idx_in.contiguous();
     const auto s = scalings.has_value() ? *scalings : torch::full({a.size(0)}, scaling, x.options().dtype(torch::kFloat32).requires_grad(false));
     EP_HOST_ASSERT_MSG(not s.requires_grad(), "scaling receives no gradient");
+    for (const auto* t : {&x, &w, &a, &b, &s}) refuse_tangent(*t);
     if (not at::GradMode::is_enabled() or not (x.requires_grad() or w.requires_grad() or a.requires_grad() or b.requires_grad()))
         return std::get<0>(lora_forward(x, w, a, b, idx, s));
     EP_HOST_ASSERT_MSG(not w.requires_grad() or (w.dim() == 2 and w.size(0) % 128 == 0 and w.size(1) % 128 == 0), "the gradient of w needs K and N to be multiples of 128");
