@@ -17,6 +17,7 @@ Everything also runs on CPU tensors through a plain PyTorch emulation of the sam
 fp32, round to bf16): that is the oracle of the GPU tests and what the CPU tests exercise.
 The reference contains no matrix math; this follows the usage the layer is meant for (`README.md:178-194` there).
 """
+import weakref
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -63,19 +64,25 @@ def block_quant(w: torch.Tensor, transposed: bool = False):
 
 
 class Fp8WeightCache:
-    """Quantised copies (forward and transposed) of weight stacks, refreshed when a parameter's version changes."""
+    """Quantised copies (forward and transposed) of weight stacks, refreshed when a parameter's version changes. An entry belongs to
+    the tensor object that it was made from: a new tensor may have the `id`, version and address of one that is gone."""
 
     def __init__(self):
-        self._entries: Dict[int, Tuple[int, int, tuple]] = {}
+        self._entries: Dict[int, Tuple[weakref.ref, int, int, tuple]] = {}
 
     def get(self, w: torch.Tensor) -> tuple:
         key = id(w)
         entry = self._entries.get(key)
-        if entry is None or entry[0] != w._version or entry[1] != w.data_ptr():
+        if entry is None or entry[0]() is not w or entry[1] != w._version or entry[2] != w.data_ptr():
+            for gone in [k for k, e in self._entries.items() if e[0]() is None]:
+                del self._entries[gone]
             with torch.no_grad():
-                entry = (w._version, w.data_ptr(), block_quant(w.detach(), transposed=True))
+                entry = (weakref.ref(w), w._version, w.data_ptr(), block_quant(w.detach(), transposed=True))
             self._entries[key] = entry
-        return entry[2]
+        return entry[3]
+
+    def __getstate__(self):
+        return {'_entries': {}}          # (a copy has other tensors)
 
     def clear(self) -> None:
         self._entries.clear()
