@@ -38,4 +38,10 @@ inline void refuse_tangent(const torch::Tensor& t) {
     EP_HOST_ASSERT_MSG(not t._fw_grad(0).defined(), "no forward-mode differentiation on the GPU");
 }
 
+// A kernel has written (or, for clipping within the limit, may write) the tensor: as after a torch operation in place, a graph that has
+// saved it refuses to go back. (Inference tensors have no version.)
+inline void mark_written(const torch::Tensor& t) {
+    if (not t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace deep_ep::ops

@@ -99,6 +99,7 @@ inline torch::Tensor embedding_grad(const torch::Tensor& dy_in, const torch::Ten
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
     const int num_tokens = static_cast<int>(idx.numel()), num_rows = static_cast<int>(out.size(0)), hidden = static_cast<int>(out.size(1));
     if (num_rows == 0 or hidden == 0) return out;
+    if (out_in.has_value()) mark_written(out);
 
     kernels::EmbGradArgs g = {};
     g.dy = dy.data_ptr(), g.dy_stride = dy.stride(0);

@@ -126,6 +126,8 @@ inline torch::Tensor grad_clip(const pybind11::object& grads, const pybind11::ob
     kernels::GradClipArgs args = {total.data_ptr<double>(), static_cast<int>(total.numel()), static_cast<float>(max_norm),
                                   norm.data_ptr<float>(), not results.has_value()};
     launch::grad_clip(list, args, c10::cuda::getCurrentCUDAStream());
+    const TensorList& written = results.has_value() ? *results : tensors;
+    for (size_t i = 0; i < written.size(); ++i) mark_written(written[i]);
     return norm;
 }
 

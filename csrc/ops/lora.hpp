@@ -116,6 +116,7 @@ inline void lora_wgrad(const torch::Tensor& x_in, const torch::Tensor& t_in, con
         if (not accumulate) out.zero_();
         return;
     }
+    mark_written(out);
     args.m = static_cast<int>(m), args.rank_major = rank_major;
     args.t = t.data_ptr<float>(), args.presence = presence.data_ptr<uint8_t>();
     args.d = out.data_ptr(), args.out_fp32 = out.scalar_type() == torch::kFloat32, args.accumulate = accumulate;
