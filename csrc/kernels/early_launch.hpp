@@ -16,8 +16,12 @@ struct LaunchShape {
 };
 
 // `early` kernels wait themselves (`cudaGridDependencySynchronize`) before they touch anything that earlier work in the stream
-// reads or writes. A kernel lets the next one begin (`cudaTriggerProgrammaticLaunchCompletion`) only after its own such wait,
-// unless the next one waits for it before doing anything at all.
+// reads or writes. A kernel lets the next one begin (`cudaTriggerProgrammaticLaunchCompletion`) only after its own such wait: the next
+// one may be any kernel, and its wait is for this one.
+// One exception: the products of lora.cuh load x and W before they wait. That is sound only behind a kernel that writes neither and
+// keeps this rule, or is not early at all: when the product begins, that kernel has waited, so whatever made x and W is done.
+// lora_shrink and its form for a few rows are launched directly before them; torch may put a fill of y in between. They write nothing
+// before the wait: every accumulator waits for the list of its tile's adapters, or for t, and the warps that bring those have waited.
 template <typename... Params, typename... Args>
 void launch_kernel_as(const LaunchShape& shape, void (*kernel)(Params...), cudaStream_t stream, const Args&... args) {
     EP_HOST_ASSERT_MSG(shape.grid > 0 and shape.grid < (int64_t(1) << 31), "too many tiles for one launch");

@@ -50,8 +50,8 @@ inline torch::Tensor lora_shrink(const torch::Tensor& x, const torch::Tensor& a,
 }
 
 // y = x . W^T + t . V_e^T; `transposed`: W is [k, n] and V [adapters, rank, n] (the data gradient), else [n, k] and [adapters, n, rank].
-// Its kernel begins beside the one before it in the stream and waits for nothing but t: that one has to be `lora_shrink`'s,
-// with no other launch (a copy of an operand, say) in between.
+// Its kernel begins beside the one before it in the stream and loads x and W before it waits (see early_launch.hpp): that one has to
+// be `lora_shrink`'s, with no launch that writes x or W (a copy of an operand, say) in between.
 inline torch::Tensor lora_gemm_after_shrink(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& t, const torch::Tensor& v,
                                             const torch::Tensor& idx, bool transposed) {
     const int64_t k = x.size(1), n = transposed ? w.size(1) : w.size(0), rank = t.size(1);

@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(const __grid_con
     using namespace emb_detail;
     constexpr int kAhead = kAccumulate ? 4 : 8;
     const int lane = ptx::lane_id();
-    cudaTriggerProgrammaticLaunchCompletion();                  // the join kernel may be set up meanwhile
     cudaGridDependencySynchronize();                            // the sort is done
+    cudaTriggerProgrammaticLaunchCompletion();                  // the join kernel, or whatever comes next, may be set up meanwhile
     const unsigned slices = math::ceil_div(unsigned(a.hidden), 32u * kElems * kPacks);
     const int64_t item = int64_t(blockIdx.x) * 8 + threadIdx.x / 32, sum_items = int64_t(a.num_chunks) * slices;
     if (item >= sum_items) {
