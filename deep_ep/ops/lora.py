@@ -8,7 +8,7 @@ occur: a call can be captured in a CUDA graph and replayed with other indices.
 
 CPU tensors take the same formulas in plain torch.
 """
-from typing import Optional, Union
+from typing import Union
 
 import torch
 
@@ -56,7 +56,7 @@ def _reference(x, w, lora_a, lora_b, idx, scaling):
 
 
 def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter_idx: torch.Tensor,
-                scaling: Optional[Union[float, torch.Tensor]] = 1.0) -> torch.Tensor:
+                scaling: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """`x @ w.T + scaling[e] * (x @ lora_a[e].T) @ lora_b[e].T` per row, bf16 `[rows, N]`.
 
     `x [rows, K]`, `w [N, K]`, `lora_a [adapters, rank, K]`, `lora_b [adapters, N, rank]`, all bf16; `adapter_idx [rows]`
