@@ -33,6 +33,13 @@ inline void refuse_second_derivatives(torch::autograd::variable_list& grads, con
     }
 }
 
+// Fake tensors and subclasses that wrap other tensors say that they lie on a GPU and have no memory there: a kernel would be given
+// address zero
+inline void check_memory(const void* data, int64_t numel) {
+    EP_HOST_ASSERT_MSG(data != nullptr or numel == 0, "a tensor without memory of its own (fake, or a wrapper of others)");
+}
+inline void check_memory(const torch::Tensor& t) { check_memory(t.const_data_ptr(), t.numel()); }
+
 // The kernels carry no tangents; a tensor that has one is refused rather than answered without its derivative
 inline void refuse_tangent(const torch::Tensor& t) {
     EP_HOST_ASSERT_MSG(not t._fw_grad(0).defined(), "no forward-mode differentiation on the GPU");

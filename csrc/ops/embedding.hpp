@@ -30,12 +30,14 @@ inline kernels::EmbType embedding_type(const torch::Tensor& t) {
 inline void check_rows(const torch::Tensor& t) {
     EP_HOST_ASSERT_MSG(t.is_cuda() and t.dim() == 2 and (t.size(1) <= 1 or t.stride(1) == 1) and t.stride(0) >= 0,
                        "a CUDA matrix with contiguous columns is needed");
+    check_memory(t);
 }
 
 inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
     EP_HOST_ASSERT_MSG(idx.is_contiguous() and (idx.scalar_type() == torch::kInt64 or idx.scalar_type() == torch::kInt32),
                        "indices are contiguous int64 or int32");
     EP_HOST_ASSERT_MSG(idx.device() == with.device(), "all tensors of a call lie on one device");
+    check_memory(idx);
 }
 
 // [*idx.shape, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)

@@ -58,6 +58,7 @@ inline std::vector<launch::GradTensor> gradient_list(const TensorList& grads, co
         EP_HOST_ASSERT_MSG(g.is_cuda() and g.device() == device, "gradients lie on one CUDA device");
         EP_HOST_ASSERT_MSG(g.is_non_overlapping_and_dense(), "gradients are dense (no gaps, no element twice)");
         launch::GradTensor t = {g.const_data_ptr(), nullptr, g.numel(), gradient_type(g), gradient_type(g)};
+        check_memory(t.in, t.numel);
         const auto begin = reinterpret_cast<uintptr_t>(t.in);
         if (outs != nullptr) {
             const auto& o = (*outs)[i];
@@ -65,6 +66,7 @@ inline std::vector<launch::GradTensor> gradient_list(const TensorList& grads, co
                                (o.strides() == g.strides() or g.numel() <= 1), "an output has its gradient's shape, strides and device");
             refuse_tangent(g), refuse_tangent(o);
             t.out = o.data_ptr(), t.out_type = gradient_type(o);
+            check_memory(t.out, t.numel);
             const auto out_begin = reinterpret_cast<uintptr_t>(t.out);
             if (t.numel > 0) {
                 ranges.push_back({out_begin, out_begin + o.nbytes(), true});

@@ -22,6 +22,7 @@ inline torch::Tensor operand(const torch::Tensor& t, int dims, const torch::Tens
     EP_HOST_ASSERT_MSG(t.device() == with.device(), "all tensors of a call lie on one device");
     for (int i = 0; i < dims; ++i) EP_HOST_ASSERT_MSG(t.size(i) <= std::numeric_limits<int>::max() / 2, "sizes above 2^30");
     const auto c = t.contiguous();
+    check_memory(c);
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
@@ -103,6 +104,7 @@ inline void lora_wgrad(const torch::Tensor& x_in, const torch::Tensor& t_in, con
     const c10::cuda::OptionalCUDAGuard guard(x_in.is_cuda() ? std::optional(x_in.device()) : std::nullopt);
     const auto x = operand(x_in, 2, x_in), t = operand(t_in, 2, x_in, torch::kFloat32);
     EP_HOST_ASSERT_MSG(out.device() == x.device() and out.dim() == 3 and out.is_contiguous(), "a contiguous result on the operands' device");
+    check_memory(out);
     EP_HOST_ASSERT_MSG(presence.device() == x.device() and presence.dim() == 2 and presence.is_contiguous() and presence.scalar_type() == torch::kUInt8, "presence of `lora_shrink`");
     const int64_t rank = t.size(1), m = x.size(1);
     EP_HOST_ASSERT_MSG(t.size(0) == x.size(0) and m >= 8 and m % 8 == 0, "one t per row, columns a multiple of 8");
@@ -183,6 +185,7 @@ public:
 inline torch::Tensor lora_linear(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& idx_in,
                                  double scaling, const std::optional<torch::Tensor>& scalings, bool pairs) {
     EP_HOST_ASSERT_MSG(x.is_cuda() and a.dim() == 3 and idx_in.dim() == 1, "x is a CUDA matrix, a [adapters, rank, K], adapter indices [rows]");
+    for (const auto* t : {&x, &w, &a, &b, &idx_in}) check_memory(*t);
     const c10::cuda::CUDAGuard guard(x.device());
     const auto idx = idx_in.contiguous();
     const auto s = scalings.has_value() ? *scalings : torch::full({a.size(0)}, scaling, x.options().dtype(torch::kFloat32).requires_grad(false));
