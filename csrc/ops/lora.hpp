@@ -193,6 +193,7 @@ inline torch::Tensor lora_linear(const torch::Tensor& x, const torch::Tensor& w,
     for (const auto* t : {&x, &w, &a, &b, &s}) refuse_tangent(*t);
     if (not at::GradMode::is_enabled() or not (x.requires_grad() or w.requires_grad() or a.requires_grad() or b.requires_grad()))
         return std::get<0>(lora_forward(x, w, a, b, idx, s));
+    EP_HOST_ASSERT_MSG(not (a.requires_grad() or b.requires_grad()) or x.size(0) <= kernels::kLoraMaxGradRows, "gradients of a and b take up to 2^23 rows");
     EP_HOST_ASSERT_MSG(not w.requires_grad() or (w.dim() == 2 and w.size(0) % 128 == 0 and w.size(1) % 128 == 0), "the gradient of w needs K and N to be multiples of 128");
     return LoraLinear::apply(x, w, a, b, idx, s, pairs);
 }

@@ -1316,7 +1316,6 @@ lora_gemm_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 // 7168 columns: 22 / 25 / 69 us at rank 16 / 32 / 128 (one register set, copied from block to block: 28 / 32 / 66 us; one group that
 // read both when it needed them: 1.4 us per block). Rows in another order cost each adapter the row tiles in which it occurs.
 constexpr int kLoraWgradColumns = 256;
-constexpr int kLoraMaxTileWords = 2048;       // bitmap of row tiles: 2048 * 32 tiles of 128 rows
 
 // kUnits: units of eight rank columns per writer thread (two threads share a row)
 template <int kUnits>

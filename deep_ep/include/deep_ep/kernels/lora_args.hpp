@@ -9,6 +9,8 @@ constexpr int kLoraTileRows = 128;        // token rows of a tile
 constexpr int kLoraBlockK = 64;           // 64 bf16 = one 128-byte swizzle row
 constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxCluster = 8;
+constexpr int kLoraMaxTileWords = 2048;   // gradients of A and B: bitmap of row tiles ...
+constexpr int64_t kLoraMaxGradRows = int64_t(kLoraMaxTileWords) * 32 * kLoraTileRows;        // ... which bounds the rows, 2^23
 
 // Which adapter a row belongs to. An id outside [0, num_adapters) means none.
 struct LoraRows {

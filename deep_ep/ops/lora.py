@@ -67,7 +67,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     Gradients reach `x`, `lora_a` and `lora_b` (or their fp32 `main_grad`), and `w` if it wants one (K and N multiples of
     128 then). Infinities or NaN in a request's rows or adapter stay with the rows and adapter they belong to, whose
     results are infinite or NaN as the formulas say. The adapters' gradients read a row tile of 128 once per adapter that occurs
-    in it, so long training batches are best ordered by adapter. A backward pass may be captured in a CUDA graph when no eager
+    in it, so long training batches are best ordered by adapter; they take up to 2^23 rows. A backward pass may be captured in a CUDA graph when no eager
     autograd graph of the same leaves is alive.
     """
     if x.is_cuda:
