@@ -40,6 +40,8 @@ inline void check_ids(const torch::Tensor& idx, const torch::Tensor& with) {
     check_memory(idx);
 }
 
+constexpr int64_t kEmbMaxGradSize = std::numeric_limits<int>::max() / 2;         // rows, columns and tokens of a gradient
+
 // [*idx.shape, hidden] = scaled rows of `table` (bf16 for an e4m3 table, else the table's type)
 inline torch::Tensor lookup_rows(const torch::Tensor& table, const torch::Tensor& idx_in, double scale,
                                  const std::optional<torch::Tensor>& table_sf) {
@@ -93,8 +95,8 @@ inline torch::Tensor embedding_grad(const torch::Tensor& dy_in, const torch::Ten
     const auto [dy_begin, dy_end] = range(dy);
     const auto [out_begin, out_end] = range(out);
     EP_HOST_ASSERT_MSG(out_end <= dy_begin or dy_end <= out_begin or out_begin == out_end or dy_begin == dy_end, "out shares memory with dy");
-    constexpr int64_t kMost = std::numeric_limits<int>::max() / 2;
-    EP_HOST_ASSERT_MSG(idx.numel() <= kMost and out.size(0) <= kMost and out.size(1) <= kMost, "sizes above 2^30");
+    EP_HOST_ASSERT_MSG(idx.numel() <= kEmbMaxGradSize and out.size(0) <= kEmbMaxGradSize and out.size(1) <= kEmbMaxGradSize,
+                       "a gradient's rows, columns and tokens are below 2^30");
     const auto in_type = embedding_type(dy), out_type = embedding_type(out);
     EP_HOST_ASSERT(in_type != kernels::EmbType::kE4M3);
     const c10::cuda::CUDAGuard guard(dy.device());
@@ -157,6 +159,9 @@ public:
 inline torch::Tensor embedding_lookup(const torch::Tensor& table, const torch::Tensor& idx, double scale, const std::optional<torch::Tensor>& table_sf) {
     refuse_tangent(table);
     if (not at::GradMode::is_enabled() or not table.requires_grad() or table_sf.has_value()) return lookup_rows(table, idx, scale, table_sf);
+    check_rows(table);
+    EP_HOST_ASSERT_MSG(idx.numel() <= kEmbMaxGradSize and table.size(0) <= kEmbMaxGradSize and table.size(1) <= kEmbMaxGradSize,
+                       "a gradient's rows, columns and tokens are below 2^30");
     return EmbeddingLookup::apply(table, idx, scale);
 }
 

@@ -57,8 +57,8 @@ def embedding_lookup(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0,
     `table` is `[rows, hidden]` with contiguous columns (rows may lie further apart): bf16, fp16 or fp32, and the result has
     its type; or e4m3 with `table_sf`, fp32 `[rows, hidden / 128]` (the 1x128 scales of an FP8 entry table), and the result
     is bf16. `idx` is int64 or int32 of any shape. Products are taken in fp32 and rounded once. The gradient reaches `table`
-    (not an e4m3 one) in its own type, or its fp32 `main_grad`; a backward pass may be captured in a CUDA graph when no eager
-    autograd graph of the same table is alive.
+    (not an e4m3 one) in its own type, or its fp32 `main_grad`, for fewer than 2^30 rows, columns and tokens; a backward pass may
+    be captured in a CUDA graph when no eager autograd graph of the same table is alive.
     """
     if table.is_cuda:
         return _C.embedding_lookup(table, idx, scale, table_sf)          # (which looks at every argument, and is the autograd node)
