@@ -16,7 +16,7 @@
 //
 // Neither zeros nor a sum of two parts hide infinities or NaN (0 * inf = NaN, and so is hi * inf + lo * inf where lo is zero or of
 // the other sign). lora_gemm therefore takes them out of both operands of an adapter's block and adds their products, in fp32, to the
-// owner's rows; lora_wgrad overwrites the rows of other requests with zeros, and where the sum of hi's products is not finite that is
+// owner's rows (a NaN of t stays: its whole row of y is NaN); lora_wgrad overwrites the rows of other requests with zeros, and where the sum of hi's products is not finite that is
 // the result. One request cannot poison another, and its own results are infinite or NaN where the formulas say so, whoever
 // shares its tile.
 #pragma once
@@ -65,18 +65,21 @@ EP_DEVICE bool has_non_finite(const uint4& u) {
     return bad;
 }
 
-// v can be written as hi + lo with both bf16: not if it is infinite, NaN, or rounds to infinity
-EP_DEVICE bool splits(float v) { return isfinite(__bfloat162float(__float2bfloat16_rn(v))); }
-// v = hi + lo. What cannot be split has no lo, and with kTakeOut no hi either; true where there is such a value.
+// t that the writers keep from the tensor cores: infinite, or infinite once it is rounded to bf16
+EP_DEVICE bool taken_out(float t) { return isinf(__bfloat162float(__float2bfloat16_rn(t))); }
+// v = hi + lo, both bf16. What is not finite has no lo, and with kTakeOut an infinity no hi either; true where there is one.
 template <bool kTakeOut>
 EP_DEVICE bool split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     hi = ptx::float2_to_bf16x2(a, b);
     const float2 h = ptx::bf16x2_to_float2(hi);
     const float ra = a - h.x, rb = b - h.y;
-    const bool fa = isfinite(ra), fb = isfinite(rb);           // exactly where `splits` is true
-    lo = ptx::float2_to_bf16x2(fa ? ra : 0.0f, fb ? rb : 0.0f);
-    if (kTakeOut) hi &= (fa ? 0x0000ffffu : 0u) | (fb ? 0xffff0000u : 0u);
-    return not (fa and fb);
+    lo = ptx::float2_to_bf16x2(isfinite(ra) ? ra : 0.0f, isfinite(rb) ? rb : 0.0f);
+    if constexpr (kTakeOut) {
+        const bool ia = isinf(h.x), ib = isinf(h.y);
+        hi &= (ia ? 0u : 0x0000ffffu) | (ib ? 0u : 0xffff0000u);
+        return ia or ib;
+    }
+    return false;
 }
 // eight values -> one 16-byte unit each of hi and lo
 template <bool kTakeOut>
@@ -109,28 +112,43 @@ EP_DEVICE int ld_cluster_int(uint32_t addr) {
     return v;
 }
 
-// Products of a row's t and its adapter's V at column n that the writers have kept from the tensor cores: those of t that cannot be
-// split, and of units of eight V elements with an infinity or NaN
-__device__ __noinline__ float poisoned(const LoraGemmArgs& a, int row, int n) {
+// Adds to v the products of a row's t and its adapter's V at columns n .. n + 7 (n a multiple of eight) that the writers have kept from
+// the tensor cores: those of `taken_out` t, and of units of eight V elements with an infinity or NaN
+__device__ __noinline__ void add_poisoned(const LoraGemmArgs& a, int row, int n, float (&v)[8]) {
     const int e = adapter_of(a.rows, row);
-    if (e < 0) return 0.0f;
-    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
+    if (e < 0) return;
+    const __nv_bfloat16* base = reinterpret_cast<const __nv_bfloat16*>(a.v) + int64_t(e) * a.n * a.rows.rank;
     const float* t = a.t + int64_t(row) * a.rows.rank;
-    float sum = 0.0f;
-    if (a.mn_major) {
-        for (int r = 0; r < a.rows.rank; ++r) {
-            const __nv_bfloat16* unit = v + int64_t(r) * a.n + (n & ~7);
-            if (not splits(t[r]) or has_non_finite(*reinterpret_cast<const uint4*>(unit))) sum += t[r] * __bfloat162float(unit[n & 7]);
+    float sum[8] = {};
+    #pragma unroll 1
+    for (int r = 0; r < a.rows.rank; r += 8) {
+        float f[8];
+        load8(t + r, f);
+        unsigned out = 0;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) out |= unsigned(taken_out(f[i])) << i;
+        // unit i: rank column r + i of the eight columns (mn_major), or eight rank columns of column n + i
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint4 u = *reinterpret_cast<const uint4*>(a.mn_major ? base + int64_t(r + i) * a.n + n : base + int64_t(n + i) * a.rows.rank + r);
+            const unsigned which = has_non_finite(u) ? 0xffu : out;
+            if (which == 0) continue;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 g = ptx::bf16x2_to_float2(w[j / 2]);
+                const float value = j % 2 ? g.y : g.x;
+                if (a.mn_major and ((which >> i) & 1u)) sum[j] += f[i] * value;
+                if (not a.mn_major and ((which >> j) & 1u)) sum[i] += f[j] * value;
+            }
         }
-    } else {
-        for (int r = 0; r < a.rows.rank; r += 8) {
-            const __nv_bfloat16* unit = v + int64_t(n) * a.rows.rank + r;
-            const bool whole = has_non_finite(*reinterpret_cast<const uint4*>(unit));
-            for (int j = 0; j < 8; ++j)
-                if (whole or not splits(t[r + j])) sum += t[r + j] * __bfloat162float(unit[j]);
-        }
+        bool decided = true;                  // a NaN stays one (rows with several infinities get there at once)
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) decided = decided and isnan(sum[j]);
+        if (decided) break;
     }
-    return sum;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += sum[j];
 }
 
 // This row's t, 32 columns from 32 * c (zeros behind the rank). Asked for a block ahead of its use: a read of a K block's own would be
@@ -144,7 +162,7 @@ EP_DEVICE void read_t(const LoraGemmArgs& a, int row, bool there, int c, float (
     }
 }
 // A row's line of an A slot: bf16 hi in the first half, lo in the second (zeros for rows of others), 16-byte unit u of row r at u ^ (r % 8).
-// True where the row has a t that cannot be split, which is written as zero.
+// True where the row has a t that is taken out, which is written as zero.
 EP_DEVICE bool write_t(uint8_t* slot, int row, bool there, const float (&t)[4][8]) {
     uint8_t* line = slot + row * 128;
     bool found = false;
@@ -176,6 +194,11 @@ EP_DEVICE bool take_out_non_finite(uint8_t* block, bool mn_major, int thread) {
     return found;
 }
 
+EP_DEVICE void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(ptx::float2_to_bf16x2(v[0], v[1]), ptx::float2_to_bf16x2(v[2], v[3]),
+                                              ptx::float2_to_bf16x2(v[4], v[5]), ptx::float2_to_bf16x2(v[6], v[7]));
+}
+
 // Epilogue of one warp: its 32 rows of an accumulator of `columns` columns, rounded to bf16 and stored by the TMA through a 4 KB
 // buffer (what lies beyond the matrix is cut off by the store). `fix`: add what the tensor cores did not get.
 EP_DEVICE void store_tile(const CUtensorMap* map_y, const LoraGemmArgs& a, uint32_t taddr, uint8_t* buffer, int row0, int n0, int columns, bool fix, int lane) {
@@ -201,13 +224,15 @@ EP_DEVICE void store_tile(const CUtensorMap* map_y, const LoraGemmArgs& a, uint3
                 *reinterpret_cast<uint4*>(line + (((4 + u) ^ (lane & 7)) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
             }
         } else {
-            for (int j = 0; j < 64; ++j) {
-                const uint32_t r = tc::tmem_ld_32x1(taddr + c + j);
+            #pragma unroll 1
+            for (int u = 0; u < 8; ++u) {
+                float v[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(tc::tmem_ld_32x1(taddr + c + 8 * u + j));
                 tc::wait_ld();
-                float v = __uint_as_float(r);
-                if (row0 + lane < a.rows.num_rows and n0 + c + j < a.n) v += poisoned(a, row0 + lane, n0 + c + j);
+                if (row0 + lane < a.rows.num_rows and n0 + c + 8 * u < a.n) add_poisoned(a, row0 + lane, n0 + c + 8 * u, v);
                 __syncwarp();
-                *reinterpret_cast<__nv_bfloat16*>(line + (((j / 8) ^ (lane & 7)) << 4) + (j % 8) * 2) = __float2bfloat16_rn(v);
+                store8(reinterpret_cast<__nv_bfloat16*>(line + ((u ^ (lane & 7)) << 4)), v);
             }
         }
         ptx::fence_proxy_async_smem();
@@ -242,10 +267,6 @@ EP_DEVICE void add_parts(float (&v)[8], const uint8_t* parts, int part_bytes, in
         const float4 y = *reinterpret_cast<const float4*>(line + (((c / 4 + 1) ^ (row & 7)) << 4));
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
-}
-EP_DEVICE void store8(__nv_bfloat16* p, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(ptx::float2_to_bf16x2(v[0], v[1]), ptx::float2_to_bf16x2(v[2], v[3]),
-                                              ptx::float2_to_bf16x2(v[4], v[5]), ptx::float2_to_bf16x2(v[6], v[7]));
 }
 
 // One lane of a converged warp, always the same. The loops that feed the tensor cores are run by a whole warp and let this lane
@@ -836,8 +857,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             if (m0 + row >= a.rows.num_rows or n0 + c >= a.n) continue;
             float v[8] = {};
             add_parts(v, smem_out, share * BN * 4, cluster, (row % share) * BN * 4, c, row);
-            if (fix)
-                for (int j = 0; j < 8; ++j) v[j] += poisoned(a, m0 + row, n0 + c + j);
+            if (fix) add_poisoned(a, m0 + row, n0 + c, v);
             store8(reinterpret_cast<__nv_bfloat16*>(a.y) + int64_t(m0 + row) * a.n + n0 + c, v);
         }
         tc::cluster_sync();                   // nobody leaves while others look at its flag
